@@ -13,6 +13,9 @@
 
 #include "kernels.h"
 
+// Serving operators (serving_ops.cpp).
+void pra_bind_serving_ops(pybind11::module_& m);
+
 // Native cache-build planner (planner.cpp).
 pybind11::object pra_plan_batch(const pybind11::list& rows, const pybind11::object& tokenizer,
                                 const pybind11::dict& cfg);
@@ -1572,8 +1575,12 @@ torch::Tensor stack_train_backward(torch::Tensor dy, int64_t B, int64_t T, std::
   return dy;
 }
 
+// The attention kernels' status word of a device, for the serving operators.
+int* pra_attention_status_word(const torch::Device& dev) { return ptr<int>(attention_status_buffer(dev)); }
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "PRA sm_100a kernels";
+  pra_bind_serving_ops(m);
   m.def("attention_fwd", &attention_fwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("heads"),
         py::arg("kv_heads"), py::arg("head_dim"), py::arg("mem_k"), py::arg("mem_v"), py::arg("mem_idx"),
         py::arg("mem_len"), py::arg("key_valid"), py::arg("scale"), py::arg("drop_p") = 0.0,

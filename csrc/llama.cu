@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(DT) decode_tma_kernel(const __grid_constant__ 
   const bool local_only = p.mem_splits > 0 && split >= p.mem_splits;
   const bool mem_only = p.mem_splits > 0 && split < p.mem_splits;
   const int mem_len = (!local_only && p.mem_len) ? p.mem_len[b] : 0;
-  const int total = mem_len + ((!mem_only && p.loc_len) ? p.loc_len[b] : 0);
+  const int total = mem_len + ((!mem_only && p.loc_len) ? max(0, min(p.loc_len[b], p.loc_cap)) : 0);
   const int keys = mem_only && p.mem_split_keys > 0 ? p.mem_split_keys : p.split_keys;
   const int k0 = (local_only ? split - p.mem_splits : split) * keys, k1 = min(total, k0 + keys);
   const int64_t part = ((int64_t)b * p.H + kvh * G) * p.n_split + split;
@@ -483,6 +483,16 @@ __global__ void __launch_bounds__(DT) decode_tma_kernel(const __grid_constant__ 
     }
     __syncthreads();  // block `it` landed for every thread; every warp is done with block it - 1
     if (s_fail) break;
+    if (blk_mode[it] < 2 && k0 + (it + 1) * DBN > k1) {
+      // a copied box reaches past the last visible key: those value rows may hold anything, NaN
+      // too, and 0 * NaN is not 0
+      uint8_t* vt = stages + buf * Lay::STAGE + Lay::TILE;
+      const int seen = k1 - (k0 + it * DBN);
+      for (int c = seen * (D / 8) + threadIdx.x; c < DBN * (D / 8); c += DT)
+        *reinterpret_cast<uint4*>(vt + sw_off(c / (D / 8), (c % (D / 8)) * 8)) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();  // before a later copy into this stage
+      __syncthreads();
+    }
     if (it + TST - 1 < n_blocks) issue(it + TST - 1, (it + TST - 1) % TST);
     else cp_async_commit();
     const uint32_t kst = smem_u32(stages + buf * Lay::STAGE), vst = kst + Lay::TILE;
@@ -1188,7 +1198,8 @@ static cudaError_t launch_decode_tma(const DecodeAttnParams& p, cudaStream_t st)
                                                                !aligned(p.mem_v) || p.mem_rows <= 0)))
     return cudaErrorNotSupported;
   const int64_t width = (int64_t)p.Hkv * D;
-  const int64_t loc_rows = (int64_t)p.B * (p.loc_batch / p.loc_row);
+  // up to the last batch row's last cache row (the view may start inside its allocation)
+  const int64_t loc_rows = (int64_t)(p.B - 1) * (p.loc_batch / p.loc_row) + p.loc_cap;
   const CUtensorMap* lk = pra_tile_map_bf16(p.loc_k, width, loc_rows, p.loc_row, DBN);
   const CUtensorMap* lv = pra_tile_map_bf16(p.loc_v, width, loc_rows, p.loc_row, DBN);
   const CUtensorMap* mk = has_mem ? pra_tile_map_bf16(p.mem_k, width, p.mem_rows, p.mem_row, DBN) : lk;

@@ -1,0 +1,566 @@
+// Attention of a batch that shares a long prefix, on the 5th-generation tensor cores.
+//
+// For the query row i (batch row b, token t, head h) one softmax runs over the prefix keys, which are
+// the same for every row, and the row's own causal keys:
+//     s_ij = scale q_i . k_j,   o_i = sum_j e^{s_ij} v_j / sum_j e^{s_ij},   lse_i = log sum_j e^{s_ij}.
+// Attending row by row would read the prefix B times; here the B * T * H / Hkv query rows of one KV
+// head are the M dimension of S = Q K^T and O = P V, so each prefix key is read once per 256 of them.
+//
+// One CTA owns NT = 1 or 2 tiles of 128 query rows of one KV head and a range of 128-key blocks:
+//   * one thread brings K and V blocks in with TMA (128-byte swizzle) through a ring of R tiles;
+//   * one thread issues the MMAs: S_i = Q_i K^T (both operands in shared memory) and O_i += P_i V
+//     (P from TMEM), committing each to an mbarrier;
+//   * a warpgroup per tile does the softmax, one thread per query row (TMEM lane): the 128 scores of
+//     a block come into registers once, the running maximum is raised lazily (only when it grows by
+//     more than 2^8, then O is rescaled in TMEM), and P goes back over S's columns as bf16.
+// P shares S's columns, so S_{j+1} of a tile is issued only after P V_j of that tile has completed;
+// with two tiles the other tile's MMAs and softmax fill that gap.  P is rounded to bf16 (one half
+// step, 2^-8 relative, of each weight: the tensor cores take 16-bit operands); the row sums use the
+// unrounded weights, and S, O, maxima and sums stay in fp32.
+//
+// Keys past the ones any query of the CTA may see are never multiplied: their scores are replaced by
+// -inf, and their value rows are zeroed in shared memory (a stale row may hold NaN, and 0 * NaN is
+// not 0).  Every wait is bounded; a CTA that times out sets *status, waits (bounded) for its copies
+// and MMAs in flight, frees its TMEM and returns.
+#include <algorithm>
+
+#include "serving.h"
+#include "tcgen05.cuh"
+
+namespace pra {
+namespace prefix {
+
+constexpr int BM = 128;  // query rows of a tile
+constexpr int BN = 128;  // keys of a block
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_LOG2 = 8.f;
+constexpr long long WAIT_CYCLES = 4000000000LL;
+
+template <int D, int NT>
+struct Cfg {
+  static constexpr int BOXES = D / 64;
+  static constexpr int BOX = BN * 128;        // 128 rows x 64 columns
+  static constexpr int TILE = BOXES * BOX;    // one K, V or Q tile
+  static constexpr int R = NT == 2 ? (D == 128 ? 4 : 6) : (D == 128 ? 2 : 4);
+  static constexpr int THREADS = NT * 128 + 64;
+  static constexpr int OFF_RING = NT * TILE;
+  static constexpr int OFF_BAR = OFF_RING + R * TILE;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment slack
+  static constexpr int O_COL = NT * BN;               // TMEM: S / P of tile i at i * BN, O at O_COL + i * D
+  static constexpr uint32_t COLS = NT == 2 ? 512 : 256;
+  static constexpr int CTAS = NT == 2 ? 1 : 2;        // per SM
+  static_assert(O_COL + NT * D <= (int)COLS, "TMEM");
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Swizzled shared-memory descriptors (128-byte rows, 8-row groups of 1,024 bytes).  K-major: the
+// stride offset is the next 8 rows; MN-major: it is the next 8 K rows, and the leading offset the
+// next 64 columns.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead) {
+  uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((lead >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// Bounded wait that also ends when another role of the CTA has given up.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (mbar_try_wait_parity(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait_parity(bar, parity)) {
+    if (*abort || clock64() - t0 > WAIT_CYCLES) {
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// What a CTA works on, computed alike by every thread.
+struct Item {
+  int kvh, b;             // KV head; batch row (-1: packed)
+  int row0, rows;         // first query row of the CTA, query rows of the whole row space
+  int prefix_seen;        // prefix keys any of the CTA's queries may see
+  int own_seen;           // own keys any of them may see
+  int prefix_blocks;      // blocks [0, prefix_blocks) are prefix, the rest own
+  int lo, hi;             // blocks of this split
+};
+
+template <int NT>
+__device__ __forceinline__ Item item_of(const PrefixAttnArgs& a, int seen) {
+  Item it;
+  const int G = a.H / a.Hkv;
+  it.rows = (a.packed ? a.B : 1) * a.T * G;
+  const int tiles = (it.rows + NT * BM - 1) / (NT * BM);
+  int x = blockIdx.x;
+  it.row0 = (x % tiles) * NT * BM;
+  x /= tiles;
+  it.kvh = x % a.Hkv;
+  it.b = a.packed ? -1 : x / a.Hkv;
+  it.prefix_seen = a.use_prefix ? seen : 0;
+  it.own_seen = 0;
+  if (a.use_own) {  // the CTA's last query sees the most
+    const int len = max(0, min(a.len[it.b], a.cap));
+    const int t = min(it.row0 + NT * BM, it.rows) - 1;
+    it.own_seen = max(0, len - a.T + t / G + 1);
+  }
+  it.prefix_blocks = (it.prefix_seen + BN - 1) / BN;
+  const int n = it.prefix_blocks + (it.own_seen + BN - 1) / BN;
+  it.lo = (int)((int64_t)n * blockIdx.y / a.splits);
+  it.hi = (int)((int64_t)n * (blockIdx.y + 1) / a.splits);
+  return it;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
+    prefix_kernel(const __grid_constant__ CUtensorMap map_pk, const __grid_constant__ CUtensorMap map_pv,
+                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const PrefixAttnArgs a) {
+  using C = Cfg<D, NT>;
+  constexpr int R = C::R;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [R] a ring tile has landed
+  uint64_t* empty = full + R;                                        // [R] a ring tile has been read
+  uint64_t* s_full = empty + R;                                      // [NT] S_i is in TMEM
+  uint64_t* p_full = s_full + NT;                                    // [NT] P_i is in TMEM
+  uint64_t* o_full = p_full + NT;                                    // [NT] O_i has P_i V
+  uint64_t* q_full = o_full + NT;                                    // [NT] Q_i is in shared memory
+  uint64_t* drain = q_full + NT;                                     // [1] every MMA issued has completed
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ int s_seen;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.H / a.Hkv;
+  if (tid == 0) {
+    for (int i = 0; i < R; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < NT; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+      mbar_init(o_full + i, 1);
+      mbar_init(q_full + i, 128);
+    }
+    mbar_init(drain, 1);
+    s_abort = 0;
+    s_seen = 0;
+    tc::fence_mbarrier_init();
+  }
+  if (warp == NT * 4) {
+    tc::alloc(&s_tmem, C::COLS);
+    tc::relinquish();
+  }
+  __syncthreads();
+  // the prefix keys any query row of this CTA may see
+  {
+    const int rows = (a.packed ? a.B : 1) * a.T * G;
+    const int tiles = (rows + NT * BM - 1) / (NT * BM);
+    const int row0 = (blockIdx.x % tiles) * NT * BM, b1 = blockIdx.x / (tiles * a.Hkv);
+    int seen = 0;
+    if (!a.use_prefix) seen = 0;
+    else if (a.prefix_len == nullptr) seen = a.P;
+    else if (!a.packed) seen = max(0, min(a.prefix_len[b1], a.P));
+    else {
+      const int b_lo = row0 / (a.T * G), b_hi = (min(rows, row0 + NT * BM) - 1) / (a.T * G);
+      for (int b = b_lo + tid; b <= b_hi; b += C::THREADS) seen = max(seen, min(a.prefix_len[b], a.P));
+    }
+    if (seen > 0) atomicMax(&s_seen, seen);
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const Item it = item_of<NT>(a, s_seen);
+  const uint32_t tmem = s_tmem;
+  const uint32_t ring = smem_u32(smem + C::OFF_RING);
+  const int n = it.hi - it.lo;
+  int issued = 0;  // ring tiles requested (the producer's count)
+  // rows of the block that some query of the CTA may see
+  auto block_seen = [&](int j) {
+    return j < it.prefix_blocks ? it.prefix_seen - j * BN : it.own_seen - (j - it.prefix_blocks) * BN;
+  };
+
+  if (warp == NT * 4) {
+    // ---------------------------------------------------------------- K / V producer
+    if (lane == 0 && n > 0) {
+      for (int j = it.lo; j < it.hi && !s_abort; ++j) {
+        const bool own = j >= it.prefix_blocks;
+        const int y = (own ? j - it.prefix_blocks : j) * BN, z = own ? it.b : 0;
+        bool ok = true;
+        for (int kv = 0; kv < 2 && ok; ++kv) {
+          const int r = issued % R;
+          if (issued >= R) ok = wait(empty + r, (uint32_t)((issued / R - 1) & 1), &s_abort);
+          if (!ok) break;
+          const CUtensorMap* map = kv == 0 ? (own ? &map_k : &map_pk) : (own ? &map_v : &map_pv);
+          expect_tx(full + r, C::TILE);
+#pragma unroll
+          for (int x = 0; x < C::BOXES; ++x)
+            tma_load3(ring + r * C::TILE + x * C::BOX, map, it.kvh * D + x * 64, y, z, full + r);
+          ++issued;
+        }
+        if (!ok) break;
+      }
+    }
+  } else if (warp == NT * 4 + 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    constexpr uint32_t ID_S = tc::idesc_bf16(BM, BN, false);
+    constexpr uint32_t ID_O = tc::idesc_bf16(BM, D, true);
+    const uint32_t q_addr = smem_u32(smem);
+    auto issue_s = [&](int i, int r) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = (kk / 4) * C::BOX + (kk % 4) * 32;
+        tc::mma_bf16(tmem + i * BN, desc_sw128(q_addr + i * C::TILE + off, 16),
+                     desc_sw128(ring + r * C::TILE + off, 16), ID_S, kk > 0);
+      }
+    };
+    auto issue_o = [&](int i, int r, bool acc) {
+#pragma unroll
+      for (int kk = 0; kk < BN / 16; ++kk)
+        tc::mma_bf16_ts(tmem + C::O_COL + i * D, tmem + i * BN + kk * 8,
+                        desc_sw128(ring + r * C::TILE + kk * 2048, C::BOX), ID_O, (acc || kk > 0) ? 1u : 0u);
+    };
+    if (lane == 0 && n > 0) {
+      bool ok = wait(full, 0, &s_abort);
+      tc::fence_after();
+      if (ok) {
+        for (int i = 0; i < NT && ok; ++i) {
+          ok = wait(q_full + i, 0, &s_abort);
+          if (!ok) break;
+          issue_s(i, 0);
+          tc::commit(s_full + i);
+        }
+        if (ok && R < 2 * n) tc::commit(empty);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int vt = 2 * j + 1, kt = 2 * j + 2;  // ring positions of V_j and K_{j+1}
+        const bool more = j + 1 < n;
+        for (int i = 0; i < NT && ok; ++i) {
+          ok = ok && wait(p_full + i, (uint32_t)(j & 1), &s_abort);
+          if (i == 0) ok = ok && wait(full + vt % R, (uint32_t)((vt / R) & 1), &s_abort);
+          if (!ok) break;
+          tc::fence_after();
+          issue_o(i, vt % R, j > 0);
+          if (i == NT - 1 && vt + R < 2 * n) tc::commit(empty + vt % R);  // only tiles that are refilled
+          tc::commit(o_full + i);
+          if (more) {
+            // P_i V_j reads the columns that S_i is about to overwrite
+            ok = ok && wait(o_full + i, (uint32_t)(j & 1), &s_abort);
+            if (i == 0) ok = ok && wait(full + kt % R, (uint32_t)((kt / R) & 1), &s_abort);
+            if (!ok) break;
+            tc::fence_after();
+            issue_s(i, kt % R);
+            if (i == NT - 1 && kt + R < 2 * n) tc::commit(empty + kt % R);
+            tc::commit(s_full + i);
+          }
+        }
+      }
+      if (!ok) {
+        tc::commit(drain);
+        tc::mbar_wait_cycles(drain, 0, WAIT_CYCLES);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int i = warp >> 2, row = tid & (BM - 1);
+    const int qr = it.row0 + i * BM + row;
+    const bool live = qr < it.rows;
+    const int TG = a.T * G;
+    const int b = it.b >= 0 ? it.b : min(qr / TG, a.B - 1);
+    const int t = (qr / G) % a.T, h = it.kvh * G + qr % G;
+    // this tile's queries into shared memory (rows past the last: zero)
+    for (int e = row; e < BM * (D / 8); e += BM) {
+      const int r = e / (D / 8), c = e % (D / 8), x = it.row0 + i * BM + r;
+      uint4 val = make_uint4(0, 0, 0, 0);
+      if (x < it.rows) {
+        const int xb = it.b >= 0 ? it.b : x / TG;
+        val = *reinterpret_cast<const uint4*>(a.q + xb * a.q_batch + (int64_t)((x / G) % a.T) * a.q_token +
+                                              (int64_t)(it.kvh * G + x % G) * D + c * 8);
+      }
+      *reinterpret_cast<uint4*>(smem + i * C::TILE + (c / 8) * C::BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = val;
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_full + i);
+    const int prefix_lim = !live ? 0 : a.prefix_len ? max(0, min(a.prefix_len[b], a.P)) : a.P;
+    int own_lim = 0;
+    if (live && a.use_own) own_lim = max(0, min(max(a.len[b], 0), a.cap) - a.T + t + 1);
+    const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + t_lane + i * BN, t_o = tmem + t_lane + C::O_COL + i * D;
+    const float sl2 = a.scale * LOG2E;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int blk = it.lo + j;
+      const bool own = blk >= it.prefix_blocks;
+      const int lim = own ? own_lim - (blk - it.prefix_blocks) * BN : prefix_lim - blk * BN;
+      ok = wait(s_full + i, (uint32_t)(j & 1), &s_abort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc::fence_after();
+      float s[BN];
+      {
+        uint32_t r[64];
+        tc::ld64(t_s, r);
+#pragma unroll
+        for (int c = 0; c < 64; ++c) s[c] = __uint_as_float(r[c]);
+        tc::ld64(t_s + 64, r);
+#pragma unroll
+        for (int c = 0; c < 64; ++c) s[64 + c] = __uint_as_float(r[c]);
+      }
+      if (__any_sync(0xffffffffu, lim < BN)) {
+#pragma unroll
+        for (int c = 0; c < BN; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < BN; ++c) mx = fmaxf(mx, s[c]);
+      // raised lazily; the first maximum costs no rescaling (O has not been written: P V of the
+      // first block overwrites it, and rows that saw nothing so far hold zeros)
+      float corr = 1.f;
+      bool rescale = false;
+      if (mx > m_run) {
+        if (m_run == -INFINITY) {
+          m_run = mx;
+        } else if ((mx - m_run) * sl2 > RESCALE_LOG2) {
+          corr = ex2((m_run - mx) * sl2);
+          l_run *= corr;
+          m_run = mx;
+          rescale = true;
+        }
+      }
+      if (j > 0 && __any_sync(0xffffffffu, rescale)) {  // P V_{j-1} has completed: S_j was issued after it
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t r[32];
+          tc::ld32(t_o + c0, r);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * corr);
+          tc::st32(t_o + c0, r);
+        }
+      }
+      const float ms = m_run == -INFINITY ? 0.f : m_run * sl2;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int c0 = 0; c0 < BN; c0 += 64) {
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float p0 = ex2(fmaf(s[c0 + 2 * c], sl2, -ms)), p1 = ex2(fmaf(s[c0 + 2 * c + 1], sl2, -ms));
+          sum0 += p0;
+          sum1 += p1;
+          w[c] = pack_bf16(p0, p1);
+        }
+        tc::st32(t_s + c0 / 2, w);
+      }
+      l_run += sum0 + sum1;
+      const int seen = block_seen(blk);
+      if (i == 0 && seen < BN) {  // value rows that no query of the CTA sees: zero
+        const int vt = 2 * j + 1;
+        ok = wait(full + vt % R, (uint32_t)((vt / R) & 1), &s_abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* v = smem + C::OFF_RING + (vt % R) * C::TILE;
+        for (int e = seen * (D / 8) + row; e < BN * (D / 8); e += BM) {
+          const int r = e / (D / 8), c = e % (D / 8);
+          *reinterpret_cast<uint4*>(v + (c / 8) * C::BOX + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      tc::fence_before();
+      mbar_arrive(p_full + i);
+    }
+    if (ok && n > 0) {
+      ok = wait(o_full + i, (uint32_t)((n - 1) & 1), &s_abort);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok) {
+      tc::fence_after();
+      const bool any = m_run != -INFINITY;  // else nothing of this range is visible to the row
+      const int64_t bt = (int64_t)b * a.T + t;
+      if (a.part_o != nullptr) {
+        const int64_t at = (bt * a.H + h) * a.n_slots + a.slot0 + blockIdx.y;
+        if (live) {
+          a.part_ml[2 * at] = any ? m_run * a.scale : -INFINITY;
+          a.part_ml[2 * at + 1] = l_run;
+        }
+        if (n > 0) {
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t r[32];
+            tc::ld32(t_o + c0, r);
+            if (live && any) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 4)
+                *reinterpret_cast<uint4*>(a.part_o + at * D + c0 + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
+            }
+          }
+        }
+      } else {
+        const float inv = any ? 1.f / l_run : 0.f;
+        __nv_bfloat16* dst = a.out + (bt * a.H + h) * D;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t r[32];
+          if (n > 0) tc::ld32(t_o + c0, r);
+          if (live) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = any ? pack_bf16(__uint_as_float(r[c + 2 * e]) * inv, __uint_as_float(r[c + 2 * e + 1]) * inv) : 0u;
+              *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (live && a.lse != nullptr)
+          a.lse[((int64_t)b * a.H + h) * a.T + t] = any ? m_run * a.scale + logf(l_run) : -INFINITY;
+      }
+    }
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  if (s_abort) {  // nothing may land in shared memory after the CTA has gone: wait for the copies in flight
+    if (tid == 0 && a.status != nullptr) atomicExch(a.status, 1);
+    for (int x = max(0, issued - R); x < issued; ++x)
+      tc::mbar_wait_cycles(full + x % R, (uint32_t)((x / R) & 1), WAIT_CYCLES);
+    __syncthreads();
+  }
+  if (warp == NT * 4) {
+    tc::fence_after();
+    tc::dealloc(tmem, C::COLS);
+  }
+}
+
+// One warp per (b, t, h): the partials weighted by their own maxima and summed in slot order.
+constexpr int MERGE_WARPS = 8;
+template <int D>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(PrefixMergeArgs a) {
+  constexpr int E = D / 32;
+  const int64_t at = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (at >= (int64_t)a.B * a.T * a.H) return;
+  const float* ml = a.part_ml + at * a.n_slots * 2;
+  const float* po = a.part_o + at * a.n_slots * D + lane * E;
+  float M = -INFINITY;
+  for (int s = lane; s < a.n_slots; s += 32) M = fmaxf(M, ml[2 * s]);
+  M = warp_max(M);
+  float L = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s = 0; s < a.n_slots; ++s) {
+    const float m = ml[2 * s];
+    if (m == -INFINITY) continue;  // nothing visible: its part of the workspace was not written
+    const float w = exp2f((m - M) * LOG2E);
+    L += w * ml[2 * s + 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += w * po[s * D + e];
+  }
+  const bool any = M != -INFINITY;
+  const float inv = any ? 1.f / L : 0.f;
+  if (a.out != nullptr) {
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) w[e / 2] = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + at * D + lane * E);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) dst[e] = w[e];
+  }
+  if (a.lse != nullptr && lane == 0) {
+    const int64_t bt = at / a.H;
+    const int h = (int)(at - bt * a.H);
+    a.lse[((bt / a.T) * a.H + h) * a.T + bt % a.T] = any ? M + logf(L) : -INFINITY;
+  }
+}
+
+bool encode(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t row, int64_t batches, int64_t batch) {
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batches};
+  const cuuint64_t strides[2] = {(cuuint64_t)row * 2, (cuuint64_t)batch * 2};
+  const cuuint32_t box[3] = {64, BN, 1}, elem[3] = {1, 1, 1};
+  return cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+                                elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int rows_of(const PrefixAttnArgs& a) { return (a.packed ? a.B : 1) * a.T * (a.H / a.Hkv); }
+
+template <int D, int NT>
+cudaError_t launch(const PrefixAttnArgs& a, cudaStream_t st) {
+  using C = Cfg<D, NT>;
+  CUtensorMap pk, pv, k, v;
+  const int64_t width = (int64_t)a.Hkv * D;
+  bool ok = true;
+  if (a.use_prefix)
+    ok = encode(&pk, a.pk, width, a.P, a.pk_row, 1, a.pk_row * a.P) && encode(&pv, a.pv, width, a.P, a.pv_row, 1, a.pv_row * a.P);
+  if (a.use_own)
+    ok = ok && encode(&k, a.k, width, a.cap, a.k_row, a.B, a.k_batch) && encode(&v, a.v, width, a.cap, a.v_row, a.B, a.v_batch);
+  if (!ok) return cudaErrorInvalidValue;
+  if (!a.use_prefix) pk = k, pv = v;
+  if (!a.use_own) k = pk, v = pv;
+  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(prefix_kernel<D, NT>), C::SMEM));
+  const int tiles = (rows_of(a) + NT * BM - 1) / (NT * BM);
+  const int64_t items = (int64_t)tiles * a.Hkv * (a.packed ? 1 : a.B);
+  if (items > INT32_MAX || a.splits > 65535) return cudaErrorInvalidValue;
+  prefix_kernel<D, NT><<<dim3((unsigned)items, a.splits), C::THREADS, C::SMEM, st>>>(pk, pv, k, v, a);
+  return cudaGetLastError();
+}
+
+// Two tiles per CTA read every key block once for 256 queries; one tile leaves room for two CTAs per SM.
+int tiles_per_cta(const PrefixAttnArgs& a) { return rows_of(a) > BM ? 2 : 1; }
+
+}  // namespace prefix
+}  // namespace pra
+
+void pra_prefix_attention_shape(const PrefixAttnArgs& a, int* tiles, int* slots) {
+  using namespace pra::prefix;
+  const int nt = tiles_per_cta(a);
+  *tiles = (rows_of(a) + nt * BM - 1) / (nt * BM) * a.Hkv * (a.packed ? 1 : a.B);
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  *slots = sms * (nt == 2 ? 1 : 2);
+}
+
+cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t st) {
+  using namespace pra::prefix;
+  if (a.B == 0 || a.T == 0) return cudaSuccess;
+  if ((!a.use_prefix && !a.use_own) || (a.packed && a.use_own) || a.H % a.Hkv || a.splits < 1) return cudaErrorInvalidValue;
+  const int nt = tiles_per_cta(a);
+  if (a.D == 128) return nt == 2 ? launch<128, 2>(a, st) : launch<128, 1>(a, st);
+  if (a.D == 64) return nt == 2 ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t pra_prefix_merge(const PrefixMergeArgs& a, cudaStream_t st) {
+  using namespace pra::prefix;
+  const int64_t rows = (int64_t)a.B * a.T * a.H;
+  if (rows == 0) return cudaSuccess;
+  const int64_t blocks = (rows + MERGE_WARPS - 1) / MERGE_WARPS;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  if (a.D == 128) merge_kernel<128><<<(unsigned)blocks, MERGE_WARPS * 32, 0, st>>>(a);
+  else if (a.D == 64) merge_kernel<64><<<(unsigned)blocks, MERGE_WARPS * 32, 0, st>>>(a);
+  else return cudaErrorInvalidValue;
+  return cudaGetLastError();
+}

@@ -1,0 +1,204 @@
+// Rotary positions for queries and keys, forward and backward, in one launch.
+//
+// Pair i of a head is (x[i], x[i + R/2]) in the half layout and (x[2i], x[2i + 1]) in the
+// interleaved one, for i < R/2 with R the rotated part of the head; with c, s the table's cosine
+// and sine of (position, i)
+//     y0 = x0 c - x1 s,    y1 = x1 c + x0 s,
+// and the elements behind R pass through.  The map is linear and a table entry may carry a scale
+// (m cos, m sin), so its transpose, the backward pass, is the same kernel with -s.  Products and
+// sums are fp32 with one rounding to the output type.
+//
+// Bound by bytes: x is read and y written once, the table adds 4 R bytes per token.  A thread owns
+// one unit (V pairs: two 16-byte vectors, at u V and R/2 + u V or side by side) of one token and
+// walks the heads with it, so a unit's cosines and sines are read once for several heads and all
+// loads of HPT heads are in flight together.  Vectors need R and D - R to be multiples of 2 V
+// and 16-byte aligned rows; other calls take V = 2 or 1.
+#include "common.cuh"
+#include "serving.h"
+
+#include <cuda_fp16.h>
+
+namespace pra {
+namespace rotary {
+
+constexpr int NT = 256;
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16(v); }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+template <typename T, int V, int HPT>
+__global__ void __launch_bounds__(NT) rotary_kernel(const RotaryArgs a, int units, int unit_lanes, int head_lanes,
+                                                    int tokens_per_block) {
+  const int per = unit_lanes * head_lanes;
+  const int lt = threadIdx.x / per;
+  const int64_t m = (int64_t)blockIdx.x * tokens_per_block + lt;
+  if (lt >= tokens_per_block || m >= a.tokens) return;
+  const int rem = threadIdx.x - lt * per;
+  const int hl = rem / unit_lanes;
+  const int half = a.rot / 2, rot_units = half / V;
+  const int heads = a.seg[0].heads + a.seg[1].heads + a.seg[2].heads;
+  const int64_t pos = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[m] : reinterpret_cast<const int*>(a.pos)[m];
+  const bool pos_ok = pos >= 0 && pos < a.max_pos;  // outside the table: the rotated part becomes NaN
+  int64_t slot = m;
+  if (a.slots != nullptr) slot = a.slots[m];
+  const bool slot_ok = a.slots == nullptr || (slot >= 0 && slot < a.slot_rows);
+  for (int u = rem - hl * unit_lanes; u < units; u += unit_lanes) {
+    const bool turns = u < rot_units;
+    int o0, o1;
+    if (!turns) {
+      o0 = a.rot + (u - rot_units) * 2 * V;
+      o1 = o0 + V;
+    } else if (a.interleaved) {
+      o0 = u * 2 * V;
+      o1 = o0 + V;
+    } else {
+      o0 = u * V;
+      o1 = half + u * V;
+    }
+    float c[V], s[V];
+    if (turns) {
+      if (pos_ok) {
+        const Vec<float, V < 4 ? V : 4>* ct =
+            reinterpret_cast<const Vec<float, V < 4 ? V : 4>*>(a.cos_t + pos * half + u * V);
+        const Vec<float, V < 4 ? V : 4>* st =
+            reinterpret_cast<const Vec<float, V < 4 ? V : 4>*>(a.sin_t + pos * half + u * V);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[j] = ct[j / 4].v[j % 4];
+          s[j] = st[j / 4].v[j % 4];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] = s[j] = __int_as_float(0x7fffffff);
+      }
+      if (a.inverse) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = -s[j];
+      }
+    }
+    for (int h0 = hl; h0 < heads; h0 += HPT * head_lanes) {
+      Vec<T, V> x0[HPT], x1[HPT];
+      T* dst[HPT];
+      bool live[HPT], rotate[HPT];
+#pragma unroll
+      for (int j = 0; j < HPT; ++j) {
+        int h = h0 + j * head_lanes, g = 0;
+        live[j] = h < heads;
+        if (!live[j]) continue;
+        if (h >= a.seg[0].heads) {
+          h -= a.seg[0].heads;
+          g = 1;
+          if (h >= a.seg[1].heads) {
+            h -= a.seg[1].heads;
+            g = 2;
+          }
+        }
+        const RotarySegment& q = a.seg[g];
+        rotate[j] = turns && q.rotate;
+        const T* src = reinterpret_cast<const T*>(q.src) + m * q.src_token + h * q.src_head;
+        dst[j] = reinterpret_cast<T*>(q.dst) + (q.to_slot ? slot : m) * q.dst_token + h * q.dst_head;
+        live[j] = !q.to_slot || slot_ok;
+        if (!live[j]) continue;
+        x0[j] = *reinterpret_cast<const Vec<T, V>*>(src + o0);
+        x1[j] = *reinterpret_cast<const Vec<T, V>*>(src + o1);
+      }
+#pragma unroll
+      for (int j = 0; j < HPT; ++j) {
+        if (!live[j]) continue;
+        if (rotate[j]) {
+          if (a.interleaved) {
+            // pair i of the unit is elements (2i, 2i + 1) of the two vectors side by side
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              T& e0 = 2 * i < V ? x0[j].v[(2 * i) % V] : x1[j].v[(2 * i) % V];
+              T& e1 = 2 * i + 1 < V ? x0[j].v[(2 * i + 1) % V] : x1[j].v[(2 * i + 1) % V];
+              const float p0 = to_f(e0), p1 = to_f(e1);
+              e0 = from_f<T>(p0 * c[i] - p1 * s[i]);
+              e1 = from_f<T>(p1 * c[i] + p0 * s[i]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float p0 = to_f(x0[j].v[i]), p1 = to_f(x1[j].v[i]);
+              x0[j].v[i] = from_f<T>(p0 * c[i] - p1 * s[i]);
+              x1[j].v[i] = from_f<T>(p1 * c[i] + p0 * s[i]);
+            }
+          }
+        }
+        *reinterpret_cast<Vec<T, V>*>(dst[j] + o0) = x0[j];
+        *reinterpret_cast<Vec<T, V>*>(dst[j] + o1) = x1[j];
+      }
+    }
+  }
+}
+
+template <typename T, int V>
+cudaError_t launch(const RotaryArgs& a, cudaStream_t st) {
+  const int heads = a.seg[0].heads + a.seg[1].heads + a.seg[2].heads;
+  const int units = a.head_dim / (2 * V);
+  const int unit_lanes = std::min(units, NT);
+  // one head per thread spreads a small call over more threads; four keep more loads in flight
+  const bool small = a.tokens * (int64_t)units * heads < (int64_t)148 * 2048 * 4;
+  const int hpt = small ? 1 : 4;
+  const int head_lanes = std::max(1, std::min((heads + hpt - 1) / hpt, NT / unit_lanes));
+  const int tpb = std::max(1, NT / (unit_lanes * head_lanes));
+  const int64_t blocks = (a.tokens + tpb - 1) / tpb;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  if (small) rotary_kernel<T, V, 1><<<(unsigned)blocks, NT, 0, st>>>(a, units, unit_lanes, head_lanes, tpb);
+  else rotary_kernel<T, V, 4><<<(unsigned)blocks, NT, 0, st>>>(a, units, unit_lanes, head_lanes, tpb);
+  return cudaGetLastError();
+}
+
+// The widest vector that the rotated part, the rest of the head and every row's alignment allow.
+template <typename T, int V>
+bool fits(const RotaryArgs& a) {
+  if (a.rot % (2 * V) || (a.head_dim - a.rot) % (2 * V)) return false;
+  const uintptr_t bytes = V * sizeof(T), table = std::min(V, 4) * 4;
+  if (reinterpret_cast<uintptr_t>(a.cos_t) % table || reinterpret_cast<uintptr_t>(a.sin_t) % table) return false;
+  for (const RotarySegment& s : a.seg) {
+    if (s.heads == 0) continue;
+    if (reinterpret_cast<uintptr_t>(s.src) % bytes || reinterpret_cast<uintptr_t>(s.dst) % bytes) return false;
+    if (s.src_token % V || s.src_head % V || s.dst_token % V || s.dst_head % V) return false;
+  }
+  return true;
+}
+
+template <typename T>
+cudaError_t dispatch(const RotaryArgs& a, cudaStream_t st) {
+  constexpr int W = 16 / sizeof(T);
+  if (fits<T, W>(a)) return launch<T, W>(a, st);
+  if (fits<T, 2>(a)) return launch<T, 2>(a, st);
+  return launch<T, 1>(a, st);
+}
+
+}  // namespace rotary
+}  // namespace pra
+
+cudaError_t pra_rotary(const RotaryArgs& a, int dtype, cudaStream_t st) {
+  if (a.tokens == 0) return cudaSuccess;
+  switch (dtype) {
+    case PRA_BF16: return pra::rotary::dispatch<__nv_bfloat16>(a, st);
+    case PRA_FP16: return pra::rotary::dispatch<__half>(a, st);
+    case PRA_FP32: return pra::rotary::dispatch<float>(a, st);
+    default: return cudaErrorInvalidValue;
+  }
+}

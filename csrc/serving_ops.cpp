@@ -1,0 +1,458 @@
+// Python bindings of the serving operators: rotary positions, attention over a shared prefix, rules
+// on logits.  Arguments are checked here; outputs and workspaces come from the caching allocator on
+// the current stream, per call, so calls on several streams or in several captured graphs share none.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "kernels.h"
+#include "serving.h"
+
+int* pra_attention_status_word(const torch::Device& dev);
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<torch::Tensor>;
+
+// Numbers in error messages (streaming an integer goes through the process's locale facets, which
+// another library's copy of the C++ runtime can leave unusable).
+std::string num(int64_t v) { return std::to_string(v); }
+
+inline cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+void check(cudaError_t e, const char* what) {
+  TORCH_CHECK(e == cudaSuccess, "pra_ops.", what, " failed: ", cudaGetErrorString(e));
+}
+
+int dtype_code(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return PRA_BF16;
+    case at::kHalf: return PRA_FP16;
+    case at::kFloat: return PRA_FP32;
+    default: break;
+  }
+  TORCH_CHECK(false, name, " has dtype ", t.scalar_type(), ", expected bf16, fp16 or fp32");
+  return -1;
+}
+
+// A tensor of the call: on the device of the first one.
+void same(const Tensor& t, const Tensor& first, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == first.device(), name, " must be on ", first.device(), ", it is on ", t.device());
+}
+
+void typed(const Tensor& t, at::ScalarType dt, const Tensor& first, const char* name) {
+  same(t, first, name);
+  TORCH_CHECK(t.scalar_type() == dt, name, " has dtype ", t.scalar_type(), ", expected ", dt);
+}
+
+// A contiguous vector with one entry per row.
+template <typename T>
+const T* per_row(const OptTensor& t, at::ScalarType dt, const Tensor& first, int64_t rows, const char* name) {
+  if (!t.has_value()) return nullptr;
+  typed(*t, dt, first, name);
+  TORCH_CHECK(t->dim() == 1 && t->size(0) == rows && t->is_contiguous(), name, " must be a contiguous vector of ", num(rows),
+              " entries");
+  return static_cast<const T*>(t->data_ptr());
+}
+
+// ---------------------------------------------------------------- rotary
+void rotary_tables(RotaryArgs& a, const Tensor& cos_t, const Tensor& sin_t, const Tensor& first, int64_t head_dim,
+                   bool interleaved) {
+  typed(cos_t, at::kFloat, first, "cos");
+  typed(sin_t, at::kFloat, first, "sin");
+  TORCH_CHECK(cos_t.dim() == 2 && cos_t.is_contiguous() && sin_t.is_contiguous() && cos_t.sizes() == sin_t.sizes(),
+              "cos and sin must be contiguous [positions, rotary_dim / 2] tables of one shape");
+  a.cos_t = cos_t.data_ptr<float>();
+  a.sin_t = sin_t.data_ptr<float>();
+  a.max_pos = cos_t.size(0);
+  a.rot = (int)(2 * cos_t.size(1));
+  TORCH_CHECK(head_dim > 0 && head_dim % 2 == 0 && head_dim <= 4096, "head_dim must be even and at most 4096");
+  TORCH_CHECK(a.rot >= 2 && a.rot <= head_dim, "the table rotates ", num(a.rot), " elements of a head of ",
+              num(head_dim));
+  a.head_dim = (int)head_dim;
+  a.interleaved = interleaved;
+}
+
+void rotary_positions(RotaryArgs& a, const Tensor& positions, const Tensor& first) {
+  same(positions, first, "positions");
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+              "positions must be int32 or int64");
+  TORCH_CHECK(positions.is_contiguous(), "positions must be contiguous");
+  a.pos = positions.data_ptr();
+  a.pos64 = positions.scalar_type() == at::kLong;
+}
+
+// The segment of x [..., heads, head_dim] (read in place where its tokens have one stride) and its new output.
+Tensor rotary_segment(RotarySegment& s, Tensor& x, int64_t head_dim) {
+  TORCH_CHECK(x.dim() >= 2 && x.size(-1) == head_dim, "queries and keys must be [..., heads, head_dim] of one head_dim");
+  auto out = torch::empty(x.sizes(), x.options());
+  const int64_t heads = x.size(-2);
+  TORCH_CHECK(heads <= 4096, "at most 4096 heads");
+  bool strided = x.stride(-1) == 1 || x.numel() == 0;
+  for (int64_t d = 0; d + 3 < x.dim(); ++d)  // the leading dimensions collapse to one token dimension
+    if (x.size(d) != 1 && x.stride(d) != x.stride(d + 1) * x.size(d + 1)) strided = false;
+  if (!strided) x = x.contiguous();
+  s.src = x.data_ptr();
+  s.src_token = x.dim() > 2 ? x.stride(-3) : heads * head_dim;
+  s.src_head = x.stride(-2);
+  s.dst = out.data_ptr();
+  s.dst_token = heads * head_dim;
+  s.dst_head = head_dim;
+  s.heads = (int)heads;
+  s.rotate = 1;
+  return out;
+}
+
+std::vector<OptTensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor cos_t, Tensor sin_t, bool interleaved,
+                              bool inverse) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(q.device());
+  const int dtype = dtype_code(q, "q");
+  TORCH_CHECK(q.dim() >= 2, "q must be [..., heads, head_dim]");
+  RotaryArgs a{};
+  rotary_tables(a, cos_t, sin_t, q, q.size(-1), interleaved);
+  rotary_positions(a, positions, q);
+  a.inverse = inverse;
+  a.tokens = positions.numel();
+  TORCH_CHECK(q.dim() == positions.dim() + 2 && q.sizes().slice(0, q.dim() - 2) == positions.sizes(),
+              "positions must have the leading dimensions of q");
+  std::vector<OptTensor> result;
+  result.emplace_back(rotary_segment(a.seg[0], q, a.head_dim));
+  if (k.has_value()) {
+    typed(*k, q.scalar_type(), q, "k");
+    TORCH_CHECK(k->dim() == q.dim() && k->sizes().slice(0, q.dim() - 2) == positions.sizes(),
+                "k must have the leading dimensions of q");
+    result.emplace_back(rotary_segment(a.seg[1], *k, a.head_dim));
+  } else {
+    result.emplace_back(c10::nullopt);
+  }
+  if (a.seg[0].heads + a.seg[1].heads > 0) check(pra_rotary(a, dtype, stream()), "rotary");
+  return result;
+}
+
+Tensor rotary_cache(Tensor qkv, int64_t heads, int64_t kv_heads, int64_t head_dim, Tensor positions, Tensor cos_t,
+                    Tensor sin_t, bool interleaved, Tensor k_cache, Tensor v_cache, Tensor slots) {
+  TORCH_CHECK(qkv.is_cuda(), "qkv must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  const int dtype = dtype_code(qkv, "qkv");
+  TORCH_CHECK(heads >= 0 && kv_heads > 0 && heads <= 4096 && kv_heads <= 4096, "1 to 4096 heads");
+  RotaryArgs a{};
+  rotary_tables(a, cos_t, sin_t, qkv, head_dim, interleaved);
+  rotary_positions(a, positions, qkv);
+  TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) >= (heads + 2 * kv_heads) * head_dim,
+              "qkv must be [tokens, >= (heads + 2 kv_heads) * head_dim] with contiguous rows");
+  a.tokens = qkv.size(0);
+  TORCH_CHECK(positions.numel() == a.tokens, "one position per token");
+  a.slots = per_row<int>(slots, at::kInt, qkv, a.tokens, "slots");
+  for (const Tensor* c : {&k_cache, &v_cache}) {
+    typed(*c, qkv.scalar_type(), qkv, "the caches");
+    TORCH_CHECK(c->dim() == 2 && c->stride(1) == 1 && c->size(1) >= kv_heads * head_dim && c->size(0) == k_cache.size(0),
+                "the caches must be [rows, >= kv_heads * head_dim] with contiguous rows");
+    TORCH_CHECK(c->size(0) <= 1 || c->stride(0) >= kv_heads * head_dim, "cache rows overlap");
+  }
+  a.slot_rows = k_cache.size(0);
+  auto q = torch::empty({a.tokens, heads * head_dim}, qkv.options());
+  const int64_t size = qkv.element_size(), ld = qkv.stride(0);
+  char* base = static_cast<char*>(qkv.data_ptr());
+  a.seg[0] = {base, q.data_ptr(), ld, head_dim, heads * head_dim, head_dim, (int)heads, 1, 0};
+  a.seg[1] = {base + heads * head_dim * size, k_cache.data_ptr(), ld, head_dim, k_cache.stride(0), head_dim, (int)kv_heads, 1, 1};
+  a.seg[2] = {base + (heads + kv_heads) * head_dim * size, v_cache.data_ptr(), ld, head_dim, v_cache.stride(0), head_dim, (int)kv_heads, 0, 1};
+  check(pra_rotary(a, dtype, stream()), "rotary_cache");
+  return q;
+}
+
+// ---------------------------------------------------------------- rules on logits
+struct Rules {
+  OptTensor ids, hist_len, prompt_len, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows;
+};
+
+LogitsArgs rules_args(const Tensor& logits, const Rules& r, int64_t vocab_start) {
+  TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1), "logits must be [B, V] with contiguous rows");
+  LogitsArgs a{};
+  const int64_t B = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(B <= 65535, "at most 65535 rows of logits");
+  TORCH_CHECK(V > 0, "logits need at least one column");
+  TORCH_CHECK(vocab_start >= 0 && vocab_start % 8 == 0, "vocab_start must be a multiple of 8");
+  TORCH_CHECK(vocab_start + V <= INT32_MAX - 64, "token ids must fit 31 bits");
+  a.logits = logits.data_ptr();
+  a.in_stride = logits.stride(0);
+  a.B = (int)B;
+  a.V = (int)V;
+  a.vocab_start = (int)vocab_start;
+  TORCH_CHECK(r.ids.has_value() == r.hist_len.has_value(), "a history is ids and lengths");
+  if (r.ids.has_value()) {
+    typed(*r.ids, at::kInt, logits, "history ids");
+    TORCH_CHECK(r.ids->dim() == 2 && r.ids->size(0) == B && (r.ids->stride(1) == 1 || r.ids->size(1) <= 1),
+                "history ids must be [B, capacity] with contiguous rows");
+    TORCH_CHECK(r.ids->size(1) < PRA_RULES_MAX_HISTORY, "a history holds fewer than ", num(PRA_RULES_MAX_HISTORY), " ids");
+    a.ids = r.ids->data_ptr<int>();
+    a.ids_stride = r.ids->stride(0);
+    a.capacity = (int)r.ids->size(1);
+    a.hist_len = const_cast<int*>(per_row<int>(r.hist_len, at::kInt, logits, B, "history lengths"));
+    a.prompt_len = per_row<int>(r.prompt_len, at::kInt, logits, B, "prompt lengths");
+    a.repetition = per_row<float>(r.repetition, at::kFloat, logits, B, "repetition");
+    a.presence = per_row<float>(r.presence, at::kFloat, logits, B, "presence");
+    a.frequency = per_row<float>(r.frequency, at::kFloat, logits, B, "frequency");
+  }
+  TORCH_CHECK(r.bias_ids.has_value() == r.bias_values.has_value(), "biases are ids and values");
+  if (r.bias_ids.has_value() && r.bias_ids->numel() > 0) {
+    typed(*r.bias_ids, at::kInt, logits, "bias ids");
+    typed(*r.bias_values, at::kFloat, logits, "bias values");
+    TORCH_CHECK(r.bias_ids->dim() == 2 && r.bias_ids->size(0) == B && r.bias_ids->sizes() == r.bias_values->sizes() &&
+                    r.bias_ids->is_contiguous() && r.bias_values->is_contiguous(),
+                "bias ids and values must be contiguous [B, n]");
+    TORCH_CHECK(r.bias_ids->size(1) <= PRA_RULES_MAX_BIASES, "at most ", num(PRA_RULES_MAX_BIASES), " biases a row");
+    a.bias_ids = r.bias_ids->data_ptr<int>();
+    a.bias_values = r.bias_values->data_ptr<float>();
+    a.n_bias = (int)r.bias_ids->size(1);
+  }
+  if (r.mask.has_value()) {
+    typed(*r.mask, at::kInt, logits, "mask");
+    TORCH_CHECK(r.mask->dim() == 2 && r.mask->is_contiguous() && r.mask->size(1) * 32 >= vocab_start + V,
+                "mask must be contiguous [masks, >= ceil(vocabulary / 32)] int32 words");
+    TORCH_CHECK(r.mask_rows.has_value() || r.mask->size(0) == B, "one mask per row, or mask_rows");
+    a.mask = reinterpret_cast<const uint32_t*>(r.mask->data_ptr<int>());
+    a.mask_count = (int)r.mask->size(0);
+    a.mask_words = r.mask->size(1);
+    a.mask_rows = per_row<int>(r.mask_rows, at::kInt, logits, B, "mask_rows");
+  } else {
+    TORCH_CHECK(!r.mask_rows.has_value(), "mask_rows without a mask");
+  }
+  TORCH_CHECK((a.ids == nullptr && a.bias_ids == nullptr) || V <= PRA_RULES_MAX_VOCAB, "a history or biases need at most ",
+              num(PRA_RULES_MAX_VOCAB), " columns");
+  return a;
+}
+
+Tensor process_logits(Tensor logits, OptTensor out_in, OptTensor ids, OptTensor hist_len, OptTensor prompt_len,
+                      OptTensor repetition, OptTensor presence, OptTensor frequency, OptTensor bias_ids,
+                      OptTensor bias_values, OptTensor mask, OptTensor mask_rows, int64_t vocab_start) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int dtype = dtype_code(logits, "logits");
+  LogitsArgs a = rules_args(logits, {ids, hist_len, prompt_len, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows}, vocab_start);
+  Tensor out;
+  if (out_in.has_value()) {
+    out = *out_in;
+    typed(out, logits.scalar_type(), logits, "out");
+    TORCH_CHECK(out.sizes() == logits.sizes() && (out.stride(1) == 1 || out.size(1) <= 1), "out must be shaped as logits");
+    TORCH_CHECK(out.size(0) <= 1 || out.stride(0) >= out.size(1), "rows of out overlap");
+    const auto extent = [](const Tensor& t) { return ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size(); };
+    const char* x = static_cast<const char*>(logits.data_ptr());
+    const char* y = static_cast<const char*>(out.data_ptr());
+    TORCH_CHECK(logits.size(0) == 0 || (x == y && (out.size(0) == 1 || out.stride(0) == logits.stride(0))) ||
+                    x + extent(logits) <= y || y + extent(out) <= x,
+                "out must be logits itself or not overlap it");
+  } else {
+    out = torch::empty(logits.sizes(), logits.options());
+  }
+  a.out = out.data_ptr();
+  a.out_stride = out.stride(0);
+  check(pra_logits_rules(a, dtype, stream()), "process_logits");
+  return out;
+}
+
+std::vector<Tensor> choose_tokens(Tensor logits, OptTensor ids, OptTensor hist_len, OptTensor prompt_len,
+                                  OptTensor repetition, OptTensor presence, OptTensor frequency, OptTensor bias_ids,
+                                  OptTensor bias_values, OptTensor mask, OptTensor mask_rows, int64_t vocab_start,
+                                  bool append) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int dtype = dtype_code(logits, "logits");
+  LogitsArgs a = rules_args(logits, {ids, hist_len, prompt_len, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows}, vocab_start);
+  TORCH_CHECK(!append || a.ids != nullptr, "append needs a history");
+  auto token = torch::empty({logits.size(0)}, logits.options().dtype(at::kLong));
+  auto value = torch::empty({logits.size(0)}, logits.options().dtype(at::kFloat));
+  a.token = token.data_ptr<int64_t>();
+  a.value = value.data_ptr<float>();
+  if (append) a.append_ids = const_cast<int*>(a.ids);
+  check(pra_logits_rules(a, dtype, stream()), "choose_tokens");
+  return {token, value};
+}
+
+// ---------------------------------------------------------------- attention over a shared prefix
+// Rows of 16-byte pieces that the tensor-memory accelerator can address.
+void rows_ok(const Tensor& t, int64_t width, const char* name) {
+  TORCH_CHECK(t.stride(-1) == 1 && t.size(-1) >= width, name, " needs contiguous rows of at least ", num(width), " elements");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must start on a 16-byte boundary");
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    TORCH_CHECK(t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0), name, " needs strides that are multiples of 16 bytes");
+}
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// out [like q], lse [B, H, T] (or undefined).
+std::vector<OptTensor> shared_prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k, Tensor v, Tensor lengths,
+                                               int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                               OptTensor prefix_lengths, double scale, bool return_lse) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(q.device());
+  TORCH_CHECK(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
+  TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
+  TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16, "q has dtype ", q.scalar_type(), ", expected bf16");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == heads * head_dim, "q must be [B, T, heads * head_dim]");
+  rows_ok(q, heads * head_dim, "q");
+  const int64_t width = kv_heads * head_dim;
+  for (const Tensor* t : {&pk, &pv, &k, &v}) typed(*t, at::kBFloat16, q, "keys and values");
+  TORCH_CHECK(pk.dim() == 2 && pv.dim() == 2 && pk.size(0) == pv.size(0), "prefix keys and values must be [P, kv_heads * head_dim]");
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.size(0) == q.size(0) && v.size(0) == q.size(0) && k.size(1) == v.size(1),
+              "own keys and values must be [B, capacity, kv_heads * head_dim]");
+  const int64_t B = q.size(0), T = q.size(1), G = heads / kv_heads;
+  TORCH_CHECK(pk.size(0) < (1 << 30) && k.size(1) < (1 << 30) && B * T * G < (1 << 30) && B * kv_heads < (1 << 24),
+              "too many keys or queries");
+  if (pk.size(0) > 0) rows_ok(pk, width, "prefix keys"), rows_ok(pv, width, "prefix values");
+  if (k.size(1) > 0 && B > 0) {
+    rows_ok(k, width, "own keys"), rows_ok(v, width, "own values");
+    for (const Tensor* t : {&k, &v})
+      TORCH_CHECK(B == 1 || k.size(1) == 1 || t->stride(0) % t->stride(1) == 0,
+                  "the batch stride of own keys and values must be a multiple of their row stride");
+  }
+  PrefixAttnArgs a{};
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  a.q_batch = q.stride(0);
+  a.q_token = q.stride(1);
+  a.pk = reinterpret_cast<const __nv_bfloat16*>(pk.data_ptr());
+  a.pv = reinterpret_cast<const __nv_bfloat16*>(pv.data_ptr());
+  a.P = (int)pk.size(0);
+  // the stride of a single row is never walked, but the tensor maps want a real one
+  a.pk_row = pk.size(0) > 1 ? pk.stride(0) : width;
+  a.pv_row = pv.size(0) > 1 ? pv.stride(0) : width;
+  a.prefix_len = per_row<int>(prefix_lengths, at::kInt, q, B, "prefix_lengths");
+  a.k = reinterpret_cast<const __nv_bfloat16*>(k.data_ptr());
+  a.v = reinterpret_cast<const __nv_bfloat16*>(v.data_ptr());
+  a.cap = (int)k.size(1);
+  a.k_row = k.size(1) > 1 ? k.stride(1) : width;
+  a.v_row = v.size(1) > 1 ? v.stride(1) : width;
+  a.k_batch = B > 1 ? k.stride(0) : a.cap * a.k_row;
+  a.v_batch = B > 1 ? v.stride(0) : a.cap * a.v_row;
+  a.len = per_row<int>(lengths, at::kInt, q, B, "lengths");
+  a.B = (int)B;
+  a.T = (int)T;
+  a.H = (int)heads;
+  a.Hkv = (int)kv_heads;
+  a.D = (int)head_dim;
+  a.scale = (float)scale;
+  a.status = pra_attention_status_word(q.device());
+  auto out = torch::empty({B, T, heads * head_dim}, q.options());
+  std::vector<OptTensor> result{out, c10::nullopt};
+  float* lse = nullptr;
+  if (return_lse) {
+    auto l = torch::empty({B, heads, T}, q.options().dtype(at::kFloat));
+    lse = l.data_ptr<float>();
+    result[1] = l;
+  }
+  if (B == 0 || T == 0) return result;
+  if (a.P == 0 && a.cap == 0) {
+    out.zero_();
+    if (return_lse) result[1]->fill_(-INFINITY);
+    return result;
+  }
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.lse = lse;
+  const int prefix_blocks = ceil_div(a.P, 128), own_blocks = ceil_div(a.cap, 128);
+  const auto splits_for = [](const PrefixAttnArgs& p, int blocks) {
+    int tiles, slots;
+    pra_prefix_attention_shape(p, &tiles, &slots);
+    return std::max(1, std::min(blocks, slots / tiles));
+  };
+  // A row with 256 or more query rows of a KV head (or the only one) fills its tiles: prefix and own keys in
+  // one walk.  Else the prefix is walked once for the query rows of the whole batch, and the own keys
+  // on their own.
+  const bool per_row_walk = B == 1 || T * G >= 256 || a.P == 0 || a.cap == 0;
+  const auto fo = q.options().dtype(at::kFloat);
+  Tensor part_o, part_ml;
+  const auto workspace = [&](int n) {
+    part_o = torch::empty({B * T, heads, n, head_dim}, fo);
+    part_ml = torch::empty({B * T, heads, n, 2}, fo);
+    a.n_slots = n;
+    a.part_o = part_o.data_ptr<float>();
+    a.part_ml = part_ml.data_ptr<float>();
+  };
+  if (per_row_walk) {
+    a.packed = a.cap == 0;
+    a.use_prefix = a.P > 0;
+    a.use_own = a.cap > 0;
+    a.splits = splits_for(a, prefix_blocks + own_blocks);
+    if (a.splits > 1) workspace(a.splits);
+    check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
+    if (a.splits == 1) return result;
+  } else {
+    PrefixAttnArgs own = a;
+    a.packed = a.use_prefix = 1;
+    a.splits = splits_for(a, prefix_blocks);
+    own.use_own = 1;
+    // single tokens: the split-K decode kernel (16 query rows a tile instead of 128)
+    const bool decode = T == 1 && G <= 16 && a.k_row == a.v_row && a.k_batch == a.v_batch && k.size(1) > 1;
+    int split_keys = 256;
+    if (decode) {
+      for (int s : {1024, 512})
+        if (B * kv_heads * ceil_div(a.cap, s) >= 3 * 148) {
+          split_keys = s;
+          break;
+        }
+      own.splits = ceil_div(a.cap, split_keys);
+    } else {
+      own.splits = splits_for(own, own_blocks);
+    }
+    workspace(a.splits + own.splits);
+    own.part_o = a.part_o;
+    own.part_ml = a.part_ml;
+    own.n_slots = a.n_slots;
+    own.slot0 = a.splits;
+    check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
+    if (decode) {
+      DecodeAttnParams p{};
+      p.q = a.q;
+      p.q_row = a.q_batch;
+      p.B = a.B;
+      p.H = a.H;
+      p.Hkv = a.Hkv;
+      p.loc_k = a.k;
+      p.loc_v = a.v;
+      p.loc_row = a.k_row;
+      p.loc_batch = a.k_batch;
+      p.loc_len = a.len;
+      p.loc_cap = a.cap;
+      p.scale = a.scale;
+      p.split_keys = split_keys;
+      p.n_split = a.n_slots;
+      p.mem_splits = a.splits;
+      p.split_lo = a.splits;
+      p.split_count = own.splits;
+      p.phase = 1;
+      p.part_o = a.part_o;
+      p.part_ml = a.part_ml;
+      p.status = a.status;
+      check(pra_decode_attention(p, a.D, stream()), "shared_prefix_attention");
+    } else {
+      check(pra_prefix_attention(own, stream()), "shared_prefix_attention");
+    }
+  }
+  PrefixMergeArgs m{};
+  m.part_o = a.part_o;
+  m.part_ml = a.part_ml;
+  m.B = a.B;
+  m.T = a.T;
+  m.H = a.H;
+  m.D = a.D;
+  m.n_slots = a.n_slots;
+  m.out = a.out;
+  m.lse = lse;
+  check(pra_prefix_merge(m, stream()), "shared_prefix_attention");
+  return result;
+}
+
+}  // namespace
+
+void pra_bind_serving_ops(pybind11::module_& m) {
+  m.def("rotary", &rotary);
+  m.def("rotary_cache", &rotary_cache);
+  m.def("process_logits", &process_logits);
+  m.def("choose_tokens", &choose_tokens);
+  m.def("shared_prefix_attention", &shared_prefix_attention);
+}

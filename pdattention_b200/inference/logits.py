@@ -1,0 +1,90 @@
+"""Rules on logits before a token is chosen: penalties for repeated tokens, biases, grammar masks.
+
+``process_logits`` writes the processed logits (for a sampler); ``choose_tokens`` reduces them to the
+greedy token in the same pass and writes no logits.  Both take everything from the device, so a
+captured decode step replays with the histories, masks and penalties of that step.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ..ops._ext import require
+
+
+@dataclass
+class TokenHistory:
+    """Token ids of every row so far: ``ids`` ``[B, capacity]`` int32, of which the first ``lengths[b]``
+    are valid and the first ``prompt_lengths[b]`` (``None``: none) are the prompt's."""
+
+    ids: torch.Tensor
+    lengths: torch.Tensor
+    prompt_lengths: torch.Tensor | None = None
+
+    @classmethod
+    def start(cls, prompts: torch.Tensor, lengths: torch.Tensor, new_tokens: int) -> "TokenHistory":
+        """History of left-aligned ``prompts`` ``[B, T]`` with room for ``new_tokens`` more."""
+        n = lengths.to(prompts.device, torch.int32).contiguous()
+        ids = torch.zeros((prompts.shape[0], prompts.shape[1] + new_tokens), dtype=torch.int32, device=prompts.device)
+        ids[:, : prompts.shape[1]] = prompts
+        return cls(ids, n.clone(), n)
+
+    def append(self, tokens: torch.Tensor) -> None:
+        """Add ``tokens`` ``[B]`` (negative: none); a full row keeps what it has.  No host read."""
+        place = self.lengths.long()
+        room = (place < self.ids.shape[1]) & (tokens >= 0)
+        at = place.clamp(max=self.ids.shape[1] - 1)[:, None]
+        kept = torch.where(room[:, None], tokens[:, None].to(torch.int32), self.ids.gather(1, at))
+        self.ids.scatter_(1, at, kept)
+        self.lengths.add_(room.to(torch.int32))
+
+
+@dataclass
+class LogitsRules:
+    """What is done to each row's logits, in this order (each step rounded to fp32):
+
+    * ``repetition`` ``[B]``: a token of the history has its logit divided by it (positive logits) or
+      multiplied by it (others);
+    * ``frequency`` / ``presence`` ``[B]``: subtracted per occurrence in the output / once if there is one;
+    * ``bias_ids`` / ``bias_values`` ``[B, n]``: added to single tokens (a token listed twice gets the
+      sum; ids outside the vocabulary, as -1, are skipped; at most 2047 entries);
+    * ``mask`` ``[M, >= ceil(V / 32)]`` int32, bit ``t % 32`` of word ``t // 32`` set where token ``t`` is
+      allowed, the others become -inf; ``mask_rows`` ``[B]`` int32 names each row's mask (negative: no
+      mask; ``M`` or more: nothing is allowed), by default mask ``b`` for row ``b``.
+
+    Penalties are fp32, absent ones are left out.
+    """
+
+    repetition: torch.Tensor | None = None
+    presence: torch.Tensor | None = None
+    frequency: torch.Tensor | None = None
+    bias_ids: torch.Tensor | None = None
+    bias_values: torch.Tensor | None = None
+    mask: torch.Tensor | None = None
+    mask_rows: torch.Tensor | None = None
+
+
+def process_logits(logits: torch.Tensor, rules: LogitsRules, history: TokenHistory | None = None, *,
+                   out: torch.Tensor | None = None, vocab_start: int = 0) -> torch.Tensor:
+    """``logits`` ``[B, V]`` (bf16, fp16 or fp32, rows may be strided) after the rules, in a new tensor or
+    in ``out`` (which may be ``logits``).  ``vocab_start``: the token id of column 0 when the columns are
+    a slice of the vocabulary (a multiple of 8)."""
+    h = history
+    return require().process_logits(logits, out, h.ids if h else None, h.lengths if h else None,
+                                    h.prompt_lengths if h else None, rules.repetition, rules.presence, rules.frequency,
+                                    rules.bias_ids, rules.bias_values, rules.mask, rules.mask_rows, vocab_start)
+
+
+def choose_tokens(logits: torch.Tensor, rules: LogitsRules, history: TokenHistory | None = None, *,
+                  vocab_start: int = 0, append: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Greedy token of each row after the rules: ``(ids [B] int64, their processed logits [B] fp32)``.
+    Ties go to the lowest id; a row with nothing above -inf gives id -1 and -inf; NaN counts as the
+    largest.  ``append`` adds the chosen tokens to ``history`` in the same launch."""
+    h = history
+    if append and h is None:
+        raise ValueError("append needs a history")
+    return require().choose_tokens(logits, h.ids if h else None, h.lengths if h else None,
+                                   h.prompt_lengths if h else None, rules.repetition, rules.presence, rules.frequency,
+                                   rules.bias_ids, rules.bias_values, rules.mask, rules.mask_rows, vocab_start, append)
