@@ -462,22 +462,27 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(PrefixMergeArgs
   const int64_t at = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (at >= (int64_t)a.B * a.T * a.H) return;
-  const float* ml = a.part_ml + at * a.n_slots * 2;
-  const float* po = a.part_o + at * a.n_slots * D + lane * E;
+  const float* sets_ml[2] = {a.part_ml + at * a.n_slots * 2, a.more_ml + at * a.n_more * 2};
+  const float* sets_o[2] = {a.part_o + at * a.n_slots * D + lane * E, a.more_o + at * a.n_more * D + lane * E};
+  const int counts[2] = {a.n_slots, a.more_o != nullptr ? a.n_more : 0};
   float M = -INFINITY;
-  for (int s = lane; s < a.n_slots; s += 32) M = fmaxf(M, ml[2 * s]);
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    for (int s = lane; s < counts[g]; s += 32) M = fmaxf(M, sets_ml[g][2 * s]);
   M = warp_max(M);
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s = 0; s < a.n_slots; ++s) {
-    const float m = ml[2 * s];
-    if (m == -INFINITY) continue;  // nothing visible: its part of the workspace was not written
-    const float w = exp2f((m - M) * LOG2E);
-    L += w * ml[2 * s + 1];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += w * po[s * D + e];
-  }
+  for (int g = 0; g < 2; ++g)
+    for (int s = 0; s < counts[g]; ++s) {
+      const float m = sets_ml[g][2 * s];
+      if (m == -INFINITY) continue;  // nothing visible: its part of the workspace was not written
+      const float w = exp2f((m - M) * LOG2E);
+      L += w * sets_ml[g][2 * s + 1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += w * sets_o[g][(int64_t)s * D + e];
+    }
   const bool any = M != -INFINITY;
   const float inv = any ? 1.f / L : 0.f;
   if (a.out != nullptr) {

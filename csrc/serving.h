@@ -96,11 +96,14 @@ cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t stream);
 // CTAs of a launch before splitting, and how many run at once (for choosing splits).
 void pra_prefix_attention_shape(const PrefixAttnArgs& a, int* tiles, int* slots);
 
-// out / lse / exported partial from the n_slots partials of every (b, t, h).
+// out / lse from the partials of every (b, t, h).
 struct PrefixMergeArgs {
   const float* part_o;
   const float* part_ml;
   int B, T, H, D, n_slots;
+  const float* more_o;            // a second set of partials [B * T, H, n_more, D] of the same queries, or null
+  const float* more_ml;
+  int n_more;
   __nv_bfloat16* out;             // [B, T, H * D] or null
   float* lse;                     // [B, H, T] or null
 };

@@ -285,10 +285,12 @@ void rows_ok(const Tensor& t, int64_t width, const char* name) {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// out [like q], lse [B, H, T] (or undefined).
-std::vector<OptTensor> shared_prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k, Tensor v, Tensor lengths,
+// {out [like q], lse [B, H, T] or none}, or with `partials` the unmerged {o [B * T, H, n, D], (max, sum)
+// [B * T, H, n, 2]}.
+std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k, Tensor v, Tensor lengths,
                                                int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                               OptTensor prefix_lengths, double scale, bool return_lse) {
+                                               OptTensor prefix_lengths, double scale, bool return_lse,
+                                               bool partials) {
   TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(q.device());
   TORCH_CHECK(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
@@ -338,21 +340,35 @@ std::vector<OptTensor> shared_prefix_attention(Tensor q, Tensor pk, Tensor pv, T
   a.D = (int)head_dim;
   a.scale = (float)scale;
   a.status = pra_attention_status_word(q.device());
-  auto out = torch::empty({B, T, heads * head_dim}, q.options());
+  const auto fo = q.options().dtype(at::kFloat);
+  Tensor part_o, part_ml;
+  const auto workspace = [&](int n) {
+    part_o = torch::empty({B * T, heads, n, head_dim}, fo);
+    part_ml = torch::empty({B * T, heads, n, 2}, fo);
+    a.n_slots = n;
+    a.part_o = part_o.data_ptr<float>();
+    a.part_ml = part_ml.data_ptr<float>();
+  };
+  Tensor out;
+  if (!partials) out = torch::empty({B, T, heads * head_dim}, q.options());
   std::vector<OptTensor> result{out, c10::nullopt};
   float* lse = nullptr;
-  if (return_lse) {
+  if (return_lse && !partials) {
     auto l = torch::empty({B, heads, T}, q.options().dtype(at::kFloat));
     lse = l.data_ptr<float>();
     result[1] = l;
   }
-  if (B == 0 || T == 0) return result;
-  if (a.P == 0 && a.cap == 0) {
+  if (B == 0 || T == 0 || (a.P == 0 && a.cap == 0)) {
+    if (partials) {
+      workspace(1);
+      part_ml.fill_(-INFINITY);
+      return {part_o, part_ml};
+    }
     out.zero_();
     if (return_lse) result[1]->fill_(-INFINITY);
     return result;
   }
-  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  if (!partials) a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.lse = lse;
   const int prefix_blocks = ceil_div(a.P, 128), own_blocks = ceil_div(a.cap, 128);
   const auto splits_for = [](const PrefixAttnArgs& p, int blocks) {
@@ -364,23 +380,14 @@ std::vector<OptTensor> shared_prefix_attention(Tensor q, Tensor pk, Tensor pv, T
   // one walk.  Else the prefix is walked once for the query rows of the whole batch, and the own keys
   // on their own.
   const bool per_row_walk = B == 1 || T * G >= 256 || a.P == 0 || a.cap == 0;
-  const auto fo = q.options().dtype(at::kFloat);
-  Tensor part_o, part_ml;
-  const auto workspace = [&](int n) {
-    part_o = torch::empty({B * T, heads, n, head_dim}, fo);
-    part_ml = torch::empty({B * T, heads, n, 2}, fo);
-    a.n_slots = n;
-    a.part_o = part_o.data_ptr<float>();
-    a.part_ml = part_ml.data_ptr<float>();
-  };
   if (per_row_walk) {
     a.packed = a.cap == 0;
     a.use_prefix = a.P > 0;
     a.use_own = a.cap > 0;
     a.splits = splits_for(a, prefix_blocks + own_blocks);
-    if (a.splits > 1) workspace(a.splits);
+    if (a.splits > 1 || partials) workspace(a.splits);
     check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
-    if (a.splits == 1) return result;
+    if (a.splits == 1 && !partials) return result;
   } else {
     PrefixAttnArgs own = a;
     a.packed = a.use_prefix = 1;
@@ -433,6 +440,7 @@ std::vector<OptTensor> shared_prefix_attention(Tensor q, Tensor pk, Tensor pv, T
       check(pra_prefix_attention(own, stream()), "shared_prefix_attention");
     }
   }
+  if (partials) return {part_o, part_ml};
   PrefixMergeArgs m{};
   m.part_o = a.part_o;
   m.part_ml = a.part_ml;
@@ -447,6 +455,50 @@ std::vector<OptTensor> shared_prefix_attention(Tensor q, Tensor pk, Tensor pv, T
   return result;
 }
 
+// {out [B, T, H * D] bf16, lse [B, H, T] or none} of one or two sets of partials [B * T, H, n, D].
+std::vector<OptTensor> merge_attention_partials(Tensor part_o, Tensor part_ml, OptTensor more_o, OptTensor more_ml,
+                                                int64_t batch, bool return_lse) {
+  TORCH_CHECK(part_o.is_cuda(), "partials must be CUDA tensors");
+  c10::cuda::CUDAGuard guard(part_o.device());
+  TORCH_CHECK(more_o.has_value() == more_ml.has_value(), "partials are sums and (max, sum) pairs");
+  const auto set = [&](const Tensor& o, const Tensor& ml) {
+    typed(o, at::kFloat, part_o, "partials");
+    typed(ml, at::kFloat, part_o, "partials");
+    TORCH_CHECK(o.dim() == 4 && ml.dim() == 4 && o.is_contiguous() && ml.is_contiguous() && ml.size(3) == 2 &&
+                    o.sizes().slice(0, 3) == ml.sizes().slice(0, 3) && o.size(0) == part_o.size(0) &&
+                    o.size(1) == part_o.size(1) && o.size(3) == part_o.size(3),
+                "partials must be contiguous [B * T, H, n, D] and [B * T, H, n, 2]");
+  };
+  set(part_o, part_ml);
+  const int64_t rows = part_o.size(0), H = part_o.size(1), D = part_o.size(3);
+  TORCH_CHECK(D == 64 || D == 128, "head_dim must be 64 or 128");
+  TORCH_CHECK(batch > 0 ? rows % batch == 0 : rows == 0, "the partials hold whole batch rows");
+  PrefixMergeArgs m{};
+  m.part_o = part_o.data_ptr<float>();
+  m.part_ml = part_ml.data_ptr<float>();
+  m.n_slots = (int)part_o.size(2);
+  if (more_o.has_value()) {
+    set(*more_o, *more_ml);
+    m.more_o = more_o->data_ptr<float>();
+    m.more_ml = more_ml->data_ptr<float>();
+    m.n_more = (int)more_o->size(2);
+  }
+  m.B = (int)batch;
+  m.T = batch > 0 ? (int)(rows / batch) : 0;
+  m.H = (int)H;
+  m.D = (int)D;
+  auto out = torch::empty({batch, m.T, H * D}, part_o.options().dtype(at::kBFloat16));
+  m.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  std::vector<OptTensor> result{out, c10::nullopt};
+  if (return_lse) {
+    auto l = torch::empty({batch, H, m.T}, part_o.options());
+    m.lse = l.data_ptr<float>();
+    result[1] = l;
+  }
+  check(pra_prefix_merge(m, stream()), "merge_attention_partials");
+  return result;
+}
+
 }  // namespace
 
 void pra_bind_serving_ops(pybind11::module_& m) {
@@ -454,5 +506,6 @@ void pra_bind_serving_ops(pybind11::module_& m) {
   m.def("rotary_cache", &rotary_cache);
   m.def("process_logits", &process_logits);
   m.def("choose_tokens", &choose_tokens);
-  m.def("shared_prefix_attention", &shared_prefix_attention);
+  m.def("shared_prefix_attention", &prefix_attention);
+  m.def("merge_attention_partials", &merge_attention_partials);
 }

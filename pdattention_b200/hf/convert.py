@@ -16,13 +16,18 @@ def config_from_hf(hf_config, **pra) -> PRALlamaConfig:
     if family is None:
         raise ValueError(f"unsupported model type {hf_config.model_type!r} (llama, mistral or qwen2)")
     heads = hf_config.num_attention_heads
+    rope = dict(getattr(hf_config, "rope_parameters", None) or getattr(hf_config, "rope_scaling", None) or {})
+    theta = rope.pop("rope_theta", None)
+    scaling = None
+    if rope.get("rope_type", rope.get("type", "default")) != "default":
+        scaling = rope  # an unknown kind of scaling is refused by the configuration
+        scaling.setdefault("original_max_position_embeddings", hf_config.max_position_embeddings)
     head_dim = getattr(hf_config, "head_dim", None) or hf_config.hidden_size // heads
     return PRALlamaConfig(
         family=family, vocab_size=hf_config.vocab_size, hidden_size=hf_config.hidden_size,
         intermediate_size=hf_config.intermediate_size, num_hidden_layers=hf_config.num_hidden_layers,
         num_attention_heads=heads, num_key_value_heads=hf_config.num_key_value_heads, head_dim=head_dim,
-        rope_theta=float(getattr(hf_config, "rope_theta", None) or
-                         (getattr(hf_config, "rope_parameters", None) or {}).get("rope_theta", 10000.0)),
+        rope_theta=float(getattr(hf_config, "rope_theta", None) or theta or 10000.0), rope_scaling=scaling,
         rms_norm_eps=hf_config.rms_norm_eps,
         attention_bias=bool(getattr(hf_config, "attention_bias", family == "qwen2")),
         tie_word_embeddings=bool(getattr(hf_config, "tie_word_embeddings", False)),

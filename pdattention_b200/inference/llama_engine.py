@@ -10,7 +10,9 @@ Layout on one GPU (tensor parallelism shards the head / column dimensions, see
   ``row0[c] .. row0[c] + len[c]``), plus the routing gists (mean pre-rotary key per
   chunk) in fp32 (exact rescoring) and bf16 (tensor-core scoring);
 * local KV cache: per layer ``[2, B, max_len, kv_dim]`` for the direct window and the
-  generated tokens.
+  generated tokens;
+* shared prefix (``set_shared_prefix``): per layer one ``[P, 2 * kv_dim]`` buffer with the keys and
+  values of a prompt that every row starts with, encoded and attended over once for the batch.
 
 Per layer and step: RMSNorm -> QKV GEMM -> routing (tensor-core scores + exact
 top-k) -> rotary copy of q in place and of k/v into the cache -> attention over
@@ -28,8 +30,11 @@ import torch
 
 from ..models.llama import PRALlamaConfig, PRALlamaReference
 from ..ops import _ext
+from ..ops.rotary import RotaryTable, rotary_cache, rotary_frequencies
 from ..tracing import traced
+from .logits import LogitsRules, TokenHistory, choose_tokens
 from .routing import select_chunks
+from .shared_prefix import merge_attention_partials, shared_prefix_attention, shared_prefix_partials
 
 # Decode projections on this library's decode GEMM (PRA_DECODE_GEMM=cutlass keeps the CUTLASS
 # stream-K GEMM and the separate all-reduce); rows per call it serves.
@@ -207,6 +212,8 @@ class PRALlamaEngine:
         self.namespace: tuple[torch.Tensor, torch.Tensor] | None = None
         self.page_table: torch.Tensor | None = None  # [B, P] pages per row (paged chunk cache)
         self._row0 = 0  # first row of the prefill row batch being routed
+        self.prefix: torch.Tensor | None = None  # [L, P, 2 * kv_dim] keys and values of the shared prefix
+        self._no_len: torch.Tensor | None = None  # zero local lengths (memory-only decode attention)
         self.last_selection: dict[int, torch.Tensor] = {}
         # Vocabulary-parallel LM head: under tensor parallelism each rank holds rows
         # [vocab_start, vocab_end) of the head and computes only that slice of the logits.
@@ -306,10 +313,11 @@ class PRALlamaEngine:
         if have < max_pos:
             cfg = self.cfg
             n = max(max_pos, 2 * have)
-            half = cfg.head_dim // 2
-            inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, half, dtype=torch.float64) / half))
-            ang = torch.arange(n, dtype=torch.float64)[:, None] * inv[None]
-            self._rope_cache = {n: (ang.cos().float().to(self.device), ang.sin().float().to(self.device))}
+            freq, scale = rotary_frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling,
+                                             cfg.max_position_embeddings)
+            ang = torch.arange(n, dtype=torch.float64)[:, None] * freq[None]
+            self._rope_cache = {n: ((ang.cos() * scale).float().to(self.device),
+                                    (ang.sin() * scale).float().to(self.device))}
         return next(iter(self._rope_cache.values()))
 
     def _norm(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
@@ -509,6 +517,7 @@ class PRALlamaEngine:
         starts = rows.view(n, tc)[:, 0].contiguous()
         x = self._embed(ids)
         qd, kd = self.q_dim, self.kv_dim
+        table = RotaryTable(cos, sin)
         for li, lw in enumerate(self.w.layers):
             h = self._norm(x, self._ln(lw.ln_in))
             qkv = self._gemm(h, lw.qkv, lw.qkv_bias)
@@ -519,13 +528,11 @@ class PRALlamaEngine:
                 self.tp.local_gist_tables(mem, li)
             ext.gist_mean_into(k_pre, qkv[:, qd + kd: qd + 2 * kd], starts - c0 * tc, lengths, dest, gk, gv, gn,
                                mem.count[li: li + 1])
-            ext.rope_copy(k_pre, pool[:, :kd], rows, pos, cos, sin, self.kv_heads, cfg.head_dim)
-            ext.rope_copy(qkv[:, qd + kd:], pool[:, kd:], rows, None, None, None, self.kv_heads, cfg.head_dim)
-            ext.rope_copy(qkv[:, :qd], qkv[:, :qd], None, pos, cos, sin, self.heads, cfg.head_dim)
+            q = rotary_cache(qkv, self.heads, self.kv_heads, cfg.head_dim, pos, table, pool[:, :kd], pool[:, kd:], rows)
             if li == len(self.w.layers) - 1:
                 break  # the last layer's output is never read
             kv = pool[c0 * tc: c0 * tc + M].view(n, tc, 2 * kd)
-            a = ext.attention_fwd(qkv.view(n, tc, -1)[:, :, :qd], kv[:, :, :kd], kv[:, :, kd:], self.heads,
+            a = ext.attention_fwd(q.view(n, tc, qd), kv[:, :, :kd], kv[:, :, kd:], self.heads,
                                   self.kv_heads, cfg.head_dim, None, None, None, None, valid,
                                   1.0 / math.sqrt(cfg.head_dim))[0]
             x = self._row_parallel(a.view(M, qd), lw.o, x)
@@ -542,6 +549,53 @@ class PRALlamaEngine:
         n = counts.to(self.device, torch.int32).contiguous()
         self.namespace = (torch.zeros_like(n), n)
         self.page_table = table.to(self.device, torch.int32).contiguous()
+
+    @property
+    def prefix_tokens(self) -> int:
+        return 0 if self.prefix is None else self.prefix.shape[1]
+
+    def _prefix_kv(self, layer: int, end: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        rows = self.prefix[layer, : self.prefix_tokens if end is None else end]
+        return rows[:, : self.kv_dim], rows[:, self.kv_dim:]
+
+    @torch.no_grad()
+    @traced("pra.llama.shared_prefix")
+    def set_shared_prefix(self, ids: torch.Tensor | None, chunk_tokens: int = 4096) -> None:
+        """Every row of the following prefills starts with ``ids`` ``[P]`` (``None``: none): a prompt encoded
+        once, whose keys and values all rows attend over.  Prompts given to ``prefill`` are what
+        follows it, at positions ``P, P + 1, ...``.  Encoded ``chunk_tokens`` at a time (activation
+        memory), each chunk behind the ones before it; prefix tokens read no chunk memory."""
+        self.prefix = None
+        self.cache = self.cache_len = None  # a cache filled behind another prefix does not fit this one
+        if ids is None or ids.numel() == 0:
+            return
+        cfg = self.cfg
+        if ids.dim() != 1:
+            raise ValueError("a shared prefix is one row of token ids")
+        if cfg.head_dim not in (64, 128):
+            raise ValueError("a shared prefix needs head dim 64 or 128")
+        ids = ids.to(self.device)
+        P, qd, kd = ids.shape[0], self.q_dim, self.kv_dim
+        self.prefix = torch.empty((cfg.num_hidden_layers, P, 2 * kd), device=self.device, dtype=torch.bfloat16)
+        table = RotaryTable(*self.rope_tables(P))
+        if self.tp is not None:  # each row-parallel partial must fit the peer buffer
+            chunk_tokens = max(1, min(chunk_tokens, self.tp.max_partial // cfg.hidden_size))
+        for p0 in range(0, P, chunk_tokens):
+            n = min(chunk_tokens, P - p0)
+            rows = torch.arange(p0, p0 + n, device=self.device, dtype=torch.int32)
+            length = torch.full((1,), n, device=self.device, dtype=torch.int32)
+            x = self._embed(ids[p0: p0 + n])
+            for li, lw in enumerate(self.w.layers):
+                qkv = self._gemm(self._norm(x, self._ln(lw.ln_in)), lw.qkv, lw.qkv_bias)
+                k, v = self._prefix_kv(li)
+                q = rotary_cache(qkv, self.heads, self.kv_heads, cfg.head_dim, rows, table, k, v, rows)
+                if li == len(self.w.layers) - 1:
+                    break  # the last layer's output is never read
+                pk, pv = self._prefix_kv(li, p0)
+                a = shared_prefix_attention(q.view(1, n, qd), pk, pv, k[None, p0: p0 + n], v[None, p0: p0 + n], length,
+                                            self.heads, self.kv_heads, cfg.head_dim)
+                x = self._row_parallel(a.view(n, qd), lw.o, x)
+                x = self._mlp(lw, x)
 
     @torch.no_grad()
     @traced("pra.llama.prefill")
@@ -563,6 +617,8 @@ class PRALlamaEngine:
         # tail continues the positions of its implicit head when they are natively legal)
         self.pos_offset = (position_offset.to(self.device, torch.int32).contiguous() if position_offset is not None
                            else torch.zeros(B, device=self.device, dtype=torch.int32))
+        if self.prefix is not None:  # the rows' own tokens follow the shared prefix
+            self.pos_offset = self.pos_offset + self.prefix_tokens
         self._max_pos = int(self.pos_offset.max()) + max_len if B else max_len
         step = row_batch or B
         outs = [self._prefill_rows(ids[r: r + step], lengths[r: r + step], r) for r in range(0, B, step)]
@@ -582,6 +638,8 @@ class PRALlamaEngine:
         valid = (torch.arange(T, device=self.device)[None] < lengths[:, None]).to(torch.uint8).contiguous()
         last = (torch.arange(B, device=self.device) * T + lengths.long() - 1)
         x = self._embed(ids)
+        table = RotaryTable(cos, sin)
+        full = torch.full((B,), T, device=self.device, dtype=torch.int32)  # token t sees own tokens 0 .. t
         use_memory = self.memory is not None and self.namespace is not None and cfg.top_k_chunks > 0
         namespace = None
         if use_memory:
@@ -596,13 +654,21 @@ class PRALlamaEngine:
                 mem_args = (self.memory.k(li), self.memory.v(li), mem_idx, mem_len)
             kc = self.cache[li, 0].view(-1, kd)
             vc = self.cache[li, 1].view(-1, kd)
-            ext.rope_copy(qkv[:, qd: qd + kd], kc, rows, pos, cos, sin, self.kv_heads, cfg.head_dim)
-            ext.rope_copy(qkv[:, qd + kd:], vc, rows, None, None, None, self.kv_heads, cfg.head_dim)
-            ext.rope_copy(qkv[:, :qd], qkv[:, :qd], None, pos, cos, sin, self.heads, cfg.head_dim)
+            q = rotary_cache(qkv, self.heads, self.kv_heads, cfg.head_dim, pos, table, kc, vc, rows).view(B, T, qd)
             k_rows = self.cache[li, 0][r0: r0 + B, :T]
             v_rows = self.cache[li, 1][r0: r0 + B, :T]
-            a = ext.attention_fwd(qkv.view(B, T, -1)[:, :, :qd], k_rows, v_rows, self.heads, self.kv_heads,
-                                  cfg.head_dim, *mem_args, valid, 1.0 / math.sqrt(cfg.head_dim))[0]
+            heads = (self.heads, self.kv_heads, cfg.head_dim)
+            if self.prefix is None:
+                a = ext.attention_fwd(q, k_rows, v_rows, *heads, *mem_args, valid, 1.0 / math.sqrt(cfg.head_dim))[0]
+            elif mem_args[0] is None:
+                a = shared_prefix_attention(q, *self._prefix_kv(li), k_rows, v_rows, full, *heads)
+            else:  # the routed memory on its own (no local key is valid), joined with [prefix ; local]
+                parts = shared_prefix_partials(q, *self._prefix_kv(li), k_rows, v_rows, full, *heads)
+                o, lse = ext.attention_fwd(q, k_rows, v_rows, *heads, *mem_args, torch.zeros_like(valid),
+                                           1.0 / math.sqrt(cfg.head_dim))[:2]
+                lse = lse.transpose(1, 2).reshape(M, self.heads, 1)
+                more = (o.view(M, self.heads, 1, cfg.head_dim).float(), torch.stack([lse, torch.ones_like(lse)], -1))
+                a = merge_attention_partials(parts, more, batch=B)
             x = self._row_parallel(a.view(M, qd), lw.o, x)
             x = self._mlp(lw, x)
         return self._logits(x[last])
@@ -642,10 +708,12 @@ class PRALlamaEngine:
 
     @torch.no_grad()
     @traced("pra.llama.decode_step")
-    def decode_step(self, token_ids: torch.Tensor, sample: bool = False) -> torch.Tensor:
+    def decode_step(self, token_ids: torch.Tensor, sample: bool = False, rules: LogitsRules | None = None,
+                    history: TokenHistory | None = None) -> torch.Tensor:
         """One token per row at position ``cache_len[b]``; returns logits ``[B, V]``, or with
         ``sample=True`` the greedy next token ids ``[B]`` (no full-vocabulary logits are formed
-        under tensor parallelism)."""
+        under tensor parallelism).  With ``rules`` the choice is made after them, -1 where they
+        leave a row nothing, and joins ``history``."""
         cfg, ext = self.cfg, self.ext
         B = token_ids.shape[0]
         qd, kd = self.q_dim, self.kv_dim
@@ -683,7 +751,9 @@ class PRALlamaEngine:
                 ext.rope_copy(qkv[:, :qd], q, None, pos, cos, sin, self.heads, cfg.head_dim)
             mem_args = (None, None, None, None)
             routed = use_memory and cfg.is_pra_layer(li)
-            if routed and self.overlap_routing:
+            if self.prefix is not None:
+                a = self._attend_prefix(li, q, None if qkv is None else qkv[:, :qd], rq, new_len, routed)
+            elif routed and self.overlap_routing:
                 a = self._attend_overlapped(li, q, None if qkv is None else qkv[:, :qd], rq, new_len, max_keys)
             else:
                 if routed:
@@ -698,7 +768,61 @@ class PRALlamaEngine:
                 x = self._row_parallel(a, lw.o, x)
                 x = self._mlp(lw, x)
         self.cache_len.copy_(new_len)  # in place: a captured step replays on the same tensors
-        return self._greedy(x) if sample else self._logits(x)
+        if not sample:
+            return self._logits(x)
+        return self._greedy(x) if rules is None else self._choose(self._local_logits(x), rules, history)
+
+    def _choose(self, local: torch.Tensor, rules: LogitsRules, history: TokenHistory | None) -> torch.Tensor:
+        """Greedy tokens after ``rules`` from this rank's vocabulary slice of the logits, merged
+        across ranks as ``_greedy`` does, and appended to ``history``."""
+        if self.tp is None:
+            return choose_tokens(local, rules, history, append=history is not None)[0]
+        token, value = choose_tokens(local, rules, history, vocab_start=self.vocab_start)
+        every = self.tp.gather_small(torch.stack([value, token.float()], dim=1)).view(-1, self.tp_size, 2)
+        score, ids = every[..., 0], every[..., 1]
+        top = score.max(dim=1, keepdim=True).values
+        token = torch.where(score == top, ids, torch.full_like(ids, float("inf"))).min(dim=1).values.long()
+        if history is not None:
+            history.append(token)
+        return token
+
+    def _attend_prefix(self, li: int, q: torch.Tensor, q_rows, rq, new_len: torch.Tensor, routed: bool) -> torch.Tensor:
+        """Decode attention over [routed memory ; shared prefix ; own tokens].  Routing and the memory part
+        run on the side stream beside the prefix and own parts (unless overlap is off)."""
+        cfg, ext = self.cfg, self.ext
+        B, H, Hkv, D = q.shape[0], self.heads, self.kv_heads, cfg.head_dim
+        kc, vc = self.cache[li, 0], self.cache[li, 1]
+        args = (q.unsqueeze(1), *self._prefix_kv(li), kc, vc, new_len, H, Hkv, D)
+        if not routed:
+            return shared_prefix_attention(*args).view(B, H * D)
+        if self._no_len is None or self._no_len.shape[0] != B:
+            self._no_len = torch.zeros(B, device=self.device, dtype=torch.int32)
+        n_mem = max(1, -(-cfg.memory_tokens_per_row // 256))
+        more = (torch.empty((B, H, n_mem, D), device=self.device, dtype=torch.float32),
+                torch.empty((B, H, n_mem, 2), device=self.device, dtype=torch.float32))
+
+        def memory_part():
+            mem_idx, mem_len = self._route(li, q_rows, B, route_query=rq)
+            ext.decode_attention(q, H, Hkv, D, self.memory.k(li), self.memory.v(li), mem_idx, mem_len, kc, vc,
+                                 self._no_len, n_mem * 256, 256, False, phase=1, part_o=more[0], part_ml=more[1])
+
+        if not self.overlap_routing:
+            memory_part()
+            return merge_attention_partials(shared_prefix_partials(*args), more, batch=B).view(B, H * D)
+        main = torch.cuda.current_stream(self.device)
+        if self._route_stream is None:
+            self._route_stream = torch.cuda.Stream(self.device, priority=-1)
+        side = self._route_stream
+        side.wait_stream(main)
+        parts = shared_prefix_partials(*args)
+        with torch.cuda.stream(side):
+            ext.set_launch_priority(True)
+            try:
+                memory_part()
+            finally:
+                ext.set_launch_priority(False)
+        main.wait_stream(side)
+        return merge_attention_partials(parts, more, batch=B).view(B, H * D)
 
     def _partials(self, B: int, n_split: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Split partials ``(o [B, H, n, Dh], (max, sum) [B, H, n, 2])`` shared by the phases of
@@ -755,8 +879,10 @@ class PRALlamaEngine:
                                     **common)[0]
 
     # -- CUDA-graph decode ------------------------------------------------------------
-    def capture_decode(self, sample: bool = False) -> None:
-        """Capture one ``decode_step`` into a CUDA graph (after at least one eager step).
+    def capture_decode(self, sample: bool = False, rules: LogitsRules | None = None,
+                       history: TokenHistory | None = None) -> None:
+        """Capture one ``decode_step`` into a CUDA graph (after at least one eager step).  ``rules`` and
+        ``history`` are read from their tensors at every replay.
 
         Replays run the whole step (32 layers of GEMMs, routing, attention and the
         tensor-parallel collectives) as one graph launch; the collectives take their
@@ -772,7 +898,7 @@ class PRALlamaEngine:
         was, before = counter.enabled, counter.launches
         counter.enabled = True  # count this library's kernels recorded in the graph
         with torch.cuda.graph(graph):
-            self._graph_out = self.decode_step(self._graph_ids, sample=sample)
+            self._graph_out = self.decode_step(self._graph_ids, sample=sample, rules=rules, history=history)
         self.graph_launches = counter.launches - before
         counter.launches, counter.enabled = before, was
         if self.tp is not None and ((self.tp.epoch_ar - ar0) % 2 or (self.tp.epoch_ag - ag0) % 2
@@ -792,14 +918,24 @@ class PRALlamaEngine:
         self._graph_out = None
 
     @torch.no_grad()
-    def generate(self, ids: torch.Tensor, lengths: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
-        """Greedy decoding: ``[B, max_new_tokens]`` new token ids."""
+    def generate(self, ids: torch.Tensor, lengths: torch.Tensor, max_new_tokens: int,
+                 rules: LogitsRules | None = None) -> torch.Tensor:
+        """Greedy decoding: ``[B, max_new_tokens]`` new token ids, each chosen after ``rules`` when given
+        (penalties see the row's prompt and what it has generated; a row whose rules leave nothing
+        gives -1 and goes on with token 0)."""
         logits = self.prefill(ids, lengths, max_new_tokens)
         out = []
-        tok = logits.float().argmax(-1)
+        if rules is None:
+            tok = logits.float().argmax(-1)
+        else:
+            history = TokenHistory.start(ids.to(self.device), lengths, max_new_tokens)
+            tok = choose_tokens(logits.contiguous(), rules, history, append=True)[0]
         for _ in range(max_new_tokens):
             out.append(tok)
             if len(out) == max_new_tokens:
                 break
-            tok = self.decode_step(tok, sample=True)
+            if rules is None:
+                tok = self.decode_step(tok, sample=True)
+            else:
+                tok = self.decode_step(tok.clamp(min=0), sample=True, rules=rules, history=history)
         return torch.stack(out, dim=1)

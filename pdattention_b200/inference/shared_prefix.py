@@ -30,5 +30,24 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     """
     out, lse = require().shared_prefix_attention(q, prefix_k, prefix_v, k, v, lengths, heads, kv_heads, head_dim,
                                                  prefix_lengths, 1.0 / math.sqrt(head_dim) if scale is None else scale,
-                                                 return_lse)
+                                                 return_lse, False)
+    return (out, lse) if return_lse else out
+
+
+def shared_prefix_partials(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
+                           v: torch.Tensor, lengths: torch.Tensor, heads: int, kv_heads: int, head_dim: int, *,
+                           prefix_lengths: torch.Tensor | None = None, scale: float | None = None):
+    """``shared_prefix_attention`` before its parts are joined: fp32 ``(sums [B T, H, n, D], (max, sum)
+    [B T, H, n, 2])``, each part's sum relative to its own maximum.  For queries that attend over
+    further keys elsewhere; ``merge_attention_partials`` joins both."""
+    return tuple(require().shared_prefix_attention(q, prefix_k, prefix_v, k, v, lengths, heads, kv_heads, head_dim,
+                                                   prefix_lengths,
+                                                   1.0 / math.sqrt(head_dim) if scale is None else scale, False, True))
+
+
+def merge_attention_partials(partials, more=None, *, batch: int, return_lse: bool = False):
+    """One softmax from one or two sets of partials of the same queries: ``[batch, T, H D]`` bf16 (and the
+    log sums ``[batch, H, T]``).  A part with maximum ``-inf`` counts as empty and is not read."""
+    more_o, more_ml = more if more is not None else (None, None)
+    out, lse = require().merge_attention_partials(*partials, more_o, more_ml, batch, return_lse)
     return (out, lse) if return_lse else out

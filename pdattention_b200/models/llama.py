@@ -35,6 +35,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.rotary import rotary_frequencies
+
 _FAMILIES = ("llama", "mistral", "qwen2")
 
 
@@ -59,6 +61,7 @@ class PRALlamaConfig:
     direct_window: int = 4096
     pra_layers: tuple | None = None   # layer ids that read memory (None: every layer)
     memory_budget_tokens: int | None = None  # cap on materialised memory tokens per row and layer
+    rope_scaling: dict | None = None  # long-context scaling of the rotary angles (ops.rotary.rotary_frequencies)
 
     def __post_init__(self):
         if self.family not in _FAMILIES:
@@ -69,6 +72,7 @@ class PRALlamaConfig:
             raise ValueError("head_dim must be even (rotary pairs)")
         if self.top_k_chunks < 0 or self.chunk_tokens <= 0:
             raise ValueError("top_k_chunks must be >= 0 and chunk_tokens > 0")
+        rotary_frequencies(self.head_dim, self.rope_theta, self.rope_scaling)  # refuses unknown scalings
         if self.pra_layers is not None:
             self.pra_layers = tuple(int(i) for i in self.pra_layers)
 
@@ -141,11 +145,10 @@ PRESETS = {"llama3-8b": llama3_8b, "mistral-7b": mistral_7b, "qwen2-7b": qwen2_7
 
 def rope_tables(cfg: PRALlamaConfig, positions: torch.Tensor, dtype=torch.float32):
     """cos/sin ``[..., Dh]`` for integer ``positions`` (HF ``rotate_half`` layout)."""
-    half = cfg.head_dim // 2
-    inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, half, dtype=torch.float64, device=positions.device) / half))
-    ang = positions.to(torch.float64)[..., None] * inv
+    freq, scale = rotary_frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, cfg.max_position_embeddings)
+    ang = positions.to(torch.float64)[..., None] * freq.to(positions.device)
     ang = torch.cat([ang, ang], dim=-1)
-    return ang.cos().to(dtype), ang.sin().to(dtype)
+    return (ang.cos() * scale).to(dtype), (ang.sin() * scale).to(dtype)
 
 
 def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
@@ -449,6 +452,8 @@ def hf_config(cfg: PRALlamaConfig):
                   num_key_value_heads=cfg.num_key_value_heads, rope_theta=cfg.rope_theta,
                   rms_norm_eps=cfg.rms_norm_eps, max_position_embeddings=cfg.max_position_embeddings,
                   tie_word_embeddings=cfg.tie_word_embeddings)
+    if cfg.rope_scaling:
+        common["rope_scaling"] = dict(cfg.rope_scaling)
     if cfg.family == "qwen2":
         return transformers.Qwen2Config(**common)
     if cfg.family == "mistral":

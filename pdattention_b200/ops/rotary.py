@@ -47,8 +47,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be a positive even number")
-    pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
-    freq = float(theta) ** -pair
+    pair = torch.arange(0, rotary_dim // 2, dtype=torch.float64) / (rotary_dim // 2)
+    freq = 1.0 / float(theta) ** pair
     if not scaling:
         return freq, 1.0
     kind = scaling.get("rope_type", scaling.get("type", "default"))

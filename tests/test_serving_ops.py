@@ -92,3 +92,39 @@ def test_history_appends_on_any_device():
     h.append(torch.tensor([9, 4]))  # row 0 is full
     assert h.ids.tolist() == [[5, 6, 1], [7, 4, 0]] and h.lengths.tolist() == [3, 2]
     assert h.prompt_lengths.tolist() == [2, 1]
+
+
+@pytest.mark.parametrize("family,scaling", [
+    ("llama", {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+               "original_max_position_embeddings": 32}),
+    ("qwen2", {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32}),
+    ("mistral", {"rope_type": "linear", "factor": 4.0})])
+def test_scaled_positions_match_hugging_face(family, scaling):
+    import transformers
+
+    from pdattention_b200.hf.convert import config_from_hf, reference_from_hf
+    from pdattention_b200.models.llama import PRALlamaReference, hf_config, tiny_llama
+
+    cfg = tiny_llama(family=family, attention_bias=family == "qwen2", rope_scaling=scaling, max_position_embeddings=128)
+    ours = PRALlamaReference(cfg).eval()
+    ours.reset_parameters(seed=0, std=0.2)
+    hcfg = hf_config(cfg)
+    hcfg._attn_implementation = "eager"
+    hf = {"llama": transformers.LlamaForCausalLM, "mistral": transformers.MistralForCausalLM,
+          "qwen2": transformers.Qwen2ForCausalLM}[family](hcfg).eval()
+    hf.load_state_dict(ours.state_dict(), strict=False)
+    ids = torch.randint(0, cfg.vocab_size, (1, 100), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        want = hf(ids).logits
+    # the other side takes angles in 32 bits: 100 * 2^-23 on the last position's fastest pair, as much again from its
+    # fp32 frequencies; scores of a few tens and two layers make of that at most some 1e-3 of logits near 1
+    assert torch.allclose(ours(ids), want, atol=2e-3, rtol=1e-3)
+    plain = PRALlamaReference(tiny_llama(family=family, attention_bias=family == "qwen2", max_position_embeddings=128)).eval()
+    plain.load_state_dict(ours.state_dict())
+    assert not torch.allclose(plain(ids), want, atol=2e-2, rtol=1e-2)  # the scaling matters here
+    back = reference_from_hf(hf)
+    assert back.cfg.rope_scaling["rope_type"] == scaling["rope_type"] and back.cfg.rope_theta == cfg.rope_theta
+    assert torch.equal(back(ids), ours(ids))
+    hcfg.rope_parameters = {"rope_type": "other", "factor": 2.0, "rope_theta": 1e4}
+    with pytest.raises(ValueError, match="scaling"):
+        config_from_hf(hcfg)
