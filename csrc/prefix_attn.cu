@@ -9,14 +9,23 @@
 // One CTA owns NT = 1 or 2 tiles of 128 query rows of one KV head and a range of 128-key blocks:
 //   * one thread brings K and V blocks in with TMA (128-byte swizzle) through a ring of R tiles;
 //   * one thread issues the MMAs: S_i = Q_i K^T (both operands in shared memory) and O_i += P_i V
-//     (P from TMEM), committing each to an mbarrier;
-//   * a warpgroup per tile does the softmax, one thread per query row (TMEM lane): the 128 scores of
-//     a block come into registers once, the running maximum is raised lazily (only when it grows by
-//     more than 2^8, then O is rescaled in TMEM), and P goes back over S's columns as bf16.
-// P shares S's columns, so S_{j+1} of a tile is issued only after P V_j of that tile has completed;
-// with two tiles the other tile's MMAs and softmax fill that gap.  P is rounded to bf16 (one half
-// step, 2^-8 relative, of each weight: the tensor cores take 16-bit operands); the row sums use the
-// unrounded weights, and S, O, maxima and sums stay in fp32.
+//     (P from TMEM), each committed to an mbarrier;
+//   * a warpgroup per tile does the softmax, one thread per query row (TMEM lane): a block's 128 scores
+//     come into registers once, the running maximum is raised lazily (only when it grows by more
+//     than 2^8, then O is rescaled in TMEM), and P goes back over S's columns as bf16 in two halves, so
+//     that P V of the first begins while the second is computed.
+// P shares S's columns (S, P and O of two tiles fill TMEM), so S_{j+1} of a tile is issued only after
+// P V_j of that tile has completed; the issuer takes the tiles in turn, which keeps one tile's softmax
+// beside the other's products.  P is rounded to bf16 (one half step, 2^-8 relative, of each weight: the
+// tensor cores take 16-bit operands); the row sums use the unrounded weights, and S, O, maxima and
+// sums stay in fp32.
+//
+// What bounds it: a tile's chain of about 3,800 cycles per block (softmax 2,000, two products of 512,
+// the rest hand-overs of 200 to 300 between the roles), against 2,048 cycles of products and 2,048 of
+// exponentials for both tiles: 1.0 to 1.1 PFLOP/s on long suffixes.  Measured beside it at 4 x 512
+// queries behind 16,384 keys (560 us): an issuer per tile 780 us (the tiles fall into step and compete),
+// two threads per row 573, S in two buffers of 64 columns 777 (an MMA of 64 columns takes 57 cycles, one
+// of 128 takes 65), a quarter of the exponentials as polynomials 557 to 600.
 //
 // Keys past the ones any query of the CTA may see are never multiplied: their scores are replaced by
 // -inf, and their value rows are zeroed in shared memory (a stale row may hold NaN, and 0 * NaN is
@@ -42,20 +51,48 @@ struct Cfg {
   static constexpr int BOX = BN * 128;        // 128 rows x 64 columns
   static constexpr int TILE = BOXES * BOX;    // one K, V or Q tile
   static constexpr int R = NT == 2 ? (D == 128 ? 4 : 6) : (D == 128 ? 2 : 4);
-  static constexpr int THREADS = NT * 128 + 64;
+  static constexpr int SOFTMAX = NT * 128;   // softmax threads; then the issuer's and the producer's warp
+  static constexpr int THREADS = SOFTMAX + 64;
   static constexpr int OFF_RING = NT * TILE;
   static constexpr int OFF_BAR = OFF_RING + R * TILE;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment slack
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;   // + alignment slack
   static constexpr int O_COL = NT * BN;               // TMEM: S / P of tile i at i * BN, O at O_COL + i * D
   static constexpr uint32_t COLS = NT == 2 ? 512 : 256;
   static constexpr int CTAS = NT == 2 ? 1 : 2;        // per SM
+  static constexpr int STAGE = 32 * D * 4;            // a warp's outputs on their way out (in the ring)
   static_assert(O_COL + NT * D <= (int)COLS, "TMEM");
+  static_assert(NT * 4 * STAGE <= R * TILE, "output staging");
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+
+// Two fp32 values in one 64-bit register pair, and the packed operations on them.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 __device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -142,7 +179,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [R] a ring tile has landed
   uint64_t* empty = full + R;                                        // [R] a ring tile has been read
   uint64_t* s_full = empty + R;                                      // [NT] S_i is in TMEM
-  uint64_t* p_full = s_full + NT;                                    // [NT] P_i is in TMEM
+  uint64_t* p_half = s_full + NT;                                    // [NT] half of P_i is in TMEM
+  uint64_t* p_full = p_half + NT;                                    // [NT] all of P_i is
   uint64_t* o_full = p_full + NT;                                    // [NT] O_i has P_i V
   uint64_t* q_full = o_full + NT;                                    // [NT] Q_i is in shared memory
   uint64_t* drain = q_full + NT;                                     // [1] every MMA issued has completed
@@ -152,23 +190,25 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.H / a.Hkv;
+  constexpr int ISSUER = C::SOFTMAX / 32, PRODUCER = ISSUER + 1;  // warps
   if (tid == 0) {
     for (int i = 0; i < R; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
+      mbar_init(empty + i, i % 2 == 0 ? NT : 1);  // K: each tile's softmax, V: the issuer
     }
     for (int i = 0; i < NT; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 128);
+      mbar_init(p_half + i, 4);
+      mbar_init(p_full + i, 4);
       mbar_init(o_full + i, 1);
-      mbar_init(q_full + i, 128);
+      mbar_init(q_full + i, 4);
     }
     mbar_init(drain, 1);
     s_abort = 0;
     s_seen = 0;
     tc::fence_mbarrier_init();
   }
-  if (warp == NT * 4) {
+  if (warp == PRODUCER) {
     tc::alloc(&s_tmem, C::COLS);
     tc::relinquish();
   }
@@ -201,7 +241,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     return j < it.prefix_blocks ? it.prefix_seen - j * BN : it.own_seen - (j - it.prefix_blocks) * BN;
   };
 
-  if (warp == NT * 4) {
+  if (warp == PRODUCER) {
     // ---------------------------------------------------------------- K / V producer
     if (lane == 0 && n > 0) {
       for (int j = it.lo; j < it.hi && !s_abort; ++j) {
@@ -222,7 +262,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
         if (!ok) break;
       }
     }
-  } else if (warp == NT * 4 + 1) {
+  } else if (warp >= ISSUER) {
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t ID_S = tc::idesc_bf16(BM, BN, false);
     constexpr uint32_t ID_O = tc::idesc_bf16(BM, D, true);
@@ -231,49 +271,47 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint32_t off = (kk / 4) * C::BOX + (kk % 4) * 32;
-        tc::mma_bf16(tmem + i * BN, desc_sw128(q_addr + i * C::TILE + off, 16),
-                     desc_sw128(ring + r * C::TILE + off, 16), ID_S, kk > 0);
+        tc::mma_bf16(tmem + i * BN, desc_sw128(q_addr + i * C::TILE + off, 16), desc_sw128(ring + r * C::TILE + off, 16), ID_S, kk > 0);
       }
     };
-    auto issue_o = [&](int i, int r, bool acc) {
+    auto issue_o = [&](int i, int r, int half, bool acc) {  // 64 keys
 #pragma unroll
-      for (int kk = 0; kk < BN / 16; ++kk)
+      for (int kk = half * (BN / 32); kk < (half + 1) * (BN / 32); ++kk)
         tc::mma_bf16_ts(tmem + C::O_COL + i * D, tmem + i * BN + kk * 8,
                         desc_sw128(ring + r * C::TILE + kk * 2048, C::BOX), ID_O, (acc || kk > 0) ? 1u : 0u);
     };
     if (lane == 0 && n > 0) {
       bool ok = wait(full, 0, &s_abort);
-      tc::fence_after();
-      if (ok) {
-        for (int i = 0; i < NT && ok; ++i) {
-          ok = wait(q_full + i, 0, &s_abort);
-          if (!ok) break;
-          issue_s(i, 0);
-          tc::commit(s_full + i);
-        }
-        if (ok && R < 2 * n) tc::commit(empty);
+      for (int i = 0; i < NT && ok; ++i) {
+        ok = wait(q_full + i, 0, &s_abort);
+        if (!ok) break;
+        tc::fence_after();
+        issue_s(i, 0);
+        tc::commit(s_full + i);
       }
       for (int j = 0; j < n && ok; ++j) {
         const int vt = 2 * j + 1, kt = 2 * j + 2;  // ring positions of V_j and K_{j+1}
-        const bool more = j + 1 < n;
-        for (int i = 0; i < NT && ok; ++i) {
-          ok = ok && wait(p_full + i, (uint32_t)(j & 1), &s_abort);
-          if (i == 0) ok = ok && wait(full + vt % R, (uint32_t)((vt / R) & 1), &s_abort);
+        ok = wait(full + vt % R, (uint32_t)((vt / R) & 1), &s_abort);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          ok = ok && wait(p_half + i, (uint32_t)(j & 1), &s_abort);
           if (!ok) break;
           tc::fence_after();
-          issue_o(i, vt % R, j > 0);
-          if (i == NT - 1 && vt + R < 2 * n) tc::commit(empty + vt % R);  // only tiles that are refilled
+          issue_o(i, vt % R, 0, j > 0);
+          ok = wait(p_full + i, (uint32_t)(j & 1), &s_abort);
+          if (!ok) break;
+          tc::fence_after();
+          issue_o(i, vt % R, 1, true);
           tc::commit(o_full + i);
-          if (more) {
-            // P_i V_j reads the columns that S_i is about to overwrite
-            ok = ok && wait(o_full + i, (uint32_t)(j & 1), &s_abort);
-            if (i == 0) ok = ok && wait(full + kt % R, (uint32_t)((kt / R) & 1), &s_abort);
-            if (!ok) break;
-            tc::fence_after();
-            issue_s(i, kt % R);
-            if (i == NT - 1 && kt + R < 2 * n) tc::commit(empty + kt % R);
-            tc::commit(s_full + i);
-          }
+          if (j + 1 == n) continue;
+          if (i == 0) ok = wait(full + kt % R, (uint32_t)((kt / R) & 1), &s_abort);
+          // P V_j reads the columns that S_{j+1} is about to overwrite
+          ok = ok && wait(o_full + i, (uint32_t)(j & 1), &s_abort);
+          if (!ok) break;
+          tc::fence_after();
+          issue_s(i, kt % R);
+          tc::commit(s_full + i);
+          if (i == NT - 1) mbar_arrive(empty + vt % R);
         }
       }
       if (!ok) {
@@ -289,19 +327,34 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     const int TG = a.T * G;
     const int b = it.b >= 0 ? it.b : min(qr / TG, a.B - 1);
     const int t = (qr / G) % a.T, h = it.kvh * G + qr % G;
-    // this tile's queries into shared memory (rows past the last: zero)
-    for (int e = row; e < BM * (D / 8); e += BM) {
-      const int r = e / (D / 8), c = e % (D / 8), x = it.row0 + i * BM + r;
-      uint4 val = make_uint4(0, 0, 0, 0);
-      if (x < it.rows) {
-        const int xb = it.b >= 0 ? it.b : x / TG;
-        val = *reinterpret_cast<const uint4*>(a.q + xb * a.q_batch + (int64_t)((x / G) % a.T) * a.q_token +
-                                              (int64_t)(it.kvh * G + x % G) * D + c * 8);
+    // this tile's queries into shared memory (rows past the last: zero), eight loads of a thread in flight
+    {
+      constexpr int CH = D / 8, STEP = BM / CH;
+      const int c = row % CH;
+#pragma unroll
+      for (int x0 = 0; x0 < CH; x0 += 8) {
+        uint4 val[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int r = it.row0 + i * BM + row / CH + (x0 + x) * STEP;
+          val[x] = make_uint4(0, 0, 0, 0);
+          if (r < it.rows) {
+            const int bt = r / G, xb = it.b >= 0 ? it.b : bt / a.T;
+            const int xt = it.b >= 0 ? bt : bt - xb * a.T;
+            val[x] = *reinterpret_cast<const uint4*>(a.q + xb * a.q_batch + xt * a.q_token +
+                                                     (int64_t)(it.kvh * G + r - bt * G) * D + c * 8);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int r = row / CH + (x0 + x) * STEP;
+          *reinterpret_cast<uint4*>(smem + i * C::TILE + (c / 8) * C::BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = val[x];
+        }
       }
-      *reinterpret_cast<uint4*>(smem + i * C::TILE + (c / 8) * C::BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = val;
     }
     fence_proxy_async_smem();
-    mbar_arrive(q_full + i);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full + i);
     const int prefix_lim = !live ? 0 : a.prefix_len ? max(0, min(a.prefix_len[b], a.P)) : a.P;
     int own_lim = 0;
     if (live && a.use_own) own_lim = max(0, min(max(a.len[b], 0), a.cap) - a.T + t + 1);
@@ -309,40 +362,42 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     const uint32_t t_s = tmem + t_lane + i * BN, t_o = tmem + t_lane + C::O_COL + i * D;
     const float sl2 = a.scale * LOG2E;
     float m_run = -INFINITY, l_run = 0.f;
+    // After a wait that gave up (here or in another role) the rest runs through without waiting; nothing
+    // is written at the end.
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int blk = it.lo + j;
       const bool own = blk >= it.prefix_blocks;
       const int lim = own ? own_lim - (blk - it.prefix_blocks) * BN : prefix_lim - blk * BN;
-      ok = wait(s_full + i, (uint32_t)(j & 1), &s_abort);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      ok &= wait(s_full + i, (uint32_t)(j & 1), &s_abort);
+      __syncwarp();
+      if (lane == 0 && (warp & 3) == 0) mbar_arrive(empty + (2 * j) % R);  // K_j has been read
       tc::fence_after();
-      float s[BN];
-      {
-        uint32_t r[64];
-        tc::ld64(t_s, r);
-#pragma unroll
-        for (int c = 0; c < 64; ++c) s[c] = __uint_as_float(r[c]);
-        tc::ld64(t_s + 64, r);
-#pragma unroll
-        for (int c = 0; c < 64; ++c) s[64 + c] = __uint_as_float(r[c]);
-      }
+      uint32_t s[BN];
+      tc::ld128(t_s, s);
       if (__any_sync(0xffffffffu, lim < BN)) {
 #pragma unroll
-        for (int c = 0; c < BN; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+        for (int c = 0; c < BN; ++c) s[c] = c < lim ? s[c] : 0xff800000u;
       }
-      float mx = -INFINITY;
+      auto at = [&](int c) { return __uint_as_float(s[c]); };
+      float mx4[4];
 #pragma unroll
-      for (int c = 0; c < BN; ++c) mx = fmaxf(mx, s[c]);
+      for (int q = 0; q < 4; ++q) mx4[q] = max3(at(q), at(q + 4), at(q + 8));
+#pragma unroll
+      for (int c = 12; c + 8 <= BN; c += 8)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx4[q] = max3(mx4[q], at(c + q), at(c + q + 4));
+      float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], at(BN - 4));
+      mx = max3(max3(mx, at(BN - 3), at(BN - 2)), at(BN - 1), mx);
       // raised lazily; the first maximum costs no rescaling (O has not been written: P V of the
-      // first block overwrites it, and rows that saw nothing so far hold zeros)
+      // first block overwrites it, and rows that saw nothing so far hold zeros).  A NaN score makes
+      // the maximum, and with it the row's sum and output, NaN.
       float corr = 1.f;
       bool rescale = false;
-      if (mx > m_run) {
+      if (!(mx <= m_run)) {
         if (m_run == -INFINITY) {
           m_run = mx;
-        } else if ((mx - m_run) * sl2 > RESCALE_LOG2) {
+        } else if (!((mx - m_run) * sl2 <= RESCALE_LOG2)) {
           corr = ex2((m_run - mx) * sl2);
           l_run *= corr;
           m_run = mx;
@@ -351,91 +406,109 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       }
       if (j > 0 && __any_sync(0xffffffffu, rescale)) {  // P V_{j-1} has completed: S_j was issued after it
 #pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t r[32];
-          tc::ld32(t_o + c0, r);
+        for (int c0 = 0; c0 < D; c0 += 16) {
+          uint32_t r[16];
+          tc::ld16(t_o + c0, r);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * corr);
-          tc::st32(t_o + c0, r);
+          for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * corr);
+          tc::st16(t_o + c0, r);
         }
       }
-      const float ms = m_run == -INFINITY ? 0.f : m_run * sl2;
-      float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-      for (int c0 = 0; c0 < BN; c0 += 64) {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float p0 = ex2(fmaf(s[c0 + 2 * c], sl2, -ms)), p1 = ex2(fmaf(s[c0 + 2 * c + 1], sl2, -ms));
-          sum0 += p0;
-          sum1 += p1;
-          w[c] = pack_bf16(p0, p1);
-        }
-        tc::st32(t_s + c0 / 2, w);
-      }
-      l_run += sum0 + sum1;
       const int seen = block_seen(blk);
-      if (i == 0 && seen < BN) {  // value rows that no query of the CTA sees: zero
+      if (seen < BN) {  // value rows that no query of the CTA sees: zero, before this tile's weights are handed on
+                        // (each tile for itself: with two, both write the same zeros)
         const int vt = 2 * j + 1;
-        ok = wait(full + vt % R, (uint32_t)((vt / R) & 1), &s_abort);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        ok &= wait(full + vt % R, (uint32_t)((vt / R) & 1), &s_abort);
         uint8_t* v = smem + C::OFF_RING + (vt % R) * C::TILE;
         for (int e = seen * (D / 8) + row; e < BN * (D / 8); e += BM) {
           const int r = e / (D / 8), c = e % (D / 8);
           *reinterpret_cast<uint4*>(v + (c / 8) * C::BOX + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
+        __syncwarp();
       }
-      tc::fence_before();
-      mbar_arrive(p_full + i);
+      const float ms = m_run == -INFINITY ? 0.f : m_run * sl2;
+      const f2 sl2x2 = pack2(sl2, sl2), msx2 = pack2(-ms, -ms);
+      f2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        constexpr int W = BN / 4;  // 32-bit words of two weights each
+        uint32_t w[W];
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+          const int k = half * 2 * W + 2 * c;
+          const f2 x = fma2(pack2(at(k), at(k + 1)), sl2x2, msx2);
+          float p0, p1;
+          unpack2(x, p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          sum[c & 1] = add2(sum[c & 1], pack2(p0, p1));
+          w[c] = pack_bf16(p0, p1);
+        }
+        tc::st32(t_s + half * W, w);
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(half == 0 ? p_half + i : p_full + i);
+      }
+      float sums[4];
+      unpack2(sum[0], sums[0], sums[1]);
+      unpack2(sum[1], sums[2], sums[3]);
+      l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
-    if (ok && n > 0) {
-      ok = wait(o_full + i, (uint32_t)((n - 1) & 1), &s_abort);
-      ok = __all_sync(0xffffffffu, ok);
-    }
-    if (ok) {
+    if (n > 0) ok &= wait(o_full + i, (uint32_t)((n - 1) & 1), &s_abort);
+    // every tile's last product has completed: the ring is idle and takes the outputs
+    asm volatile("bar.sync 1, %0;\n" ::"n"(C::SOFTMAX) : "memory");
+    if (__all_sync(0xffffffffu, ok)) {
       tc::fence_after();
       const bool any = m_run != -INFINITY;  // else nothing of this range is visible to the row
       const int64_t bt = (int64_t)b * a.T + t;
-      if (a.part_o != nullptr) {
-        const int64_t at = (bt * a.H + h) * a.n_slots + a.slot0 + blockIdx.y;
-        if (live) {
-          a.part_ml[2 * at] = any ? m_run * a.scale : -INFINITY;
-          a.part_ml[2 * at + 1] = l_run;
-        }
-        if (n > 0) {
-#pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t r[32];
-            tc::ld32(t_o + c0, r);
-            if (live && any) {
-#pragma unroll
-              for (int c = 0; c < 32; c += 4)
-                *reinterpret_cast<uint4*>(a.part_o + at * D + c0 + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
-            }
-          }
-        }
-      } else {
-        const float inv = any ? 1.f / l_run : 0.f;
-        __nv_bfloat16* dst = a.out + (bt * a.H + h) * D;
-#pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t r[32];
-          if (n > 0) tc::ld32(t_o + c0, r);
-          if (live) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = any ? pack_bf16(__uint_as_float(r[c + 2 * e]) * inv, __uint_as_float(r[c + 2 * e + 1]) * inv) : 0u;
-              *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
-        }
-        if (live && a.lse != nullptr)
+      const int64_t slot = (bt * a.H + h) * a.n_slots + a.slot0 + blockIdx.y;
+      const bool partial = a.part_o != nullptr;
+      if (live) {
+        if (partial) {
+          *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(any ? m_run * a.scale : -INFINITY, l_run);
+        } else if (a.lse != nullptr) {
           a.lse[((int64_t)b * a.H + h) * a.T + t] = any ? m_run * a.scale + logf(l_run) : -INFINITY;
+        }
+      }
+      // The warp's 32 rows go through shared memory: a thread has one row, a store instruction should
+      // write whole rows.  Pieces of 16 bytes, swizzled within 128 bytes.
+      const float inv = partial || !any ? 1.f : 1.f / l_run;
+      uint8_t* stage = smem + C::OFF_RING + warp * C::STAGE;
+      constexpr int PIECES = D / 4;  // fp32 pieces of a row
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t r[16];
+        if (n > 0) tc::ld16(t_o + c0, r);
+        auto val = [&](int c) { return n > 0 && any ? __uint_as_float(r[c]) * inv : 0.f; };
+        if (partial) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) {
+            const int piece = (c0 + c) / 4;
+            *reinterpret_cast<float4*>(stage + lane * PIECES * 16 + ((piece ^ (lane & 7)) << 4)) =
+                make_float4(val(c), val(c + 1), val(c + 2), val(c + 3));
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; c += 8) {
+            const int piece = (c0 + c) / 8;
+            *reinterpret_cast<uint4*>(stage + lane * PIECES * 8 + ((piece ^ (lane & 7)) << 4)) =
+                make_uint4(pack_bf16(val(c), val(c + 1)), pack_bf16(val(c + 2), val(c + 3)),
+                           pack_bf16(val(c + 4), val(c + 5)), pack_bf16(val(c + 6), val(c + 7)));
+          }
+        }
+      }
+      __syncwarp();
+      const int per_row = partial ? PIECES : PIECES / 2;  // 16-byte pieces of a row, 8 to 32
+      const int rows_at_once = 32 / per_row;
+      const int64_t base = partial ? slot * D : (bt * a.H + h) * D;
+      for (int r0 = 0; r0 < 32; r0 += rows_at_once) {
+        const int r = r0 + lane / per_row, piece = lane % per_row;
+        const int64_t to = __shfl_sync(0xffffffffu, base, r);
+        if (!__shfl_sync(0xffffffffu, live ? 1 : 0, r)) continue;
+        const uint4 val = *reinterpret_cast<const uint4*>(stage + (r * per_row + (piece ^ (r & 7))) * 16);
+        if (partial) *reinterpret_cast<uint4*>(a.part_o + to + piece * 4) = val;
+        else *reinterpret_cast<uint4*>(a.out + to + piece * 8) = val;
       }
     }
   }
@@ -448,41 +521,62 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       tc::mbar_wait_cycles(full + x % R, (uint32_t)((x / R) & 1), WAIT_CYCLES);
     __syncthreads();
   }
-  if (warp == NT * 4) {
+  if (warp == PRODUCER) {
     tc::fence_after();
     tc::dealloc(tmem, C::COLS);
   }
 }
 
-// One warp per (b, t, h): the partials weighted by their own maxima and summed in slot order.
-constexpr int MERGE_WARPS = 8;
+// One warp per (b, t, h): the partials weighted by their own maxima and summed in slot order.  Lane s
+// holds the weight of slot s (32 slots at a time), so the sums' loads wait for nothing but the maxima.
+constexpr int MERGE_WARPS = 4;
 template <int D>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(PrefixMergeArgs a) {
   constexpr int E = D / 32;
   const int64_t at = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (at >= (int64_t)a.B * a.T * a.H) return;
-  const float* sets_ml[2] = {a.part_ml + at * a.n_slots * 2, a.more_ml + at * a.n_more * 2};
+  const float2* sets_ml[2] = {reinterpret_cast<const float2*>(a.part_ml) + at * a.n_slots,
+                              reinterpret_cast<const float2*>(a.more_ml) + at * a.n_more};
   const float* sets_o[2] = {a.part_o + at * a.n_slots * D + lane * E, a.more_o + at * a.n_more * D + lane * E};
   const int counts[2] = {a.n_slots, a.more_o != nullptr ? a.n_more : 0};
   float M = -INFINITY;
 #pragma unroll
   for (int g = 0; g < 2; ++g)
-    for (int s = lane; s < counts[g]; s += 32) M = fmaxf(M, sets_ml[g][2 * s]);
+    for (int s = lane; s < counts[g]; s += 32) M = fmaxf(M, sets_ml[g][s].x);
   M = warp_max(M);
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
   for (int g = 0; g < 2; ++g)
-    for (int s = 0; s < counts[g]; ++s) {
-      const float m = sets_ml[g][2 * s];
-      if (m == -INFINITY) continue;  // nothing visible: its part of the workspace was not written
-      const float w = exp2f((m - M) * LOG2E);
-      L += w * sets_ml[g][2 * s + 1];
+    for (int s0 = 0; s0 < counts[g]; s0 += 32) {
+      float w = 0.f;
+      if (s0 + lane < counts[g]) {
+        const float2 ml = sets_ml[g][s0 + lane];
+        if (ml.x != -INFINITY) {
+          w = exp2f((ml.x - M) * LOG2E);
+          L += w * ml.y;
+        }
+      }
+      const int n = min(32, counts[g] - s0);
+      for (int s = 0; s < n; s += 4) {  // four slots' loads in flight
+        float ws[4], v[4][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += w * sets_o[g][(int64_t)s * D + e];
+        for (int q = 0; q < 4; ++q) {
+          ws[q] = __shfl_sync(0xffffffffu, w, (s + q) & 31);
+          if (s + q >= n) ws[q] = 0.f;
+          const float* o = sets_o[g] + (int64_t)(s0 + s + q) * D;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[q][e] = ws[q] != 0.f ? o[e] : 0.f;  // 0: nothing visible (not written), or too small to count
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += ws[q] * v[q][e];
+      }
     }
+  L = warp_sum(L);
   const bool any = M != -INFINITY;
   const float inv = any ? 1.f / L : 0.f;
   if (a.out != nullptr) {

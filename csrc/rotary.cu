@@ -11,7 +11,7 @@
 // Bound by bytes: x is read and y written once, the table adds 4 R bytes per token.  A thread owns
 // one unit (V pairs: two 16-byte vectors, at u V and R/2 + u V or side by side) of one token and
 // walks the heads with it, so a unit's cosines and sines are read once for several heads and all
-// loads of HPT heads are in flight together.  Vectors need R and D - R to be multiples of 2 V
+// loads of two heads are in flight together.  Vectors need R and D - R to be multiples of 2 V
 // and 16-byte aligned rows; other calls take V = 2 or 1.
 #include "common.cuh"
 #include "serving.h"
@@ -45,9 +45,9 @@ struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
 
-template <typename T, int V, int HPT>
-__global__ void __launch_bounds__(NT) rotary_kernel(const RotaryArgs a, int units, int unit_lanes, int head_lanes,
-                                                    int tokens_per_block) {
+template <typename T, int V>
+__global__ void __launch_bounds__(NT, 4) rotary_kernel(const RotaryArgs a, int units, int unit_lanes, int head_lanes,
+                                                       int tokens_per_block) {
   const int per = unit_lanes * head_lanes;
   const int lt = threadIdx.x / per;
   const int64_t m = (int64_t)blockIdx.x * tokens_per_block + lt;
@@ -55,7 +55,6 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const RotaryArgs a, int unit
   const int rem = threadIdx.x - lt * per;
   const int hl = rem / unit_lanes;
   const int half = a.rot / 2, rot_units = half / V;
-  const int heads = a.seg[0].heads + a.seg[1].heads + a.seg[2].heads;
   const int64_t pos = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[m] : reinterpret_cast<const int*>(a.pos)[m];
   const bool pos_ok = pos >= 0 && pos < a.max_pos;  // outside the table: the rotated part becomes NaN
   int64_t slot = m;
@@ -76,61 +75,36 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const RotaryArgs a, int unit
     }
     float c[V], s[V];
     if (turns) {
-      if (pos_ok) {
-        const Vec<float, V < 4 ? V : 4>* ct =
-            reinterpret_cast<const Vec<float, V < 4 ? V : 4>*>(a.cos_t + pos * half + u * V);
-        const Vec<float, V < 4 ? V : 4>* st =
-            reinterpret_cast<const Vec<float, V < 4 ? V : 4>*>(a.sin_t + pos * half + u * V);
+      constexpr int F = V < 4 ? V : 4;
+      const Vec<float, F>* ct = reinterpret_cast<const Vec<float, F>*>(a.cos_t + (pos_ok ? pos : 0) * half + u * V);
+      const Vec<float, F>* st = reinterpret_cast<const Vec<float, F>*>(a.sin_t + (pos_ok ? pos : 0) * half + u * V);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          c[j] = ct[j / 4].v[j % 4];
-          s[j] = st[j / 4].v[j % 4];
+      for (int j = 0; j < V / F; ++j) {
+        const Vec<float, F> cv = ct[j], sv = st[j];
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+          c[j * F + i] = pos_ok ? cv.v[i] : __int_as_float(0x7fffffff);
+          s[j * F + i] = pos_ok ? (a.inverse ? -sv.v[i] : sv.v[i]) : __int_as_float(0x7fffffff);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) c[j] = s[j] = __int_as_float(0x7fffffff);
-      }
-      if (a.inverse) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = -s[j];
       }
     }
-    for (int h0 = hl; h0 < heads; h0 += HPT * head_lanes) {
-      Vec<T, V> x0[HPT], x1[HPT];
-      T* dst[HPT];
-      bool live[HPT], rotate[HPT];
 #pragma unroll
-      for (int j = 0; j < HPT; ++j) {
-        int h = h0 + j * head_lanes, g = 0;
-        live[j] = h < heads;
-        if (!live[j]) continue;
-        if (h >= a.seg[0].heads) {
-          h -= a.seg[0].heads;
-          g = 1;
-          if (h >= a.seg[1].heads) {
-            h -= a.seg[1].heads;
-            g = 2;
-          }
-        }
-        const RotarySegment& q = a.seg[g];
-        rotate[j] = turns && q.rotate;
-        const T* src = reinterpret_cast<const T*>(q.src) + m * q.src_token + h * q.src_head;
-        dst[j] = reinterpret_cast<T*>(q.dst) + (q.to_slot ? slot : m) * q.dst_token + h * q.dst_head;
-        live[j] = !q.to_slot || slot_ok;
-        if (!live[j]) continue;
-        x0[j] = *reinterpret_cast<const Vec<T, V>*>(src + o0);
-        x1[j] = *reinterpret_cast<const Vec<T, V>*>(src + o1);
-      }
-#pragma unroll
-      for (int j = 0; j < HPT; ++j) {
-        if (!live[j]) continue;
-        if (rotate[j]) {
-          if (a.interleaved) {
-            // pair i of the unit is elements (2i, 2i + 1) of the two vectors side by side
+    for (int g = 0; g < 3; ++g) {
+      const RotarySegment& q = a.seg[g];
+      if (q.heads == 0 || (q.to_slot && !slot_ok)) continue;
+      const bool rotate = turns && q.rotate;
+      const T* src = reinterpret_cast<const T*>(q.src) + m * q.src_token;
+      T* dst = reinterpret_cast<T*>(q.dst) + (q.to_slot ? slot : m) * q.dst_token;
+#pragma unroll 2
+      for (int h = hl; h < q.heads; h += head_lanes) {
+        Vec<T, V> x0 = *reinterpret_cast<const Vec<T, V>*>(src + h * q.src_head + o0);
+        Vec<T, V> x1 = *reinterpret_cast<const Vec<T, V>*>(src + h * q.src_head + o1);
+        if (rotate) {
+          if (a.interleaved) {  // pair i of the unit is elements (2i, 2i + 1) of the two vectors side by side
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              T& e0 = 2 * i < V ? x0[j].v[(2 * i) % V] : x1[j].v[(2 * i) % V];
-              T& e1 = 2 * i + 1 < V ? x0[j].v[(2 * i + 1) % V] : x1[j].v[(2 * i + 1) % V];
+              T& e0 = 2 * i < V ? x0.v[(2 * i) % V] : x1.v[(2 * i) % V];
+              T& e1 = 2 * i + 1 < V ? x0.v[(2 * i + 1) % V] : x1.v[(2 * i + 1) % V];
               const float p0 = to_f(e0), p1 = to_f(e1);
               e0 = from_f<T>(p0 * c[i] - p1 * s[i]);
               e1 = from_f<T>(p1 * c[i] + p0 * s[i]);
@@ -138,14 +112,14 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const RotaryArgs a, int unit
           } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const float p0 = to_f(x0[j].v[i]), p1 = to_f(x1[j].v[i]);
-              x0[j].v[i] = from_f<T>(p0 * c[i] - p1 * s[i]);
-              x1[j].v[i] = from_f<T>(p1 * c[i] + p0 * s[i]);
+              const float p0 = to_f(x0.v[i]), p1 = to_f(x1.v[i]);
+              x0.v[i] = from_f<T>(p0 * c[i] - p1 * s[i]);
+              x1.v[i] = from_f<T>(p1 * c[i] + p0 * s[i]);
             }
           }
         }
-        *reinterpret_cast<Vec<T, V>*>(dst[j] + o0) = x0[j];
-        *reinterpret_cast<Vec<T, V>*>(dst[j] + o1) = x1[j];
+        *reinterpret_cast<Vec<T, V>*>(dst + h * q.dst_head + o0) = x0;
+        *reinterpret_cast<Vec<T, V>*>(dst + h * q.dst_head + o1) = x1;
       }
     }
   }
@@ -153,18 +127,18 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const RotaryArgs a, int unit
 
 template <typename T, int V>
 cudaError_t launch(const RotaryArgs& a, cudaStream_t st) {
-  const int heads = a.seg[0].heads + a.seg[1].heads + a.seg[2].heads;
+  const int heads = std::max(a.seg[0].heads, std::max(a.seg[1].heads, a.seg[2].heads));
   const int units = a.head_dim / (2 * V);
   const int unit_lanes = std::min(units, NT);
-  // one head per thread spreads a small call over more threads; four keep more loads in flight
+  // one head of the widest segment per thread spreads a small call over more threads; four share
+  // a unit's cosines and sines
   const bool small = a.tokens * (int64_t)units * heads < (int64_t)148 * 2048 * 4;
   const int hpt = small ? 1 : 4;
   const int head_lanes = std::max(1, std::min((heads + hpt - 1) / hpt, NT / unit_lanes));
   const int tpb = std::max(1, NT / (unit_lanes * head_lanes));
   const int64_t blocks = (a.tokens + tpb - 1) / tpb;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  if (small) rotary_kernel<T, V, 1><<<(unsigned)blocks, NT, 0, st>>>(a, units, unit_lanes, head_lanes, tpb);
-  else rotary_kernel<T, V, 4><<<(unsigned)blocks, NT, 0, st>>>(a, units, unit_lanes, head_lanes, tpb);
+  rotary_kernel<T, V><<<(unsigned)blocks, NT, 0, st>>>(a, units, unit_lanes, head_lanes, tpb);
   return cudaGetLastError();
 }
 
