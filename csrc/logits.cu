@@ -12,13 +12,19 @@
 // largest; a row with nothing above -inf gives -1.
 //
 // Bound by bytes: each logit is read once (and written once), the history read once.  A cluster of
-// CL CTAs owns a row, one slice of the vocabulary each.  The history cannot be looked up per logit,
-// so it is turned around: a 32-bit word per token of the slice in shared memory counts its
-// occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 bias entry + 1), filled by
-// shared-memory atomics (integer: any order gives the same counts), and the pass over the logits
-// reads the words beside them.  Every CTA needs every id of the row: a long history is read once
-// per cluster, each CTA bringing its share into shared memory and reading the others' through
-// the cluster.  A thread's first logits are loaded before the table is built.
+// 1 to 8 CTAs owns a row, one slice of the vocabulary each.  The history cannot be looked up per logit,
+// so each CTA turns its slice of it around in shared memory: a bit per token that the history or a
+// bias names (their ranks by a prefix sum of the bits), and for each such token its id and a word with
+// its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 bias entry + 1).  Integer atomics fill
+// them, so any order gives the same table.  The pass over all logits then only masks and takes
+// maxima, on packed 16-bit pairs, leaving out what is named; the named tokens follow one to a
+// thread.  (Looking the penalties up within the pass over all logits took 107 us for 256 rows of
+// 152,064 logits with 8,192 ids each, a word per token of the slice instead of the table 183 us.)  A
+// thread only remembers which vector held its maximum: the element is looked up at the end, by the
+// warps' winners.  A thread's first logits and mask bytes are loaded before the table is built.
+#include <algorithm>
+#include <type_traits>
+
 #include "common.cuh"
 #include "serving.h"
 
@@ -30,13 +36,7 @@ namespace cg = cooperative_groups;
 namespace pra {
 namespace rules {
 
-#ifndef NTT
-#define NTT 512
-#endif
-#ifndef LB
-#define LB 2
-#endif
-constexpr int NT = NTT;
+constexpr int NT = 512;
 constexpr uint32_t COUNT = (1u << 20) - 1, SEEN = 1u << 20;
 
 __device__ __forceinline__ float widen(float v) { return v; }
@@ -64,98 +64,76 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   return m;
 }
 
-constexpr int STAGE = 2048;   // ids of a long history that a CTA holds for its cluster at a time
-#ifndef DIR
-#define DIR 2048
-#endif
-constexpr int DIRECT = DIR;  // up to here every CTA reads the whole history itself
+// All ones where bit j of `bits` is set, else 0.
+__device__ __forceinline__ uint32_t spread(uint32_t bits, int j) {
+  uint32_t m;
+  asm("bfe.s32 %0, %1, %2, 1;" : "=r"(m) : "r"(bits), "r"(j));
+  return m;
+}
+
+// -inf where the element's bit is 0.
+template <int V>
+__device__ __forceinline__ void mask_vec(Vec<float, V>& x, uint32_t bits) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) x.v[j] = (bits >> j) & 1u ? x.v[j] : -INFINITY;
+}
+template <typename T, int V>
+__device__ __forceinline__ void mask_vec(Vec<T, V>& x, uint32_t bits) {
+  constexpr uint32_t NEG = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+  if constexpr (V == 1) {
+    if (!(bits & 1u)) narrow(-INFINITY, x.v[0]);
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      const uint32_t m = __byte_perm(spread(bits, 2 * j), spread(bits, 2 * j + 1), 0x5410);
+      w[j] = (w[j] & m) | (NEG & ~m);
+    }
+  }
+}
+
+// The largest element (NaN if one is).
+template <int V>
+__device__ __forceinline__ float max_vec(const Vec<float, V>& x) {
+  float m = x.v[0];
+#pragma unroll
+  for (int j = 1; j < V; ++j) m = max_nan(m, x.v[j]);
+  return m;
+}
+__device__ __forceinline__ __nv_bfloat162 max_pair(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __half2 max_pair(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
+template <typename T, int V>
+__device__ __forceinline__ float max_vec(const Vec<T, V>& x) {
+  if constexpr (V == 1) {
+    return widen(x.v[0]);
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* w = reinterpret_cast<const T2*>(&x);
+    T2 m = w[0];
+#pragma unroll
+    for (int j = 1; j < V / 2; ++j) m = max_pair(m, w[j]);
+    return max_nan(widen(m.x), widen(m.y));
+  }
+}
+
+// 32-bit words of a slice's bits.
+__host__ __device__ constexpr int bit_words(int slice) { return (slice + 31) / 32; }
 
 // T: type of the logits; V: elements of one access; TABLE: a history or biases are given.
 template <typename T, int V, bool TABLE>
-__global__ void __launch_bounds__(NT, LB) rules_kernel(const LogitsArgs a, int slice) {
-  #ifndef UU
-#define UU 2
-#endif
-  constexpr int U = V == 1 ? 4 : UU;  // accesses of a thread in flight
-  extern __shared__ uint4 smem_raw[];
-  uint32_t* smem = reinterpret_cast<uint32_t*>(smem_raw);
+__global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int slice, int table_words) {
+    constexpr int U = 3;  // accesses of a batch
+  extern __shared__ uint32_t smem[];
+  __shared__ uint32_t s_scan[NT / 32];
   __shared__ unsigned long long s_best[NT / 32];
   __shared__ unsigned long long s_cluster;  // this CTA's best, read by the cluster's first CTA
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.y;
   const int v0 = part * slice, n = max(min(a.V, v0 + slice) - v0, 0);
   const T* x = reinterpret_cast<const T*>(a.logits) + (int64_t)b * a.in_stride + v0;
   T* y = a.out ? reinterpret_cast<T*>(a.out) + (int64_t)b * a.out_stride + v0 : nullptr;
-  const int vecs = n / V;
-  Vec<T, V> in[U];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i0 + u * NT < vecs) in[u] = *reinterpret_cast<const Vec<T, V>*>(x + (i0 + u * NT) * V);
-  };
-  load(threadIdx.x);
-
-  uint32_t* words = smem;                                              // [slice]
-  int* stage = reinterpret_cast<int*>(smem + (TABLE ? slice : 0));     // [STAGE], long histories only
-  const int len = a.ids ? max(0, min(a.hist_len[b], a.capacity)) : 0;
-  const bool staged = a.capacity > DIRECT;  // the same for the whole cluster
-  int* bias_id = stage + (staged ? STAGE : 0);                         // [n_bias]
-  float* bias_sum = reinterpret_cast<float*>(bias_id + a.n_bias);      // [n_bias]
-  const float rep = a.repetition ? a.repetition[b] : 1.f;
-  const float pres = a.presence ? a.presence[b] : 0.f;
-  const float freq = a.frequency ? a.frequency[b] : 0.f;
-  if constexpr (TABLE) {
-    const int prompt = a.prompt_len ? a.prompt_len[b] : 0;
-    const int* ids = a.ids + (int64_t)b * a.ids_stride;
-    const uint32_t base = (uint32_t)a.vocab_start + (uint32_t)v0;
-    uint4* w4 = reinterpret_cast<uint4*>(words);
-    for (int i = threadIdx.x; i < slice / 4; i += NT) w4[i] = make_uint4(0, 0, 0, 0);
-    for (int i = threadIdx.x; i < a.n_bias; i += NT) bias_id[i] = a.bias_ids[(int64_t)b * a.n_bias + i];
-    auto count = [&](int id, int i) {
-      const uint32_t t = (uint32_t)id - base;
-      if (t >= (uint32_t)n) return;
-      if (i < prompt) atomicOr(words + t, SEEN);
-      else atomicAdd(words + t, 1u);
-    };
-    if (!staged) {
-      __syncthreads();
-#pragma unroll 4
-      for (int i = threadIdx.x; i < len; i += NT) count(ids[i], i);
-    } else {
-      for (int i0 = 0; i0 < len; i0 += parts * STAGE) {
-        // CTA p of the cluster brings in ids [i0 + p * per, i0 + (p + 1) * per)
-        const int per = (min(len - i0, parts * STAGE) + parts - 1) / parts;
-        const int lo = i0 + part * per, mine = max(0, min(per, len - lo));
-#pragma unroll 4
-        for (int i = threadIdx.x; i < mine; i += NT) stage[i] = ids[lo + i];
-        cluster.sync();
-        for (int q = 0; q < parts; ++q) {
-          const int p = (part + q) % parts;  // each CTA begins with its own: not all read one at once
-          const int* other = cluster.map_shared_rank(stage, p);
-          const int first = i0 + p * per, there = max(0, min(per, len - first));
-#pragma unroll 4
-          for (int i = threadIdx.x; i < there; i += NT) count(other[i], first + i);
-        }
-        cluster.sync();  // the stage is refilled, or its CTA goes on
-      }
-    }
-    __syncthreads();  // the counts are whole before the bias entries join their words
-    // an entry whose id no earlier entry has owns the token and sums all its entries in list order
-    for (int i = threadIdx.x; i < a.n_bias; i += NT) {
-      const uint32_t t = (uint32_t)bias_id[i] - base;
-      if (t >= (uint32_t)n) continue;
-      bool first = true;
-      for (int j = 0; j < i && first; ++j) first = bias_id[j] != bias_id[i];
-      if (!first) continue;
-      float sum = 0.f;
-      for (int j = i; j < a.n_bias; ++j)
-        if (bias_id[j] == bias_id[i]) sum += a.bias_values[(int64_t)b * a.n_bias + j];
-      bias_sum[i] = sum;
-      atomicOr(words + t, (uint32_t)(i + 1) << 21);
-    }
-    __syncthreads();
-  }
   // the row's mask as bytes: element e of the slice is bit (vocab_start + v0 + e) % 8 of its byte
   const uint8_t* mask = nullptr;
   bool none = false;  // a mask row outside the masks allows nothing
@@ -165,76 +143,200 @@ __global__ void __launch_bounds__(NT, LB) rules_kernel(const LogitsArgs a, int s
     if (r >= 0 && !none)
       mask = reinterpret_cast<const uint8_t*>(a.mask + r * a.mask_words) + (a.vocab_start + v0) / 8;
   }
-  const bool choose = a.token != nullptr;
-  float best = -INFINITY;  // largest so far, and its element: strictly larger ones replace it, in ascending order
-  int best_e = 0;
-  // The rules on V logits at element e of the slice.
-  auto apply = [&](Vec<T, V> raw, int e) {
-    float z[V];
+  const int vecs = n / V;
+  struct Batch {
+    Vec<T, V> x[U];
+    uint32_t allowed[U];
+  } here, next;  // one being worked on, one on its way
+  auto load = [&](Batch& q, int i0) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) z[j] = widen(raw.v[j]);
-    bool changed = false;
-    if constexpr (TABLE) {
-      const Vec<uint32_t, V> w = *reinterpret_cast<const Vec<uint32_t, V>*>(words + e);
-      uint32_t any = 0;
-#pragma unroll
-      for (int j = 0; j < V; ++j) any |= w.v[j];
-      if (any) {
-        changed = true;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (w.v[j] & (SEEN | COUNT)) z[j] = z[j] > 0.f ? __fdiv_rn(z[j], rep) : __fmul_rn(z[j], rep);
-          const uint32_t times = w.v[j] & COUNT;
-          if (times) z[j] = __fsub_rn(__fsub_rn(z[j], __fmul_rn(freq, (float)times)), pres);
-          if (w.v[j] >> 21) z[j] = __fadd_rn(z[j], bias_sum[(w.v[j] >> 21) - 1]);
-        }
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * NT;
+      q.allowed[u] = none ? 0u : 0xFFu;
+      if (i < vecs) {
+        q.x[u] = *reinterpret_cast<const Vec<T, V>*>(x + i * V);
+        if (mask) q.allowed[u] = mask[i * V / 8] >> (i * V & 7);
       }
-    }
-    uint32_t bits = none ? 0u : 0xFFFFFFFFu;
-    if (mask) bits = mask[e / 8] >> (e & 7);
-    if ((~bits & ((1u << V) - 1)) != 0) {
-      changed = true;
-#pragma unroll
-      for (int j = 0; j < V; ++j) z[j] = (bits >> j) & 1u ? z[j] : -INFINITY;
-    }
-    if (choose) {
-      float m = z[0];
-#pragma unroll
-      for (int j = 1; j < V; ++j) m = max_nan(m, z[j]);
-      if (!(m <= best) && best == best) {
-#pragma unroll
-        for (int j = V - 1; j >= 0; --j)
-          if (z[j] == m || (m != m && z[j] != z[j])) best_e = e + j;
-        best = m;
-      }
-    }
-    if (y) {
-      if (changed) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) narrow(z[j], raw.v[j]);
-      }
-      *reinterpret_cast<Vec<T, V>*>(y + e) = raw;
     }
   };
-  for (int i0 = threadIdx.x; i0 < vecs; i0 += U * NT) {
-    if (i0 != (int)threadIdx.x) load(i0);
+  load(here, tid);
+
+  uint32_t* named = smem;                                       // [bit_words(slice)] tokens with a table word
+  uint32_t* rank = named + bit_words(slice);                    // [bit_words(slice)] table words before
+  uint32_t* table = rank + bit_words(slice);                    // [table_words]
+  uint32_t* token = table + table_words;                        // [table_words] their elements of the slice
+  int* bias_id = reinterpret_cast<int*>(token + table_words);   // [n_bias]
+  float* bias_sum = reinterpret_cast<float*>(bias_id + a.n_bias);
+  const int len = a.ids ? max(0, min(a.hist_len[b], a.capacity)) : 0;
+  const float rep = a.repetition ? a.repetition[b] : 1.f;
+  const float pres = a.presence ? a.presence[b] : 0.f;
+  const float freq = a.frequency ? a.frequency[b] : 0.f;
+  auto entry_of = [&](uint32_t t) { return rank[t >> 5] + __popc(named[t >> 5] & ((1u << (t & 31)) - 1u)); };
+  int named_tokens = 0;
+  if constexpr (TABLE) {
+    const int prompt = a.prompt_len ? a.prompt_len[b] : 0;
+    const int* ids = a.ids + (int64_t)b * a.ids_stride;
+    const uint32_t base = (uint32_t)a.vocab_start + (uint32_t)v0;
+    const int words = bit_words(slice);
+    for (int i = tid; i < words; i += NT) named[i] = 0;
+    for (int i = tid; i < table_words; i += NT) table[i] = 0;
+    for (int i = tid; i < a.n_bias; i += NT) bias_id[i] = a.bias_ids[(int64_t)b * a.n_bias + i];
+    __syncthreads();
+    auto name = [&](int id) {
+      const uint32_t t = (uint32_t)id - base, bit = 1u << (t & 31);
+      if (t < (uint32_t)n && !(named[t >> 5] & bit)) atomicOr(named + (t >> 5), bit);
+    };
+    // every id of the row, four to a load where the row is aligned (the second walk finds them in L1)
+    const bool quads = (reinterpret_cast<uintptr_t>(ids) & 15) == 0;
+    auto walk = [&](auto visit) {
+      int done = 0;
+      if (quads) {
+        done = len & ~3;
+#pragma unroll 2
+        for (int i = tid * 4; i < done; i += NT * 4) {
+          const int4 q = *reinterpret_cast<const int4*>(ids + i);
+          visit(q.x, i);
+          visit(q.y, i + 1);
+          visit(q.z, i + 2);
+          visit(q.w, i + 3);
+        }
+      }
+#pragma unroll 4
+      for (int i = done + tid; i < len; i += NT) visit(ids[i], i);
+    };
+    walk([&](int id, int) { name(id); });
+    for (int i = tid; i < a.n_bias; i += NT) name(bias_id[i]);
+    __syncthreads();
+    {  // exclusive prefix sum of the words' bit counts, each thread a run of words
+      const int per = (words + NT - 1) / NT, first = min(tid * per, words), last = min(first + per, words);
+      uint32_t mine = 0;
+      for (int i = first; i < last; ++i) mine += __popc(named[i]);
+      uint32_t upto = mine;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i0 + u * NT < vecs) apply(in[u], (i0 + u * NT) * V);
-  }
-  unsigned long long key = choice_key(best, (uint32_t)(a.vocab_start + v0 + best_e));
-  for (int e = vecs * V + threadIdx.x; e < n; e += NT) {  // fewer than V elements at the end of the last slice
-    float z = widen(x[e]);
-    if constexpr (TABLE) {
-      const uint32_t w = words[e], times = w & COUNT;
-      if (w & (SEEN | COUNT)) z = z > 0.f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
-      if (times) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)times)), pres);
-      if (w >> 21) z = __fadd_rn(z, bias_sum[(w >> 21) - 1]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) s_scan[warp] = upto;
+      __syncthreads();
+      uint32_t at = upto - mine;
+      for (int w = 0; w < warp; ++w) at += s_scan[w];
+      for (int i = first; i < last; ++i) {
+        rank[i] = at;
+        at += __popc(named[i]);
+      }
+      for (int w = 0; w < NT / 32; ++w) named_tokens += s_scan[w];
+      __syncthreads();
     }
-    if (none || (mask && !(mask[e / 8] >> (e & 7) & 1))) z = -INFINITY;
-    const unsigned long long k = choice_key(z, (uint32_t)(a.vocab_start + v0 + e));
-    key = k > key ? k : key;
+    walk([&](int id, int i) {
+      const uint32_t t = (uint32_t)id - base;
+      if (t >= (uint32_t)n) return;
+      const uint32_t at = entry_of(t);
+      token[at] = t;  // every occurrence writes the same
+      if (i >= prompt) atomicAdd(table + at, 1u);
+      else if (!(table[at] & SEEN)) atomicOr(table + at, SEEN);
+    });
+    // an entry whose id no earlier entry has owns the token and sums all its entries in list order
+    for (int i = tid; i < a.n_bias; i += NT) {
+      const uint32_t t = (uint32_t)bias_id[i] - base;
+      if (t >= (uint32_t)n) continue;
+      bool first = true;
+      for (int j = 0; j < i && first; ++j) first = bias_id[j] != bias_id[i];
+      if (!first) continue;
+      float sum = 0.f;
+      for (int j = i; j < a.n_bias; ++j)
+        if (bias_id[j] == bias_id[i]) sum += a.bias_values[(int64_t)b * a.n_bias + j];
+      bias_sum[i] = sum;
+      token[entry_of(t)] = t;
+      atomicOr(table + entry_of(t), (uint32_t)(i + 1) << 21);
+    }
+    __syncthreads();
+  }
+  const bool choose = a.token != nullptr;
+  float best = -INFINITY;  // largest so far, and the first vector that has it
+  int best_i = 0;
+  // The bits of the vector's elements that this pass chooses among: allowed, and not named.
+  auto choosable = [&](uint32_t bits, int e) {
+    if constexpr (TABLE) bits &= ~(named[e >> 5] >> (e & 31));
+    return bits;
+  };
+  auto apply = [&](Batch& q, int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * NT;
+      if (i >= vecs) continue;
+      if (choose) {
+        if (TABLE || mask || none) mask_vec(q.x[u], choosable(q.allowed[u], i * V));
+        const float m = max_vec(q.x[u]);
+        if (!(m <= best) && best == best) {
+          best = m;
+          best_i = i;
+        }
+      }
+      if (y) {
+        if (mask || none) mask_vec(q.x[u], q.allowed[u]);
+        *reinterpret_cast<Vec<T, V>*>(y + i * V) = q.x[u];
+      }
+    }
+  };
+  for (int i0 = tid; i0 < vecs; i0 += 2 * U * NT) {
+    load(next, i0 + U * NT);
+    apply(here, i0);
+    load(here, i0 + 2 * U * NT);
+    apply(next, i0 + U * NT);
+  }
+  // the warp's largest value; the lanes that have it look for their element
+  unsigned long long key = 0;
+  if (choose) {
+    const uint32_t mine = (uint32_t)(choice_key(best, 0) >> 32);
+    if (mine == __reduce_max_sync(0xffffffffu, mine) && best_i < vecs) {
+      Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(x + best_i * V);
+      uint32_t bits = none ? 0u : 0xFFu;
+      if (mask) bits = mask[best_i * V / 8] >> (best_i * V & 7);
+      mask_vec(raw, choosable(bits, best_i * V));
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const unsigned long long k = choice_key(widen(raw.v[j]), (uint32_t)(a.vocab_start + v0 + best_i * V + j));
+        key = k > key ? k : key;
+      }
+    }
+  }
+  auto is_allowed = [&](int e) { return !none && (!mask || (mask[e / 8] >> (e & 7) & 1)); };
+  for (int e = vecs * V + tid; e < n; e += NT) {  // fewer than V elements at the end of the last slice
+    if (TABLE && ((named[e >> 5] >> (e & 31)) & 1u)) continue;
+    const float z = is_allowed(e) ? widen(x[e]) : -INFINITY;
+    if (choose) {
+      const unsigned long long k = choice_key(z, (uint32_t)(a.vocab_start + v0 + e));
+      key = k > key ? k : key;
+    }
     if (y) narrow(z, y[e]);
+  }
+  if constexpr (TABLE) {
+    // the named tokens, after their vectors have been written (in place, an allowed one is still as it came)
+    if (y) __syncthreads();
+    for (int i0 = tid; i0 < named_tokens; i0 += 4 * NT) {
+      float z4[4];  // four scattered logits on their way
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + u * NT < named_tokens) z4[u] = widen(x[token[i0 + u * NT]]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * NT;
+        if (i >= named_tokens) break;
+        const uint32_t w = table[i], times = w & COUNT;
+        const int e = token[i];
+        float z = z4[u];
+        if (w & (SEEN | COUNT)) z = z > 0.f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
+        if (times) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)times)), pres);
+        if (w >> 21) z = __fadd_rn(z, bias_sum[(w >> 21) - 1]);
+        if (!is_allowed(e)) z = -INFINITY;
+        if (choose) {
+          const unsigned long long k = choice_key(z, (uint32_t)(a.vocab_start + v0 + e));
+          key = k > key ? k : key;
+        }
+        if (y) narrow(z, y[e]);
+      }
+    }
   }
   if (choose) {
 #pragma unroll
@@ -242,28 +344,33 @@ __global__ void __launch_bounds__(NT, LB) rules_kernel(const LogitsArgs a, int s
       const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
       key = other > key ? other : key;
     }
-    if ((threadIdx.x & 31) == 0) s_best[threadIdx.x >> 5] = key;
+    if (lane == 0) s_best[warp] = key;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < NT / 32; ++w) key = s_best[w] > key ? s_best[w] : key;
-      s_cluster = key;
+    if (warp == 0) {
+      key = lane < NT / 32 ? s_best[lane] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+        key = other > key ? other : key;
+      }
+      if (lane == 0) s_cluster = key;
     }
     cluster.sync();
-    if (part == 0 && threadIdx.x < 32) {
-      unsigned long long other = (int)threadIdx.x < parts ? *cluster.map_shared_rank(&s_cluster, (int)threadIdx.x) : 0;
+    if (part == 0 && warp == 0) {
+      unsigned long long other = lane < parts ? *cluster.map_shared_rank(&s_cluster, lane) : 0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const unsigned long long k = __shfl_xor_sync(0xffffffffu, other, o);
         other = k > other ? k : other;
       }
-      if (threadIdx.x == 0) {
+      if (lane == 0) {
         const uint32_t k = (uint32_t)(other >> 32);
         const float z = k == 0xFFFFFFFFu ? __int_as_float(0x7fffffff) : __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
         const int64_t id = 0xFFFFFFFFu - (uint32_t)other;
         const bool any = z != -INFINITY;
         a.token[b] = any ? id : -1;
         if (a.value) a.value[b] = z;
-        if (a.append_ids && any && len < a.capacity) {  // every CTA of the row has read its length by now
+        if (a.append_ids && any && len < a.capacity) {  // every CTA of the row has read its history by now
           a.append_ids[(int64_t)b * a.ids_stride + len] = (int)id;
           a.hist_len[b] = len + 1;
         }
@@ -275,11 +382,27 @@ __global__ void __launch_bounds__(NT, LB) rules_kernel(const LogitsArgs a, int s
 
 template <typename T, int V, bool TABLE>
 cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
-  const int cl = 8;
-  const int slice = ((a.V + cl - 1) / cl + 15) / 16 * 16;
-  const size_t bytes = TABLE ? (size_t)slice * 4 + (a.capacity > DIRECT ? STAGE * 4 : 0) + (size_t)a.n_bias * 8 : 0;
+  // One wave of two CTAs per SM: rows in 8 slices while few, whole rows (every id then read once, no
+  // exchange) when many; more slices again where the table would leave one CTA per SM.
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int cl = 8, slice = 0, table_words = 0;
+  size_t bytes = 0;
+  const auto shape = [&](int c) {
+    cl = c;
+    slice = ((a.V + cl - 1) / cl + 31) / 32 * 32;
+    table_words = TABLE ? (int)std::min<int64_t>(slice, (int64_t)a.capacity + a.n_bias) : 0;
+    bytes = TABLE ? (size_t)bit_words(slice) * 8 + (size_t)table_words * 8 + (size_t)a.n_bias * 8 : 0;
+  };
+  shape(8);
+  while (cl > 1 && (int64_t)a.B * cl > 2 * sms) shape(cl / 2);
+  while (cl < 8 && bytes > 110 * 1024) shape(cl * 2);
+  if (bytes > 220 * 1024) shape(16);
   auto kernel = rules_kernel<T, V, TABLE>;
   if (bytes > 48 * 1024) PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), (int)bytes));
+  if (cl > 8)
+    PRA_RETURN_IF_ERROR(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cl, a.B);
   cfg.blockDim = dim3(NT);
@@ -292,7 +415,7 @@ cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a, slice);
+  return cudaLaunchKernelEx(&cfg, kernel, a, slice, table_words);
 }
 
 template <typename T>

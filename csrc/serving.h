@@ -35,7 +35,7 @@ cudaError_t pra_rotary(const RotaryArgs& a, int dtype, cudaStream_t stream);
 // ---- rules on logits (logits.cu) ---------------------------------------------------------
 constexpr int PRA_RULES_MAX_BIASES = 2047;         // entries of one row's bias list (11 bits of a table word)
 constexpr int64_t PRA_RULES_MAX_HISTORY = 1 << 20;  // history capacity (20-bit counts)
-constexpr int64_t PRA_RULES_MAX_VOCAB = 400 * 1024;  // columns of a call with a history or biases
+constexpr int64_t PRA_RULES_MAX_VOCAB = 384 * 1024;  // columns of a call with a history or biases
 struct LogitsArgs {
   const void* logits;      // [B, V] rows at stride in_stride
   void* out;               // [B, V] rows at stride out_stride, same type (may be logits), or null

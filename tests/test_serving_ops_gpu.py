@@ -378,7 +378,8 @@ def make_rules(B, V, hist, biases, mask, seed=0):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("B,V,hist,biases,mask", [(1, 1, 3, 0, False), (2, 31, 5, 3, True), (6, 1000, 0, 0, True),
                                                   (5, 4099, 64, 300, True), (3, 32768, 2000, 0, False),
-                                                  (4, 50257, 100, 17, True), (7, 128256, 700, 40, True)])
+                                                  (4, 50257, 100, 17, True), (7, 128256, 700, 40, True),
+                                                  (2, 5000, 30001, 2047, True), (1, 393216, 60000, 2047, False)])
 def test_process_and_choose(dtype, B, V, hist, biases, mask):
     from pdattention_b200.inference.logits import choose_tokens, process_logits
 
@@ -559,5 +560,5 @@ def test_refusals_of_logits_rules():
     refused(lambda: process_logits(x, LogitsRules(mask_rows=i32(B))), "without a mask")
     refused(lambda: process_logits(x, LogitsRules(), out=x[:, :50]), "shaped as")
     refused(lambda: process_logits(x.view(-1)[:100].view(1, 100), LogitsRules(), out=x.view(-1)[10:110].view(1, 100)), "overlap")
-    refused(lambda: process_logits(torch.zeros(1, 400 * 1024 + 8, device=DEV), LogitsRules(), TokenHistory(i32(1, 2), i32(1))), "columns")
+    refused(lambda: process_logits(torch.zeros(1, 384 * 1024 + 8, device=DEV), LogitsRules(), TokenHistory(i32(1, 2), i32(1))), "columns")
     refused(lambda: choose_tokens(x, LogitsRules(), append=True), "append")
