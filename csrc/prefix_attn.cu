@@ -55,7 +55,8 @@ struct Cfg {
   static constexpr int THREADS = SOFTMAX + 64;
   static constexpr int OFF_RING = NT * TILE;
   static constexpr int OFF_BAR = OFF_RING + R * TILE;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;   // + alignment slack
+  static constexpr int OFF_ROW = OFF_BAR + 256;        // [NT][BM] offsets of the rows in global memory
+  static constexpr int SMEM = OFF_ROW + NT * BM * 8 + 1024;  // + alignment slack
   static constexpr int O_COL = NT * BN;               // TMEM: S / P of tile i at i * BN, O at O_COL + i * D
   static constexpr uint32_t COLS = NT == 2 ? 512 : 256;
   static constexpr int CTAS = NT == 2 ? 1 : 2;        // per SM
@@ -327,30 +328,23 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     const int TG = a.T * G;
     const int b = it.b >= 0 ? it.b : min(qr / TG, a.B - 1);
     const int t = (qr / G) % a.T, h = it.kvh * G + qr % G;
-    // this tile's queries into shared memory (rows past the last: zero), eight loads of a thread in flight
+    // This tile's queries into shared memory (rows past the last: zero), all in flight together.  Each
+    // thread works out its own row's place once: divisions by G and T for every piece took 3 us.
+    int64_t* row_at = reinterpret_cast<int64_t*>(smem + C::OFF_ROW) + i * BM;
+    auto tile_sync = [&]() { asm volatile("bar.sync %0, 128;\n" ::"r"(2 + i) : "memory"); };
+    row_at[row] = live ? b * a.q_batch + t * a.q_token + (int64_t)h * D : -1;
+    tile_sync();
     {
       constexpr int CH = D / 8, STEP = BM / CH;
       const int c = row % CH;
-#pragma unroll
-      for (int x0 = 0; x0 < CH; x0 += 8) {
-        uint4 val[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int r = it.row0 + i * BM + row / CH + (x0 + x) * STEP;
-          val[x] = make_uint4(0, 0, 0, 0);
-          if (r < it.rows) {
-            const int bt = r / G, xb = it.b >= 0 ? it.b : bt / a.T;
-            const int xt = it.b >= 0 ? bt : bt - xb * a.T;
-            val[x] = *reinterpret_cast<const uint4*>(a.q + xb * a.q_batch + xt * a.q_token +
-                                                     (int64_t)(it.kvh * G + r - bt * G) * D + c * 8);
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int r = row / CH + (x0 + x) * STEP;
-          *reinterpret_cast<uint4*>(smem + i * C::TILE + (c / 8) * C::BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = val[x];
-        }
+      const uint32_t to = i * C::TILE + (c / 8) * C::BOX;
+#pragma unroll 4
+      for (int r = row / CH; r < BM; r += STEP) {
+        const int64_t at = row_at[r];
+        cp_async16(smem + to + r * 128 + (((c & 7) ^ (r & 7)) << 4), at >= 0 ? a.q + at + c * 8 : a.q, at >= 0);
       }
+      cp_async_commit();
+      cp_async_wait<0>();
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -474,41 +468,48 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       // The warp's 32 rows go through shared memory: a thread has one row, a store instruction should
       // write whole rows.  Pieces of 16 bytes, swizzled within 128 bytes.
       const float inv = partial || !any ? 1.f : 1.f / l_run;
+      row_at[row] = !live ? -1 : partial ? slot * D * 4 : (bt * a.H + h) * D * 2;  // bytes (read by this warp only)
       uint8_t* stage = smem + C::OFF_RING + warp * C::STAGE;
       constexpr int PIECES = D / 4;  // fp32 pieces of a row
-#pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 16) {
-        uint32_t r[16];
-        if (n > 0) tc::ld16(t_o + c0, r);
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 64) {
+        uint32_t r[64];
+        if (n > 0) tc::ld64(t_o + c0, r);
         auto val = [&](int c) { return n > 0 && any ? __uint_as_float(r[c]) * inv : 0.f; };
         if (partial) {
 #pragma unroll
-          for (int c = 0; c < 16; c += 4) {
-            const int piece = (c0 + c) / 4;
-            *reinterpret_cast<float4*>(stage + lane * PIECES * 16 + ((piece ^ (lane & 7)) << 4)) =
+          for (int c = 0; c < 64; c += 4)
+            *reinterpret_cast<float4*>(stage + lane * PIECES * 16 + (((c0 / 4 + c / 4) ^ (lane & 7)) << 4)) =
                 make_float4(val(c), val(c + 1), val(c + 2), val(c + 3));
-          }
         } else {
 #pragma unroll
-          for (int c = 0; c < 16; c += 8) {
-            const int piece = (c0 + c) / 8;
-            *reinterpret_cast<uint4*>(stage + lane * PIECES * 8 + ((piece ^ (lane & 7)) << 4)) =
+          for (int c = 0; c < 64; c += 8)
+            *reinterpret_cast<uint4*>(stage + lane * PIECES * 8 + (((c0 / 8 + c / 8) ^ (lane & 7)) << 4)) =
                 make_uint4(pack_bf16(val(c), val(c + 1)), pack_bf16(val(c + 2), val(c + 3)),
                            pack_bf16(val(c + 4), val(c + 5)), pack_bf16(val(c + 6), val(c + 7)));
-          }
         }
       }
       __syncwarp();
       const int per_row = partial ? PIECES : PIECES / 2;  // 16-byte pieces of a row, 8 to 32
       const int rows_at_once = 32 / per_row;
-      const int64_t base = partial ? slot * D : (bt * a.H + h) * D;
-      for (int r0 = 0; r0 < 32; r0 += rows_at_once) {
-        const int r = r0 + lane / per_row, piece = lane % per_row;
-        const int64_t to = __shfl_sync(0xffffffffu, base, r);
-        if (!__shfl_sync(0xffffffffu, live ? 1 : 0, r)) continue;
-        const uint4 val = *reinterpret_cast<const uint4*>(stage + (r * per_row + (piece ^ (r & 7))) * 16);
-        if (partial) *reinterpret_cast<uint4*>(a.part_o + to + piece * 4) = val;
-        else *reinterpret_cast<uint4*>(a.out + to + piece * 8) = val;
+      const int piece = lane % per_row;
+      uint8_t* dst = partial ? reinterpret_cast<uint8_t*>(a.part_o) : reinterpret_cast<uint8_t*>(a.out);
+#pragma unroll 1
+      for (int r0 = lane / per_row; r0 < 32; r0 += 8 * rows_at_once) {  // eight rows read, then written
+        int64_t at[8];
+        uint4 val[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int r = r0 + x * rows_at_once;
+          at[x] = -1;
+          if (r < 32) {
+            at[x] = row_at[(warp & 3) * 32 + r];
+            val[x] = *reinterpret_cast<const uint4*>(stage + (r * per_row + (piece ^ (r & 7))) * 16);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (at[x] >= 0) *reinterpret_cast<uint4*>(dst + at[x] + piece * 16) = val[x];
       }
     }
   }
