@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   __shared__ int s_seen;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();  // the own part, as this grid's CTAs make room, or the merge
   const int G = a.H / a.Hkv;
   constexpr int ISSUER = C::SOFTMAX / 32, PRODUCER = ISSUER + 1;  // warps
   if (tid == 0) {
@@ -528,46 +529,405 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   }
 }
 
-// One warp per (b, t, h): the partials weighted by their own maxima and summed in slot order.  Lane s
-// holds the weight of slot s (32 slots at a time), so the sums' loads wait for nothing but the maxima.
+// ---------------------------------------------------------------- own keys of few queries
+// Up to 16 query rows (t, g) of a (batch row, KV head) against its own keys: bound by reading K and V once.
+// A persistent grid of two CTAs per SM; each walks its run of 64-key blocks across items without
+// draining its pipeline: one thread streams K and V tiles (TMA, 128-byte swizzle) and the items' queries
+// (bulk copies) some stages ahead, four warps take 16 keys of every block each (mma.sync m16n8k16, the
+// queries' fragments in registers for the whole item) with their own running maximum and sum, and
+// join at the end of an item.  Equal runs of blocks keep every SM busy to the end whatever the
+// lengths: at 64 rows of 64 to 1,024 keys a CTA per (row, KV head) took 39 us, at 128 rows of 128 to 2,048
+// 65 us.
+constexpr int OB = 64;       // keys of a block
+constexpr int OWARPS = 4;
+template <int D>
+struct OwnCfg {
+  static constexpr int BOXES = D / 64, BOX = OB * 128, TILE = BOXES * BOX, STAGE = 2 * TILE;
+  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int THREADS = OWARPS * 32 + 32;
+  static constexpr int RED_LD = D / 2 + 2;  // half of the columns at a time
+  static constexpr int smem(int rows) {
+    return 1024 + STAGES * STAGE + 2 * rows * D * 2 + OWARPS * rows * RED_LD * 4 + OWARPS * rows * 8 + 256;
+  }
+};
+
+// Byte offset of (key r, column c) in a swizzled tile.
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+  return (uint32_t)((c >> 6) * (OB * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + ((c & 7) << 1));
+}
+
+__device__ __forceinline__ int own_blocks(const OwnAttnArgs& a, int b) {
+  return max(1, (max(0, min(a.len[b], a.cap)) + OB - 1) / OB);
+}
+
+template <int D>
+__global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
+    own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const OwnAttnArgs a) {
+  using C = OwnCfg<D>;
+  pdl_launch_dependents();        // the merge (it waits for this grid's end)
+  if (!a.after_prefix) pdl_wait();  // else the launch before is the prefix part's, which writes none of this one's inputs
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.H / a.Hkv, rows = a.T * G;
+  __nv_bfloat16* sq = reinterpret_cast<__nv_bfloat16*>(smem + C::STAGES * C::STAGE);  // [2][rows][D]
+  float* red = reinterpret_cast<float*>(sq + 2 * rows * D);                            // [4][rows][RED_LD]
+  float* red_ml = red + OWARPS * rows * C::RED_LD;                                     // [4][rows][2]
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], q_full[2], q_empty[2];
+  __shared__ long long s_part[C::THREADS / 32];
+  __shared__ long long s_before;
+  __shared__ int s_row, s_abort;
+  if (tid == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, OWARPS);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, OWARPS);
+    }
+    s_abort = 0;
+    s_row = -1;
+    tc::fence_mbarrier_init();
+  }
+  // blocks of all rows, and the row and first block of this CTA's run: a sum, then a scan over the lengths
+  auto block_total = [&](long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) s_part[warp] = v;
+    __syncthreads();
+    long long all = 0;
+    for (int w = 0; w < C::THREADS / 32; ++w) all += s_part[w];
+    return all;
+  };
+  long long mine = 0;
+  for (int b = tid; b < a.B; b += C::THREADS) mine += own_blocks(a, b);
+  const long long total = block_total(mine) * a.Hkv;
+  // no CTA between an item's first and last may be without a block of it: at most one CTA per block
+  const long long n = min((long long)a.ctas, total), me = min((long long)blockIdx.x, n);
+  const long long u0 = total * me / n, u1 = total * min(me + 1, n) / n;
+  for (long long b0 = 0, base = 0; b0 < a.B && u0 < u1; b0 += C::THREADS) {
+    const long long nb = b0 + tid < a.B ? (long long)own_blocks(a, (int)b0 + tid) * a.Hkv : 0;
+    long long upto = nb;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    __syncthreads();
+    if (lane == 31) s_part[warp] = upto;
+    __syncthreads();
+    long long all = 0;
+    for (int w = 0; w < C::THREADS / 32; ++w) {
+      if (w < warp) upto += s_part[w];
+      all += s_part[w];
+    }
+    if (nb > 0 && base + upto - nb <= u0 && u0 < base + upto) {
+      s_row = (int)b0 + tid;
+      s_before = base + upto - nb;
+    }
+    base += all;
+    if (base > u0) break;  // the same for every thread
+  }
+  __syncthreads();
+  const int count = s_row < 0 ? 0 : (int)(u1 - u0);
+  int issued = 0, queries = 0;  // stages and query tiles requested (the producer's counts)
+  // where a unit is: row, KV head, block of the item
+  struct Place {
+    int b, kvh, blk, blocks;
+  };
+  auto start = [&]() {
+    Place p;
+    p.b = s_row;
+    p.blocks = own_blocks(a, p.b);
+    const int at = (int)(u0 - s_before);
+    p.kvh = at / p.blocks;
+    p.blk = at - p.kvh * p.blocks;
+    return p;
+  };
+  auto advance = [&](Place& p) {  // to the next unit; true when it begins an item
+    if (++p.blk < p.blocks) return false;
+    p.blk = 0;
+    if (++p.kvh == a.Hkv) {
+      p.kvh = 0;
+      if (++p.b < a.B) p.blocks = own_blocks(a, p.b);
+    }
+    return true;
+  };
+
+  if (warp == OWARPS) {
+    if (lane == 0 && count > 0) {
+      Place p = start();
+      bool fresh = true;
+      for (int u = 0; u < count && !s_abort; ++u) {
+        if (fresh) {  // the item's queries: one run of G heads per token
+          const int slot = queries & 1;
+          if (queries > 1 && !wait(q_empty + slot, (uint32_t)((queries / 2 - 1) & 1), &s_abort)) break;
+          expect_tx(q_full + slot, rows * D * 2);
+          for (int t = 0; t < a.T; ++t)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                             smem_u32(sq + (slot * rows + t * G) * D)),
+                         "l"(a.q + p.b * a.q_batch + t * a.q_token + (int64_t)p.kvh * G * D), "r"(G * D * 2),
+                         "r"(smem_u32(q_full + slot))
+                         : "memory");
+          ++queries;
+        }
+        const int st = issued % C::STAGES;
+        if (issued >= C::STAGES && !wait(empty + st, (uint32_t)((issued / C::STAGES - 1) & 1), &s_abort)) break;
+        expect_tx(full + st, C::STAGE);
+        const uint32_t to = smem_u32(smem + st * C::STAGE);
+#pragma unroll
+        for (int x = 0; x < C::BOXES; ++x) {
+          tma_load3(to + x * C::BOX, &map_k, p.kvh * D + x * 64, p.blk * OB, p.b, full + st);
+          tma_load3(to + C::TILE + x * C::BOX, &map_v, p.kvh * D + x * 64, p.blk * OB, p.b, full + st);
+        }
+        ++issued;
+        fresh = advance(p);
+      }
+    }
+  } else if (count > 0) {
+    // After a wait that gave up the rest runs through without waiting (the barriers between warps stay
+    // matched) and nothing more is written.
+    bool ok = true;
+    Place p = start();
+    bool fresh = true;
+    int item_no = 0;
+    uint32_t qa[D / 16][4];
+    float o[D / 8][4], m_run[2], l_run[2];
+    int lim[2], len = 0;
+    const float sl2 = a.scale * LOG2E;
+    for (int u = 0; u < count; ++u) {
+      if (fresh) {
+        const int slot = item_no & 1;
+        ok &= wait(q_full + slot, (uint32_t)((item_no >> 1) & 1), &s_abort);
+        __syncwarp();
+        const __nv_bfloat16* qs = sq + slot * rows * D;
+        const int r = min(lane & 15, rows - 1);  // rows past the last repeat it, their results are not used
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) ldmatrix_x4(qa[kk], smem_u32(qs + r * D + kk * 16 + (lane >> 4) * 8));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty + slot);
+        ++item_no;
+        len = max(0, min(a.len[p.b], a.cap));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = (lane >> 2) + 8 * e;
+          lim[e] = row < rows ? max(0, len - a.T + row / G + 1) : 0;
+          m_run[e] = -INFINITY;
+          l_run[e] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      }
+      const int st = u % C::STAGES;
+      ok &= wait(full + st, (uint32_t)((u / C::STAGES) & 1), &s_abort);
+      __syncwarp();
+      uint8_t* kt = smem + st * C::STAGE;
+      const uint32_t k_addr = smem_u32(kt), v_addr = k_addr + C::TILE;
+      const int key0 = p.blk * OB + warp * 16;  // this warp's first key
+      if (key0 + 16 > len) {  // value rows past the last key: zero (they may hold NaN)
+        for (int e = max(0, len - key0) * (D / 8) + lane; e < 16 * (D / 8); e += 32)
+          *reinterpret_cast<uint4*>(kt + C::TILE + tile_off(warp * 16 + e / (D / 8), (e % (D / 8)) * 8)) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // before a later copy into this stage
+        __syncwarp();
+      }
+      float s[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t kb[4];
+        ldmatrix_x4(kb, k_addr + tile_off(warp * 16 + ((lane >> 4) & 1) * 8 + (lane & 7), kk * 16 + ((lane >> 3) & 1) * 8));
+        mma_bf16_16816(s[0], qa[kk], kb);
+        mma_bf16_16816(s[1], qa[kk], kb + 2);
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (key0 + i * 8 + (lane & 3) * 2 + (e & 1) >= lim[e >> 1]) s[i][e] = -INFINITY;
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mx[e] = max3(max3(s[0][2 * e], s[0][2 * e + 1], s[1][2 * e]), s[1][2 * e + 1], s[1][2 * e + 1]);
+        float other = __shfl_xor_sync(0xffffffffu, mx[e], 1);
+        mx[e] = max3(mx[e], other, other);
+        other = __shfl_xor_sync(0xffffffffu, mx[e], 2);
+        mx[e] = max3(mx[e], other, m_run[e]);
+      }
+      // O is rescaled only when some row's maximum has grown
+      if (__any_sync(0xffffffffu, !(mx[0] <= m_run[0]) || !(mx[1] <= m_run[1]))) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float corr = mx[e] == -INFINITY ? 1.f : ex2((m_run[e] - mx[e]) * sl2);
+          m_run[e] = mx[e];
+          l_run[e] *= corr;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][2 * e] *= corr;
+            o[i][2 * e + 1] *= corr;
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float ms = m_run[e] == -INFINITY ? 0.f : m_run[e] * sl2;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float w = ex2(fmaf(s[i][2 * e + c], sl2, -ms));
+            s[i][2 * e + c] = w;
+            l_run[e] += w;
+          }
+      }
+      uint32_t pa[4];
+      pa[0] = pack_bf16(s[0][0], s[0][1]);
+      pa[1] = pack_bf16(s[0][2], s[0][3]);
+      pa[2] = pack_bf16(s[1][0], s[1][1]);
+      pa[3] = pack_bf16(s[1][2], s[1][3]);
+#pragma unroll
+      for (int nb = 0; nb < D / 16; ++nb) {
+        uint32_t vb[4];
+        ldmatrix_x4_trans(vb, v_addr + tile_off(warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), nb * 16 + (lane >> 4) * 8));
+        mma_bf16_16816(o[2 * nb], pa, vb);
+        mma_bf16_16816(o[2 * nb + 1], pa, vb + 2);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + st);
+      const Place at = p;
+      fresh = advance(p);
+      if (!fresh && u + 1 < count) continue;
+      // the item (or this CTA's part of it) is done: join the four warps' sums, half of the columns at a time
+      const int item = at.b * a.Hkv + at.kvh;
+      const int64_t piece = (int64_t)(item + (int)blockIdx.x) * rows;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
+        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
+        const int row = (lane >> 2) + 8 * e;
+        if ((lane & 3) == 0 && row < rows) {
+          red_ml[(warp * rows + row) * 2] = m_run[e];
+          red_ml[(warp * rows + row) * 2 + 1] = l_run[e];
+        }
+      }
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = (lane >> 2) + 8 * e;
+          if (row < rows) {
+            float* dst = red + (warp * rows + row) * C::RED_LD + (lane & 3) * 2;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+              *reinterpret_cast<float2*>(dst + i * 8) =
+                  half == 0 ? make_float2(o[i][2 * e], o[i][2 * e + 1])
+                            : make_float2(o[i + D / 16][2 * e], o[i + D / 16][2 * e + 1]);
+          }
+        }
+        asm volatile("bar.sync 1, %0;\n" ::"n"(OWARPS * 32) : "memory");
+        for (int e = tid; e < rows * (D / 2); e += OWARPS * 32) {
+          const int row = e / (D / 2), col = e % (D / 2);
+          float M = -INFINITY;
+          for (int w = 0; w < OWARPS; ++w) M = max3(M, red_ml[(w * rows + row) * 2], red_ml[(w * rows + row) * 2]);
+          float acc = 0.f, L = 0.f;
+          for (int w = 0; w < OWARPS; ++w) {
+            const float m = red_ml[(w * rows + row) * 2];
+            const float f = m == -INFINITY ? 0.f : ex2((m - M) * sl2);
+            acc += red[(w * rows + row) * C::RED_LD + col] * f;
+            L += red_ml[(w * rows + row) * 2 + 1] * f;
+          }
+          if (ok) {
+            a.piece_o[(piece + row) * D + half * (D / 2) + col] = acc;
+            if (half == 0 && col == 0)
+              *reinterpret_cast<float2*>(a.piece_ml + (piece + row) * 2) = make_float2(M == -INFINITY ? M : M * a.scale, L);
+          }
+        }
+        asm volatile("bar.sync 1, %0;\n" ::"n"(OWARPS * 32) : "memory");
+      }
+      if (tid == 0 && ok) {
+        if (u >= at.blk) a.first[item] = blockIdx.x;  // the run began at or before the item's first block
+        if (at.blk + 1 == at.blocks) a.last[item] = blockIdx.x;
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (s_abort) {  // nothing may land in shared memory after the CTA has gone: wait for the copies in flight
+    if (tid == 0 && a.status != nullptr) atomicExch(a.status, 1);
+    for (int x = max(0, issued - C::STAGES); x < issued; ++x)
+      tc::mbar_wait_cycles(full + x % C::STAGES, (uint32_t)((x / C::STAGES) & 1), WAIT_CYCLES);
+    for (int x = max(0, queries - 2); x < queries; ++x)
+      tc::mbar_wait_cycles(q_full + (x & 1), (uint32_t)((x >> 1) & 1), WAIT_CYCLES);
+    __syncthreads();
+  }
+  pdl_wait();  // the prefix part, launched before, has ended when this grid has
+}
+
+// One warp per (b, t, h): the partials weighted by their own maxima and summed in order.  Lane s holds
+// the weight of part s (32 parts at a time), so the sums' loads wait for nothing but the maxima.
 constexpr int MERGE_WARPS = 4;
 template <int D>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(PrefixMergeArgs a) {
+__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const PrefixMergeArgs a) {
   constexpr int E = D / 32;
   const int64_t at = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  pdl_wait();
   if (at >= (int64_t)a.B * a.T * a.H) return;
-  const float2* sets_ml[2] = {reinterpret_cast<const float2*>(a.part_ml) + at * a.n_slots,
-                              reinterpret_cast<const float2*>(a.more_ml) + at * a.n_more};
-  const float* sets_o[2] = {a.part_o + at * a.n_slots * D + lane * E, a.more_o + at * a.n_more * D + lane * E};
-  const int counts[2] = {a.n_slots, a.more_o != nullptr ? a.n_more : 0};
+  const int64_t bt = at / a.H;
+  const int h = (int)(at - bt * a.H), b = (int)(bt / a.T), t = (int)(bt - (int64_t)b * a.T);
+  // three sets of parts: base of the (max, sum) pairs and of the sums, stride between parts, number
+  const float2* ml[3] = {nullptr, nullptr, nullptr};
+  const float* po[3] = {nullptr, nullptr, nullptr};
+  int64_t step[3] = {1, 1, 1};
+  int count[3] = {0, 0, 0};
+  if (a.part_o != nullptr) {
+    ml[0] = reinterpret_cast<const float2*>(a.part_ml) + at * a.n_slots;
+    po[0] = a.part_o + at * a.n_slots * D;
+    count[0] = a.n_slots;
+  }
+  if (a.more_o != nullptr) {
+    ml[1] = reinterpret_cast<const float2*>(a.more_ml) + at * a.n_more;
+    po[1] = a.more_o + at * a.n_more * D;
+    count[1] = a.n_more;
+  }
+  if (a.piece_o != nullptr) {
+    const int G = a.H / a.Hkv, item = b * a.Hkv + h / G, first = a.first[item];
+    const int64_t rows = a.T * G, row = (int64_t)(item + first) * rows + t * G + h % G;
+    ml[2] = reinterpret_cast<const float2*>(a.piece_ml) + row;
+    po[2] = a.piece_o + row * D;
+    step[2] = rows;
+    count[2] = a.last[item] - first + 1;
+  }
   float M = -INFINITY;
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
-    for (int s = lane; s < counts[g]; s += 32) M = fmaxf(M, sets_ml[g][s].x);
+  for (int g = 0; g < 3; ++g)
+    for (int s = lane; s < count[g]; s += 32) M = fmaxf(M, ml[g][s * step[g]].x);
   M = warp_max(M);
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
-    for (int s0 = 0; s0 < counts[g]; s0 += 32) {
+  for (int g = 0; g < 3; ++g)
+    for (int s0 = 0; s0 < count[g]; s0 += 32) {
       float w = 0.f;
-      if (s0 + lane < counts[g]) {
-        const float2 ml = sets_ml[g][s0 + lane];
-        if (ml.x != -INFINITY) {
-          w = exp2f((ml.x - M) * LOG2E);
-          L += w * ml.y;
+      if (s0 + lane < count[g]) {
+        const float2 p = ml[g][(s0 + lane) * step[g]];
+        if (p.x != -INFINITY) {
+          w = exp2f((p.x - M) * LOG2E);
+          L += w * p.y;
         }
       }
-      const int n = min(32, counts[g] - s0);
-      for (int s = 0; s < n; s += 4) {  // four slots' loads in flight
+      const int n = min(32, count[g] - s0);
+      for (int s = 0; s < n; s += 4) {  // four parts' loads in flight
         float ws[4], v[4][E];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           ws[q] = __shfl_sync(0xffffffffu, w, (s + q) & 31);
           if (s + q >= n) ws[q] = 0.f;
-          const float* o = sets_o[g] + (int64_t)(s0 + s + q) * D;
+          const float* o = po[g] + (s0 + s + q) * step[g] * D + lane * E;
 #pragma unroll
           for (int e = 0; e < E; ++e) v[q][e] = ws[q] != 0.f ? o[e] : 0.f;  // 0: nothing visible (not written), or too small to count
         }
@@ -588,17 +948,19 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(PrefixMergeArgs
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) dst[e] = w[e];
   }
-  if (a.lse != nullptr && lane == 0) {
-    const int64_t bt = at / a.H;
-    const int h = (int)(at - bt * a.H);
-    a.lse[((bt / a.T) * a.H + h) * a.T + bt % a.T] = any ? M + logf(L) : -INFINITY;
+  if (a.lse != nullptr && lane == 0) a.lse[((int64_t)b * a.H + h) * a.T + t] = any ? M + logf(L) : -INFINITY;
+  if (a.joined_o != nullptr) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) a.joined_o[at * D + lane * E + e] = acc[e];
+    if (lane == 0) *reinterpret_cast<float2*>(a.joined_ml + 2 * at) = make_float2(M, L);
   }
 }
 
-bool encode(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t row, int64_t batches, int64_t batch) {
+bool encode(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t row, int64_t batches, int64_t batch,
+            int keys) {
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batches};
   const cuuint64_t strides[2] = {(cuuint64_t)row * 2, (cuuint64_t)batch * 2};
-  const cuuint32_t box[3] = {64, BN, 1}, elem[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)keys, 1}, elem[3] = {1, 1, 1};
   return cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
                                 elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -613,9 +975,9 @@ cudaError_t launch(const PrefixAttnArgs& a, cudaStream_t st) {
   const int64_t width = (int64_t)a.Hkv * D;
   bool ok = true;
   if (a.use_prefix)
-    ok = encode(&pk, a.pk, width, a.P, a.pk_row, 1, a.pk_row * a.P) && encode(&pv, a.pv, width, a.P, a.pv_row, 1, a.pv_row * a.P);
+    ok = encode(&pk, a.pk, width, a.P, a.pk_row, 1, a.pk_row * a.P, BN) && encode(&pv, a.pv, width, a.P, a.pv_row, 1, a.pv_row * a.P, BN);
   if (a.use_own)
-    ok = ok && encode(&k, a.k, width, a.cap, a.k_row, a.B, a.k_batch) && encode(&v, a.v, width, a.cap, a.v_row, a.B, a.v_batch);
+    ok = ok && encode(&k, a.k, width, a.cap, a.k_row, a.B, a.k_batch, BN) && encode(&v, a.v, width, a.cap, a.v_row, a.B, a.v_batch, BN);
   if (!ok) return cudaErrorInvalidValue;
   if (!a.use_prefix) pk = k, pv = v;
   if (!a.use_own) k = pk, v = pv;
@@ -653,14 +1015,52 @@ cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t st) {
   return cudaErrorInvalidValue;
 }
 
+namespace pra {
+namespace prefix {
+
+template <int D>
+cudaError_t launch_own(const OwnAttnArgs& a, cudaStream_t st) {
+  using C = OwnCfg<D>;
+  CUtensorMap k, v;
+  const int64_t width = (int64_t)a.Hkv * D;
+  if (!encode(&k, a.k, width, a.cap, a.k_row, a.B, a.k_batch, OB) || !encode(&v, a.v, width, a.cap, a.v_row, a.B, a.v_batch, OB))
+    return cudaErrorInvalidValue;
+  const int smem = C::smem(a.T * (a.H / a.Hkv));
+  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(own_kernel<D>), smem));
+  return pra_launch_pdl(own_kernel<D>, dim3(a.ctas), dim3(C::THREADS), smem, st, k, v, a);
+}
+
+}  // namespace prefix
+}  // namespace pra
+
+int pra_own_attention_ctas(const OwnAttnArgs& a) {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int rows = a.T * (a.H / a.Hkv);
+  const int smem = a.D == 128 ? pra::prefix::OwnCfg<128>::smem(rows) : pra::prefix::OwnCfg<64>::smem(rows);
+  const int per_sm = smem <= 113 * 1024 ? 2 : 1;
+  // no more CTAs than blocks there can be
+  const int64_t most = (int64_t)a.B * a.Hkv * ((a.cap + pra::prefix::OB - 1) / pra::prefix::OB);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(per_sm * sms, most));
+}
+
+cudaError_t pra_own_attention(const OwnAttnArgs& a, cudaStream_t st) {
+  using namespace pra::prefix;
+  if (a.B == 0 || a.T == 0) return cudaSuccess;
+  if (a.cap < 1 || a.H % a.Hkv || a.T * (a.H / a.Hkv) > PRA_OWN_ROWS || a.ctas < 1) return cudaErrorInvalidValue;
+  if (a.D == 128) return launch_own<128>(a, st);
+  if (a.D == 64) return launch_own<64>(a, st);
+  return cudaErrorInvalidValue;
+}
+
 cudaError_t pra_prefix_merge(const PrefixMergeArgs& a, cudaStream_t st) {
   using namespace pra::prefix;
   const int64_t rows = (int64_t)a.B * a.T * a.H;
   if (rows == 0) return cudaSuccess;
   const int64_t blocks = (rows + MERGE_WARPS - 1) / MERGE_WARPS;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  if (a.D == 128) merge_kernel<128><<<(unsigned)blocks, MERGE_WARPS * 32, 0, st>>>(a);
-  else if (a.D == 64) merge_kernel<64><<<(unsigned)blocks, MERGE_WARPS * 32, 0, st>>>(a);
-  else return cudaErrorInvalidValue;
-  return cudaGetLastError();
+  if (a.D == 128) return pra_launch_pdl(merge_kernel<128>, dim3((unsigned)blocks), dim3(MERGE_WARPS * 32), 0, st, a);
+  if (a.D == 64) return pra_launch_pdl(merge_kernel<64>, dim3((unsigned)blocks), dim3(MERGE_WARPS * 32), 0, st, a);
+  return cudaErrorInvalidValue;
 }

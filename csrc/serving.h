@@ -96,15 +96,48 @@ cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t stream);
 // CTAs of a launch before splitting, and how many run at once (for choosing splits).
 void pra_prefix_attention_shape(const PrefixAttnArgs& a, int* tiles, int* slots);
 
-// out / lse from the partials of every (b, t, h).
+// The own keys of rows with few queries (T * H / Hkv <= PRA_OWN_ROWS per KV head), which a 128-row tile would
+// leave mostly empty: every (batch row, KV head) is an item of ceil(len / 64) blocks (at least one), the
+// CTAs take equal runs of the blocks of all items, and an item that several CTAs share has a piece in
+// each.  CTA c's piece of item i is piece i + c: pieces of an item follow one another.
+constexpr int PRA_OWN_ROWS = 16;
+struct OwnAttnArgs {
+  const __nv_bfloat16* q;         // as in PrefixAttnArgs
+  int64_t q_batch, q_token;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  int64_t k_batch, k_row, v_batch, v_row;
+  int cap;
+  const int* len;
+  int B, T, H, Hkv, D;
+  float scale;
+  int ctas;                       // grid
+  int after_prefix;               // the launch before it on the stream is pra_prefix_attention's
+  float* piece_o;                 // [B * Hkv + ctas, T * G, D] unnormalised
+  float* piece_ml;                // [B * Hkv + ctas, T * G, 2]
+  int* first;                     // [B * Hkv] first and last CTA of each item
+  int* last;
+  int* status;
+};
+int pra_own_attention_ctas(const OwnAttnArgs& a);
+cudaError_t pra_own_attention(const OwnAttnArgs& a, cudaStream_t stream);
+
+// out / lse, or the joined partial, from the partials of every (b, t, h).
 struct PrefixMergeArgs {
-  const float* part_o;
+  int B, T, H, Hkv, D;
+  const float* part_o;            // [B * T, H, n_slots, D] and (max, sum) pairs, or null
   const float* part_ml;
-  int B, T, H, D, n_slots;
-  const float* more_o;            // a second set of partials [B * T, H, n_more, D] of the same queries, or null
+  int n_slots;
+  const float* more_o;            // a second such set [B * T, H, n_more, D], or null
   const float* more_ml;
   int n_more;
+  const float* piece_o;           // pieces of pra_own_attention, or null
+  const float* piece_ml;
+  const int* first;
+  const int* last;
   __nv_bfloat16* out;             // [B, T, H * D] or null
   float* lse;                     // [B, H, T] or null
+  float* joined_o;                // [B * T, H, D] unnormalised or null
+  float* joined_ml;               // [B * T, H, 2]
 };
 cudaError_t pra_prefix_merge(const PrefixMergeArgs& a, cudaStream_t stream);

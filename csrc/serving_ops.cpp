@@ -285,8 +285,8 @@ void rows_ok(const Tensor& t, int64_t width, const char* name) {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// {out [like q], lse [B, H, T] or none}, or with `partials` the unmerged {o [B * T, H, n, D], (max, sum)
-// [B * T, H, n, 2]}.
+// {out [like q], lse [B, H, T] or none}, or with `partials` {unnormalised o [B * T, H, 1, D], (max, sum)
+// [B * T, H, 1, 2]}.
 std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k, Tensor v, Tensor lengths,
                                                int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                OptTensor prefix_lengths, double scale, bool return_lse,
@@ -376,83 +376,101 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     pra_prefix_attention_shape(p, &tiles, &slots);
     return std::max(1, std::min(blocks, slots / tiles));
   };
-  // A row with 256 or more query rows of a KV head (or the only one) fills its tiles: prefix and own keys in
-  // one walk.  Else the prefix is walked once for the query rows of the whole batch, and the own keys
-  // on their own.
-  const bool per_row_walk = B == 1 || T * G >= 256 || a.P == 0 || a.cap == 0;
-  if (per_row_walk) {
+  PrefixMergeArgs m{};
+  m.B = a.B;
+  m.T = a.T;
+  m.H = a.H;
+  m.Hkv = a.Hkv;
+  m.D = a.D;
+  Tensor joined_o, joined_ml;
+  const auto merge = [&]() -> std::vector<OptTensor> {
+    m.part_o = a.part_o;
+    m.part_ml = a.part_ml;
+    m.n_slots = a.part_o != nullptr ? a.n_slots : 0;
+    if (partials) {
+      joined_o = torch::empty({B * T, heads, 1, head_dim}, fo);
+      joined_ml = torch::empty({B * T, heads, 1, 2}, fo);
+      m.joined_o = joined_o.data_ptr<float>();
+      m.joined_ml = joined_ml.data_ptr<float>();
+    } else {
+      m.out = a.out;
+      m.lse = lse;
+    }
+    check(pra_prefix_merge(m, stream()), "shared_prefix_attention");
+    if (partials) return {joined_o, joined_ml};
+    return result;
+  };
+  const int64_t rows = T * G;  // query rows of a (batch row, KV head)
+  const bool few = rows <= PRA_OWN_ROWS && a.cap > 0;
+  // A batch row with 256 or more query rows of a KV head (or the only batch row) fills its tiles: prefix and own
+  // keys in one walk.  Else the prefix is walked once for the query rows of the whole batch, and the own
+  // keys on their own.
+  if (a.cap == 0 || rows >= 256 || (B == 1 && a.P > 0) || (a.P == 0 && !few)) {
     a.packed = a.cap == 0;
     a.use_prefix = a.P > 0;
     a.use_own = a.cap > 0;
     a.splits = splits_for(a, prefix_blocks + own_blocks);
     if (a.splits > 1 || partials) workspace(a.splits);
     check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
-    if (a.splits == 1 && !partials) return result;
-  } else {
-    PrefixAttnArgs own = a;
+    if (a.splits > 1) return merge();
+    if (partials) return {part_o, part_ml};
+    return result;
+  }
+  PrefixAttnArgs own = a;
+  if (a.P > 0) {
     a.packed = a.use_prefix = 1;
     a.splits = splits_for(a, prefix_blocks);
-    own.use_own = 1;
-    // single tokens: the split-K decode kernel (16 query rows a tile instead of 128)
-    const bool decode = T == 1 && G <= 16 && a.k_row == a.v_row && a.k_batch == a.v_batch && k.size(1) > 1;
-    int split_keys = 256;
-    if (decode) {
-      for (int s : {1024, 512})
-        if (B * kv_heads * ceil_div(a.cap, s) >= 3 * 148) {
-          split_keys = s;
-          break;
-        }
-      own.splits = ceil_div(a.cap, split_keys);
-    } else {
-      own.splits = splits_for(own, own_blocks);
-    }
-    workspace(a.splits + own.splits);
-    own.part_o = a.part_o;
-    own.part_ml = a.part_ml;
-    own.n_slots = a.n_slots;
-    own.slot0 = a.splits;
-    check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
-    if (decode) {
-      DecodeAttnParams p{};
-      p.q = a.q;
-      p.q_row = a.q_batch;
-      p.B = a.B;
-      p.H = a.H;
-      p.Hkv = a.Hkv;
-      p.loc_k = a.k;
-      p.loc_v = a.v;
-      p.loc_row = a.k_row;
-      p.loc_batch = a.k_batch;
-      p.loc_len = a.len;
-      p.loc_cap = a.cap;
-      p.scale = a.scale;
-      p.split_keys = split_keys;
-      p.n_split = a.n_slots;
-      p.mem_splits = a.splits;
-      p.split_lo = a.splits;
-      p.split_count = own.splits;
-      p.phase = 1;
-      p.part_o = a.part_o;
-      p.part_ml = a.part_ml;
-      p.status = a.status;
-      check(pra_decode_attention(p, a.D, stream()), "shared_prefix_attention");
-    } else {
-      check(pra_prefix_attention(own, stream()), "shared_prefix_attention");
-    }
   }
-  if (partials) return {part_o, part_ml};
-  PrefixMergeArgs m{};
-  m.part_o = a.part_o;
-  m.part_ml = a.part_ml;
-  m.B = a.B;
-  m.T = a.T;
-  m.H = a.H;
-  m.D = a.D;
-  m.n_slots = a.n_slots;
-  m.out = a.out;
-  m.lse = lse;
-  check(pra_prefix_merge(m, stream()), "shared_prefix_attention");
-  return result;
+  if (few) {
+    if (a.P > 0) {
+      workspace(a.splits);
+      check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
+    }
+    OwnAttnArgs o{};
+    o.q = a.q;
+    o.q_batch = a.q_batch;
+    o.q_token = a.q_token;
+    o.k = a.k;
+    o.v = a.v;
+    o.k_batch = a.k_batch;
+    o.k_row = a.k_row;
+    o.v_batch = a.v_batch;
+    o.v_row = a.v_row;
+    o.cap = a.cap;
+    o.len = a.len;
+    o.B = a.B;
+    o.T = a.T;
+    o.H = a.H;
+    o.Hkv = a.Hkv;
+    o.D = a.D;
+    o.scale = a.scale;
+    o.status = a.status;
+    o.after_prefix = a.P > 0;
+    o.ctas = pra_own_attention_ctas(o);
+    const int64_t items = B * kv_heads, pieces = (items + o.ctas) * rows;
+    // one workspace: the pieces' sums, their (max, sum) pairs, the items' first and last CTAs
+    auto work = torch::empty({pieces * (head_dim + 2) + 2 * items}, fo);
+    o.piece_o = work.data_ptr<float>();
+    o.piece_ml = o.piece_o + pieces * head_dim;
+    o.first = reinterpret_cast<int*>(o.piece_ml + pieces * 2);
+    o.last = o.first + items;
+    m.piece_o = o.piece_o;
+    m.piece_ml = o.piece_ml;
+    m.first = o.first;
+    m.last = o.last;
+    check(pra_own_attention(o, stream()), "shared_prefix_attention");
+    return merge();
+  }
+  own.use_own = 1;
+  own.splits = splits_for(own, own_blocks);
+  workspace(a.splits + own.splits);
+  own.part_o = a.part_o;
+  own.part_ml = a.part_ml;
+  own.n_slots = a.n_slots;
+  own.slot0 = a.splits;
+  check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
+  check(pra_prefix_attention(own, stream()), "shared_prefix_attention");
+  return merge();
 }
 
 // {out [B, T, H * D] bf16, lse [B, H, T] or none} of one or two sets of partials [B * T, H, n, D].
@@ -485,7 +503,7 @@ std::vector<OptTensor> merge_attention_partials(Tensor part_o, Tensor part_ml, O
   }
   m.B = (int)batch;
   m.T = batch > 0 ? (int)(rows / batch) : 0;
-  m.H = (int)H;
+  m.H = m.Hkv = (int)H;
   m.D = (int)D;
   auto out = torch::empty({batch, m.T, H * D}, part_o.options().dtype(at::kBFloat16));
   m.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());

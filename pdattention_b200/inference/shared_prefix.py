@@ -37,9 +37,9 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
 def shared_prefix_partials(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
                            v: torch.Tensor, lengths: torch.Tensor, heads: int, kv_heads: int, head_dim: int, *,
                            prefix_lengths: torch.Tensor | None = None, scale: float | None = None):
-    """``shared_prefix_attention`` before its parts are joined: fp32 ``(sums [B T, H, n, D], (max, sum)
-    [B T, H, n, 2])``, each part's sum relative to its own maximum.  For queries that attend over
-    further keys elsewhere; ``merge_attention_partials`` joins both."""
+    """``shared_prefix_attention`` before the division: fp32 ``(sums [B T, H, 1, D], (max, sum)
+    [B T, H, 1, 2])``, the sums relative to the maximum.  For queries that attend over further keys
+    elsewhere; ``merge_attention_partials`` joins both."""
     return tuple(require().shared_prefix_attention(q, prefix_k, prefix_v, k, v, lengths, heads, kv_heads, head_dim,
                                                    prefix_lengths,
                                                    1.0 / math.sqrt(head_dim) if scale is None else scale, False, True))
