@@ -533,11 +533,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
 // Up to 16 query rows (t, g) of a (batch row, KV head) against its own keys: bound by reading K and V once.
 // A persistent grid of two CTAs per SM; each walks its run of 64-key blocks across items without
 // draining its pipeline: one thread streams K and V tiles (TMA, 128-byte swizzle) and the items' queries
-// (bulk copies) some stages ahead, four warps take 16 keys of every block each (mma.sync m16n8k16, the
-// queries' fragments in registers for the whole item) with their own running maximum and sum, and
-// join at the end of an item.  Equal runs of blocks keep every SM busy to the end whatever the
-// lengths: at 64 rows of 64 to 1,024 keys a CTA per (row, KV head) took 39 us, at 128 rows of 128 to 2,048
-// 65 us.
+// (bulk copies) some stages ahead, four warps take 16 keys of every block each, with their own running
+// maximum and sum, and join at the end of an item.  The products are transposed, S^T = K Q^T and
+// O^T = V^T P^T (mma.sync m16n8k16, keys or features as M, 8 NB query rows as N): with the queries as M
+// the 16 rows of a tile were mostly padding and twice the MMAs bound an SM to 44 GB/s of keys, an SM's
+// share of HBM.  P^T goes from accumulator to operand layout with movmatrix.  Equal runs of blocks
+// keep every SM busy to the end whatever the lengths.
 constexpr int OB = 64;       // keys of a block
 constexpr int OWARPS = 4;
 template <int D>
@@ -545,7 +546,7 @@ struct OwnCfg {
   static constexpr int BOXES = D / 64, BOX = OB * 128, TILE = BOXES * BOX, STAGE = 2 * TILE;
   static constexpr int STAGES = D == 128 ? 3 : 6;
   static constexpr int THREADS = OWARPS * 32 + 32;
-  static constexpr int RED_LD = D / 2 + 2;  // half of the columns at a time
+  static constexpr int RED_LD = D / 2 + 4;  // half of the columns at a time
   static constexpr int smem(int rows) {
     return 1024 + STAGES * STAGE + 2 * rows * D * 2 + OWARPS * rows * RED_LD * 4 + OWARPS * rows * 8 + 256;
   }
@@ -560,7 +561,14 @@ __device__ __forceinline__ int own_blocks(const OwnAttnArgs& a, int b) {
   return max(1, (max(0, min(a.len[b], a.cap)) + OB - 1) / OB);
 }
 
-template <int D>
+// The 8 x 8 matrix of 16-bit elements in the mma fragment layout, transposed.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <int D, int NB>  // NB: query rows / 8
 __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
     own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const OwnAttnArgs a) {
   using C = OwnCfg<D>;
@@ -693,9 +701,9 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
     Place p = start();
     bool fresh = true;
     int item_no = 0;
-    uint32_t qa[D / 16][4];
-    float o[D / 8][4], m_run[2], l_run[2];
-    int lim[2], len = 0;
+    uint32_t qb[NB][D / 16][2];                     // Q^T, the B operand of S^T
+    float o[NB][D / 16][4], m_run[NB][2], l_run[NB][2];  // O^T; this thread's two query rows of each 8
+    int lim[NB][2], len = 0;
     const float sl2 = a.scale * LOG2E;
     for (int u = 0; u < count; ++u) {
       if (fresh) {
@@ -703,22 +711,35 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
         ok &= wait(q_full + slot, (uint32_t)((item_no >> 1) & 1), &s_abort);
         __syncwarp();
         const __nv_bfloat16* qs = sq + slot * rows * D;
-        const int r = min(lane & 15, rows - 1);  // rows past the last repeat it, their results are not used
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) ldmatrix_x4(qa[kk], smem_u32(qs + r * D + kk * 16 + (lane >> 4) * 8));
+        for (int nb = 0; nb < NB; ++nb) {
+          const int r = min(nb * 8 + (lane & 7), rows - 1);  // rows past the last repeat it, their results are not used
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk += 2) {
+            uint32_t f[4];
+            ldmatrix_x4(f, smem_u32(qs + r * D + kk * 16 + (lane >> 3) * 8));
+            qb[nb][kk][0] = f[0];
+            qb[nb][kk][1] = f[1];
+            qb[nb][kk + 1][0] = f[2];
+            qb[nb][kk + 1][1] = f[3];
+          }
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty + slot);
         ++item_no;
         len = max(0, min(a.len[p.b], a.cap));
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = (lane >> 2) + 8 * e;
-          lim[e] = row < rows ? max(0, len - a.T + row / G + 1) : 0;
-          m_run[e] = -INFINITY;
-          l_run[e] = 0.f;
-        }
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+          for (int e = 0; e < 2; ++e) {
+            const int row = nb * 8 + (lane & 3) * 2 + e;
+            lim[nb][e] = row < rows ? max(0, len - a.T + row / G + 1) : 0;
+            m_run[nb][e] = -INFINITY;
+            l_run[nb][e] = 0.f;
+          }
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) o[nb][d][0] = o[nb][d][1] = o[nb][d][2] = o[nb][d][3] = 0.f;
+        }
       }
       const int st = u % C::STAGES;
       ok &= wait(full + st, (uint32_t)((u / C::STAGES) & 1), &s_abort);
@@ -732,68 +753,67 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
         fence_proxy_async_smem();  // before a later copy into this stage
         __syncwarp();
       }
-      float s[2][4];
+      // S^T of this warp's 16 keys, two accumulators so that the MMAs do not wait for one another
+      float s[NB][2][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) s[nb][x][0] = s[nb][x][1] = s[nb][x][2] = s[nb][x][3] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t kb[4];
-        ldmatrix_x4(kb, k_addr + tile_off(warp * 16 + ((lane >> 4) & 1) * 8 + (lane & 7), kk * 16 + ((lane >> 3) & 1) * 8));
-        mma_bf16_16816(s[0], qa[kk], kb);
-        mma_bf16_16816(s[1], qa[kk], kb + 2);
-      }
-      float mx[2] = {-INFINITY, -INFINITY};
+        uint32_t ka[4];
+        ldmatrix_x4(ka, k_addr + tile_off(warp * 16 + (lane & 15), kk * 16 + (lane >> 4) * 8));
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int nb = 0; nb < NB; ++nb) mma_bf16_16816(s[nb][kk & 1], ka, qb[nb][kk]);
+      }
+      uint32_t pb[NB][2];  // P^T, the B operand of O^T
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float z[4];  // keys (lane >> 2) + 8 (e >> 1), query rows 8 nb + 2 (lane & 3) + (e & 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (key0 + i * 8 + (lane & 3) * 2 + (e & 1) >= lim[e >> 1]) s[i][e] = -INFINITY;
+          z[e] = s[nb][0][e] + s[nb][1][e];
+          if (key0 + (lane >> 2) + 8 * (e >> 1) >= lim[nb][e & 1]) z[e] = -INFINITY;
         }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        mx[e] = max3(max3(s[0][2 * e], s[0][2 * e + 1], s[1][2 * e]), s[1][2 * e + 1], s[1][2 * e + 1]);
-        float other = __shfl_xor_sync(0xffffffffu, mx[e], 1);
-        mx[e] = max3(mx[e], other, other);
-        other = __shfl_xor_sync(0xffffffffu, mx[e], 2);
-        mx[e] = max3(mx[e], other, m_run[e]);
-      }
-      // O is rescaled only when some row's maximum has grown
-      if (__any_sync(0xffffffffu, !(mx[0] <= m_run[0]) || !(mx[1] <= m_run[1]))) {
+        float mx[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float corr = mx[e] == -INFINITY ? 1.f : ex2((m_run[e] - mx[e]) * sl2);
-          m_run[e] = mx[e];
-          l_run[e] *= corr;
+          mx[e] = max3(z[e], z[e + 2], m_run[nb][e]);
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][2 * e] *= corr;
-            o[i][2 * e + 1] *= corr;
+          for (int x = 4; x < 32; x <<= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, mx[e], x);
+            mx[e] = max3(mx[e], other, other);
           }
         }
-      }
+        // O is rescaled only when some row's maximum has grown
+        if (__any_sync(0xffffffffu, !(mx[0] <= m_run[nb][0]) || !(mx[1] <= m_run[nb][1]))) {
+          float corr[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float ms = m_run[e] == -INFINITY ? 0.f : m_run[e] * sl2;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float w = ex2(fmaf(s[i][2 * e + c], sl2, -ms));
-            s[i][2 * e + c] = w;
-            l_run[e] += w;
+          for (int e = 0; e < 2; ++e) {
+            corr[e] = mx[e] == -INFINITY ? 1.f : ex2((m_run[nb][e] - mx[e]) * sl2);
+            m_run[nb][e] = mx[e];
+            l_run[nb][e] *= corr[e];
           }
-      }
-      uint32_t pa[4];
-      pa[0] = pack_bf16(s[0][0], s[0][1]);
-      pa[1] = pack_bf16(s[0][2], s[0][3]);
-      pa[2] = pack_bf16(s[1][0], s[1][1]);
-      pa[3] = pack_bf16(s[1][2], s[1][3]);
 #pragma unroll
-      for (int nb = 0; nb < D / 16; ++nb) {
-        uint32_t vb[4];
-        ldmatrix_x4_trans(vb, v_addr + tile_off(warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), nb * 16 + (lane >> 4) * 8));
-        mma_bf16_16816(o[2 * nb], pa, vb);
-        mma_bf16_16816(o[2 * nb + 1], pa, vb + 2);
+          for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nb][d][e] *= corr[e & 1];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float m = m_run[nb][e & 1];
+          z[e] = ex2(fmaf(z[e], sl2, m == -INFINITY ? 0.f : -m * sl2));
+          l_run[nb][e & 1] += z[e];
+        }
+        pb[nb][0] = movmatrix_trans(pack_bf16(z[0], z[1]));
+        pb[nb][1] = movmatrix_trans(pack_bf16(z[2], z[3]));
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t va[4];
+        ldmatrix_x4_trans(va, v_addr + tile_off(warp * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, d * 16 + ((lane >> 3) & 1) * 8));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma_bf16_16816(o[nb][d], va, pb[nb]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + st);
@@ -804,29 +824,32 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
       const int item = at.b * a.Hkv + at.kvh;
       const int64_t piece = (int64_t)(item + (int)blockIdx.x) * rows;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
-        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
-        const int row = (lane >> 2) + 8 * e;
-        if ((lane & 3) == 0 && row < rows) {
-          red_ml[(warp * rows + row) * 2] = m_run[e];
-          red_ml[(warp * rows + row) * 2 + 1] = l_run[e];
-        }
-      }
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = (lane >> 2) + 8 * e;
-          if (row < rows) {
-            float* dst = red + (warp * rows + row) * C::RED_LD + (lane & 3) * 2;
+          float l = l_run[nb][e];
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-              *reinterpret_cast<float2*>(dst + i * 8) =
-                  half == 0 ? make_float2(o[i][2 * e], o[i][2 * e + 1])
-                            : make_float2(o[i + D / 16][2 * e], o[i + D / 16][2 * e + 1]);
-          }
+          for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+          const int row = nb * 8 + (lane & 3) * 2 + e;
+          if ((lane >> 2) == 0 && row < rows)
+            *reinterpret_cast<float2*>(red_ml + (warp * rows + row) * 2) = make_float2(m_run[nb][e], l);
         }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = nb * 8 + (lane & 3) * 2 + e;
+            if (row < rows) {
+              float* dst = red + (warp * rows + row) * C::RED_LD + (lane >> 2);
+#pragma unroll
+              for (int d = 0; d < D / 32; ++d) {
+                dst[d * 16] = o[nb][d + half * (D / 32)][e];
+                dst[d * 16 + 8] = o[nb][d + half * (D / 32)][e + 2];
+              }
+            }
+          }
         asm volatile("bar.sync 1, %0;\n" ::"n"(OWARPS * 32) : "memory");
         for (int e = tid; e < rows * (D / 2); e += OWARPS * 32) {
           const int row = e / (D / 2), col = e % (D / 2);
@@ -866,77 +889,91 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
   pdl_wait();  // the prefix part, launched before, has ended when this grid has
 }
 
-// One warp per (b, t, h): the partials weighted by their own maxima and summed in order.  Lane s holds
-// the weight of part s (32 parts at a time), so the sums' loads wait for nothing but the maxima.
+// One warp per (b, t, h): the parts weighted by their own maxima and summed in order.  Bound by
+// latency: lane s finds part s (32 at a time) and holds its weight, and the first eight parts' sums are
+// on their way while the maxima are still being compared (a part that holds nothing was not written:
+// what is read there is dropped).
 constexpr int MERGE_WARPS = 4;
 template <int D>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const PrefixMergeArgs a) {
   constexpr int E = D / 32;
+  struct alignas(4 * E) Piece {
+    float v[E];
+  };
   const int64_t at = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  pdl_wait();
-  if (at >= (int64_t)a.B * a.T * a.H) return;
   const int64_t bt = at / a.H;
   const int h = (int)(at - bt * a.H), b = (int)(bt / a.T), t = (int)(bt - (int64_t)b * a.T);
-  // three sets of parts: base of the (max, sum) pairs and of the sums, stride between parts, number
-  const float2* ml[3] = {nullptr, nullptr, nullptr};
-  const float* po[3] = {nullptr, nullptr, nullptr};
-  int64_t step[3] = {1, 1, 1};
-  int count[3] = {0, 0, 0};
-  if (a.part_o != nullptr) {
-    ml[0] = reinterpret_cast<const float2*>(a.part_ml) + at * a.n_slots;
-    po[0] = a.part_o + at * a.n_slots * D;
-    count[0] = a.n_slots;
-  }
-  if (a.more_o != nullptr) {
-    ml[1] = reinterpret_cast<const float2*>(a.more_ml) + at * a.n_more;
-    po[1] = a.more_o + at * a.n_more * D;
-    count[1] = a.n_more;
-  }
+  pdl_wait();
+  if (at >= (int64_t)a.B * a.T * a.H) return;
+  // parts [0, n0) are the first set's, [n0, n1) the second's, [n1, n) the pieces
+  const int n0 = a.part_o != nullptr ? a.n_slots : 0, n1 = n0 + (a.more_o != nullptr ? a.n_more : 0);
+  int n = n1;
+  int64_t row0 = 0;
+  const int rows = a.T * (a.H / a.Hkv);
   if (a.piece_o != nullptr) {
     const int G = a.H / a.Hkv, item = b * a.Hkv + h / G, first = a.first[item];
-    const int64_t rows = a.T * G, row = (int64_t)(item + first) * rows + t * G + h % G;
-    ml[2] = reinterpret_cast<const float2*>(a.piece_ml) + row;
-    po[2] = a.piece_o + row * D;
-    step[2] = rows;
-    count[2] = a.last[item] - first + 1;
+    n += a.last[item] - first + 1;
+    row0 = (int64_t)(item + first) * rows + t * G + h % G;
   }
-  float M = -INFINITY;
+  // (max, sum) and sums of part s
+  auto find = [&](int s, const float2*& ml, const float*& o) {
+    const int64_t i = s < n0 ? at * a.n_slots + s : s < n1 ? at * a.n_more + (s - n0) : row0 + (int64_t)(s - n1) * rows;
+    ml = reinterpret_cast<const float2*>(s < n0 ? a.part_ml : s < n1 ? a.more_ml : a.piece_ml) + i;
+    o = (s < n0 ? a.part_o : s < n1 ? a.more_o : a.piece_o) + i * D;
+  };
+  const float2 nothing = make_float2(-INFINITY, 0.f);
+  const float2* ml = nullptr;
+  const float* o = nullptr;
+  float2 mine = nothing;
+  if (lane < n) {
+    find(lane, ml, o);
+    mine = *ml;
+  }
+  Piece v[8];
+  auto fetch = [&](int s0) {  // parts s0 .. s0 + 7 of the 32 that the lanes hold
 #pragma unroll
-  for (int g = 0; g < 3; ++g)
-    for (int s = lane; s < count[g]; s += 32) M = fmaxf(M, ml[g][s * step[g]].x);
+    for (int q = 0; q < 8; ++q) {
+      const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), s0 + q));
+      if (src != nullptr) v[q] = *reinterpret_cast<const Piece*>(src + lane * E);
+    }
+  };
+  fetch(0);
+  float M = mine.x;
+  for (int s = lane + 32; s < n; s += 32) {
+    const float2* m2;
+    const float* o2;
+    find(s, m2, o2);
+    M = fmaxf(M, m2->x);
+  }
   M = warp_max(M);
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll
-  for (int g = 0; g < 3; ++g)
-    for (int s0 = 0; s0 < count[g]; s0 += 32) {
-      float w = 0.f;
-      if (s0 + lane < count[g]) {
-        const float2 p = ml[g][(s0 + lane) * step[g]];
-        if (p.x != -INFINITY) {
-          w = exp2f((p.x - M) * LOG2E);
-          L += w * p.y;
-        }
-      }
-      const int n = min(32, count[g] - s0);
-      for (int s = 0; s < n; s += 4) {  // four parts' loads in flight
-        float ws[4], v[4][E];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          ws[q] = __shfl_sync(0xffffffffu, w, (s + q) & 31);
-          if (s + q >= n) ws[q] = 0.f;
-          const float* o = po[g] + (s0 + s + q) * step[g] * D + lane * E;
-#pragma unroll
-          for (int e = 0; e < E; ++e) v[q][e] = ws[q] != 0.f ? o[e] : 0.f;  // 0: nothing visible (not written), or too small to count
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += ws[q] * v[q][e];
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    if (s0 > 0) {
+      mine = nothing;
+      o = nullptr;
+      if (s0 + lane < n) {
+        find(s0 + lane, ml, o);
+        mine = *ml;
       }
     }
+    const float w = mine.x == -INFINITY ? 0.f : exp2f((mine.x - M) * LOG2E);
+    if (w != 0.f) L += w * mine.y;
+    const int m = min(32, n - s0);
+    for (int s = 0; s < m; s += 8) {
+      if (s0 + s > 0) fetch(s);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float ws = __shfl_sync(0xffffffffu, w, (s + q) & 31);
+        if (s + q < m && ws != 0.f) {  // 0: nothing visible, or too small to count
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += ws * v[q].v[e];
+        }
+      }
+    }
+  }
   L = warp_sum(L);
   const bool any = M != -INFINITY;
   const float inv = any ? 1.f / L : 0.f;
@@ -1018,7 +1055,7 @@ cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t st) {
 namespace pra {
 namespace prefix {
 
-template <int D>
+template <int D, int NB>
 cudaError_t launch_own(const OwnAttnArgs& a, cudaStream_t st) {
   using C = OwnCfg<D>;
   CUtensorMap k, v;
@@ -1026,8 +1063,8 @@ cudaError_t launch_own(const OwnAttnArgs& a, cudaStream_t st) {
   if (!encode(&k, a.k, width, a.cap, a.k_row, a.B, a.k_batch, OB) || !encode(&v, a.v, width, a.cap, a.v_row, a.B, a.v_batch, OB))
     return cudaErrorInvalidValue;
   const int smem = C::smem(a.T * (a.H / a.Hkv));
-  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(own_kernel<D>), smem));
-  return pra_launch_pdl(own_kernel<D>, dim3(a.ctas), dim3(C::THREADS), smem, st, k, v, a);
+  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(own_kernel<D, NB>), smem));
+  return pra_launch_pdl(own_kernel<D, NB>, dim3(a.ctas), dim3(C::THREADS), smem, st, k, v, a);
 }
 
 }  // namespace prefix
@@ -1049,8 +1086,9 @@ cudaError_t pra_own_attention(const OwnAttnArgs& a, cudaStream_t st) {
   using namespace pra::prefix;
   if (a.B == 0 || a.T == 0) return cudaSuccess;
   if (a.cap < 1 || a.H % a.Hkv || a.T * (a.H / a.Hkv) > PRA_OWN_ROWS || a.ctas < 1) return cudaErrorInvalidValue;
-  if (a.D == 128) return launch_own<128>(a, st);
-  if (a.D == 64) return launch_own<64>(a, st);
+  const bool few = a.T * (a.H / a.Hkv) <= 8;
+  if (a.D == 128) return few ? launch_own<128, 1>(a, st) : launch_own<128, 2>(a, st);
+  if (a.D == 64) return few ? launch_own<64, 1>(a, st) : launch_own<64, 2>(a, st);
   return cudaErrorInvalidValue;
 }
 
