@@ -724,8 +724,6 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
             qb[nb][kk + 1][1] = f[3];
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_empty + slot);
         ++item_no;
         len = max(0, min(a.len[p.b], a.cap));
 #pragma unroll
@@ -765,6 +763,12 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
         ldmatrix_x4(ka, k_addr + tile_off(warp * 16 + (lane & 15), kk * 16 + (lane >> 4) * 8));
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) mma_bf16_16816(s[nb][kk & 1], ka, qb[nb][kk]);
+      }
+      if (fresh) {
+        // the MMAs have taken the queries' fragments, so their loads are done and the tile may be filled
+        // again (an arrival right behind the loads is not ordered after their reads)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty + ((item_no - 1) & 1));
       }
       uint32_t pb[NB][2];  // P^T, the B operand of O^T
 #pragma unroll

@@ -268,6 +268,25 @@ def test_shared_prefix_attention_views_lengths_and_scale(T):
     assert torch.equal(shared_prefix_attention(q, pk, pv, k, v, lengths, H, Hkv, D, scale=0.9), out)
 
 
+@pytest.mark.parametrize("B,T,P,lo,hi,H,Hkv,D", [(78, 1, 2170, 1, 66, 28, 4, 128), (64, 1, 8192, 64, 700, 32, 8, 128),
+                                                 (150, 1, 900, 1, 64, 16, 8, 128), (48, 3, 1500, 3, 90, 8, 2, 64)])
+def test_shared_prefix_attention_repeats_exactly(B, T, P, lo, hi, H, Hkv, D):
+    """Both parts at once, many short rows to a CTA: every call gives the same bits, and the right ones."""
+    from pdattention_b200.inference.shared_prefix import shared_prefix_attention
+
+    torch.manual_seed(P)
+    w = Hkv * D
+    q = (1.5 * torch.randn(B, T, H * D, device=DEV)).bfloat16()
+    pk, pv = torch.randn(2, P, w, device=DEV).bfloat16()
+    k, v = torch.randn(2, B, hi + 3, w, device=DEV).bfloat16()
+    lengths = torch.tensor([lo + (hi - lo) * i // (B - 1) for i in range(B)], dtype=torch.int32, device=DEV)[torch.randperm(B, device=DEV)]
+    run = lambda: shared_prefix_attention(q, pk, pv, k, v, lengths, H, Hkv, D, return_lse=True)  # noqa: E731
+    first = run()
+    prefix_close(*first, prefix64(q, pk, pv, k, v, lengths, None, H, Hkv, D, 1 / math.sqrt(D)), D)
+    again = [run() for _ in range(20)]
+    assert all(torch.equal(a, b) for r in again for a, b in zip(r, first))
+
+
 def test_shared_prefix_attention_streams_and_graphs():
     from pdattention_b200.inference.shared_prefix import shared_prefix_attention
 
