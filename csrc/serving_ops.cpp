@@ -108,8 +108,8 @@ Tensor rotary_segment(RotarySegment& s, Tensor& x, int64_t head_dim) {
   return out;
 }
 
-std::vector<OptTensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor cos_t, Tensor sin_t, bool interleaved,
-                              bool inverse) {
+std::vector<OptTensor> rotate(Tensor q, OptTensor k, const Tensor& positions, const Tensor& cos_t, const Tensor& sin_t,
+                              bool interleaved, bool inverse) {
   TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(q.device());
   const int dtype = dtype_code(q, "q");
@@ -133,6 +133,47 @@ std::vector<OptTensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor co
   }
   if (a.seg[0].heads + a.seg[1].heads > 0) check(pra_rotary(a, dtype, stream()), "rotary");
   return result;
+}
+
+std::vector<OptTensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& cos_t,
+                              const Tensor& sin_t, bool interleaved, bool inverse);
+
+// The rotation is linear in (q, k): its backward is the transposed rotation, differentiable again.
+struct Rotary : torch::autograd::Function<Rotary> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k,
+                                                const Tensor& positions, const Tensor& cos_t, const Tensor& sin_t,
+                                                bool interleaved, bool inverse) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions, cos_t, sin_t});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    auto y = rotate(q, k, positions, cos_t, sin_t, interleaved, inverse);
+    if (!k.has_value()) return {*y[0]};
+    return {*y[0], *y[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
+    const auto saved = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = ctx->saved_data["inverse"].toBool();
+    torch::autograd::variable_list dx(7);
+    const bool dq = dy[0].defined(), dk = dy.size() > 1 && dy[1].defined();
+    if (dq || dk) {  // where only one of the two took part, it goes alone
+      const auto r = rotary(dq ? dy[0] : dy[1], dq && dk ? OptTensor(dy[1]) : OptTensor(), saved[0], saved[1], saved[2],
+                            interleaved, !inverse);
+      dx[dq ? 0 : 1] = *r[0];
+      if (dq && dk) dx[1] = *r[1];
+    }
+    return dx;
+  }
+};
+
+std::vector<OptTensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& cos_t,
+                              const Tensor& sin_t, bool interleaved, bool inverse) {
+  if (!torch::GradMode::is_enabled() || !(q.requires_grad() || (k.has_value() && k->requires_grad())))
+    return rotate(q, k, positions, cos_t, sin_t, interleaved, inverse);
+  auto y = Rotary::apply(q, k, positions, cos_t, sin_t, interleaved, inverse);
+  if (!k.has_value()) return {y[0], c10::nullopt};
+  return {y[0], y[1]};
 }
 
 Tensor rotary_cache(Tensor qkv, int64_t heads, int64_t kv_heads, int64_t head_dim, Tensor positions, Tensor cos_t,

@@ -106,59 +106,14 @@ def rotary_table(rotary_dim: int, max_positions: int, *, theta: float = 10000.0,
     return RotaryTable((angle.cos() * scale).float().to(device), (angle.sin() * scale).float().to(device), interleaved)
 
 
-class _Rotary(torch.autograd.Function):
-    """Linear in (q, k): the backward is the transposed rotation, differentiable again."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, cos, sin, interleaved: bool, inverse: bool):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, cos, sin)
-        ctx.flags = interleaved, inverse
-        return tuple(require().rotary(q, k, positions, cos, sin, interleaved, inverse))
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        positions, cos, sin = ctx.saved_tensors
-        interleaved, inverse = ctx.flags
-        if dq is None and dk is None:
-            return None, None, None, None, None, None, None
-        if dq is None:  # only one of the two took part
-            return None, _apply(dk, None, positions, cos, sin, interleaved, not inverse)[0], None, None, None, None, None
-        dq, dk = _apply(dq, dk, positions, cos, sin, interleaved, not inverse)
-        return dq, dk, None, None, None, None, None
-
-
-class _RotaryOne(torch.autograd.Function):
-    """``_Rotary`` of a single tensor (a function may not return ``None`` beside a tensor's gradient)."""
-
-    @staticmethod
-    def forward(ctx, q, positions, cos, sin, interleaved: bool, inverse: bool):
-        ctx.save_for_backward(positions, cos, sin)
-        ctx.flags = interleaved, inverse
-        return require().rotary(q, None, positions, cos, sin, interleaved, inverse)[0]
-
-    @staticmethod
-    def backward(ctx, dq):
-        positions, cos, sin = ctx.saved_tensors
-        interleaved, inverse = ctx.flags
-        return _apply(dq, None, positions, cos, sin, interleaved, not inverse)[0], None, None, None, None, None
-
-
-def _apply(q, k, positions, cos, sin, interleaved: bool, inverse: bool):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        if k is None:
-            return _RotaryOne.apply(q, positions, cos, sin, interleaved, inverse), None
-        return _Rotary.apply(q, k, positions, cos, sin, interleaved, inverse)
-    return tuple(require().rotary(q, k, positions, cos, sin, interleaved, inverse))
-
-
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: RotaryTable):
     """``q`` ``[..., H, D]`` and ``k`` ``[..., Hkv, D]`` (bf16, fp16 or fp32; the same leading
     dimensions; strided views are read in place) rotated by ``positions`` ``[...]`` (int32 or
     int64).  Returns new contiguous tensors ``(q', k')`` (``k'`` is ``None`` without ``k``), with
-    gradients for ``q`` and ``k``.  Elements behind ``table.rotary_dim`` pass through; a position
+    gradients for ``q`` and ``k`` (of any order; a backward pass captured into a CUDA graph needs, as
+    with every operator, that no eager graph of the same leaves is alive).  Elements behind ``table.rotary_dim`` pass through; a position
     outside the table gives NaN in the rotated part of its token."""
-    return _apply(q, k, positions, table.cos, table.sin, table.interleaved, False)
+    return tuple(require().rotary(q, k, positions, table.cos, table.sin, table.interleaved, False))
 
 
 def rotary_cache(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int, positions: torch.Tensor,

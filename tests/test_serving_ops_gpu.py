@@ -142,6 +142,35 @@ def test_rotary_only_one_gradient_and_bad_positions():
     assert rotary(e, e[:, :1], torch.empty(0, device=DEV, dtype=torch.long), table)[1].shape == (0, 1, 64)
 
 
+def test_rotary_backward_in_a_captured_graph():
+    """Forward and backward captured, then replayed on other gradients and positions.  (No eager graph of the
+    same leaves may be alive then: their accumulation nodes belong to the stream of that graph.)"""
+    from pdattention_b200.ops.rotary import rotary, rotary_table
+
+    torch.manual_seed(6)
+    table = rotary_table(32, 50, interleaved=True, device=DEV)
+    q = torch.randn(11, 3, 64, device=DEV, requires_grad=True)
+    k = torch.randn(11, 1, 64, device=DEV, requires_grad=True)
+    pos = torch.randint(0, 50, (11,), device=DEV)
+    w = torch.randn_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm-up on a side stream, as captures want
+        torch.autograd.grad((rotary(q, k, pos, table)[0] * w).sum(), q)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, z = rotary(q, k, pos, table)
+        dq, dk = torch.autograd.grad((y * w).sum() + z.sum(), (q, k))
+    with torch.no_grad():
+        w.mul_(2)
+        pos.add_(-1).clamp_(min=0)
+    graph.replay()
+    want = torch.autograd.grad((rotary(q, k, pos, table)[0] * w).sum(), q)[0]
+    assert torch.equal(dq, want)
+    assert ((dk.double() - rotate64(torch.ones_like(k), pos, table, True)).abs() <= 2.0 ** -21).all()
+
+
 @pytest.mark.parametrize("tokens,heads,kv,dim,rot,interleaved", [(1, 8, 2, 64, 64, False), (77, 28, 4, 128, 128, False),
                                                                   (300, 12, 12, 64, 32, True), (5, 3, 1, 128, 18, False)])
 def test_rotary_cache(tokens, heads, kv, dim, rot, interleaved):
