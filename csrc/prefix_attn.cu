@@ -32,6 +32,9 @@
 // not 0).  Every wait is bounded; a CTA that times out sets *status, waits (bounded) for its copies
 // and MMAs in flight, frees its TMEM and returns.
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "serving.h"
 #include "tcgen05.cuh"
@@ -997,6 +1000,22 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const PrefixMer
   }
 }
 
+// Shared memory of a kernel, and the whole of an SM's for it: an SM only runs CTAs of two kernels side
+// by side under one split between L1 and shared memory.  Once per kernel and device.
+cudaError_t prepare(const void* kernel, int bytes) {
+  static std::mutex mu;
+  static auto* done = new std::map<std::pair<const void*, int>, int>();  // never freed
+  int dev = 0;
+  PRA_RETURN_IF_ERROR(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(mu);
+  int& have = (*done)[{kernel, dev}];
+  if (have >= bytes) return cudaSuccess;
+  PRA_RETURN_IF_ERROR(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  PRA_RETURN_IF_ERROR(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  have = bytes;
+  return cudaSuccess;
+}
+
 bool encode(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t row, int64_t batches, int64_t batch,
             int keys) {
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batches};
@@ -1022,7 +1041,7 @@ cudaError_t launch(const PrefixAttnArgs& a, cudaStream_t st) {
   if (!ok) return cudaErrorInvalidValue;
   if (!a.use_prefix) pk = k, pv = v;
   if (!a.use_own) k = pk, v = pv;
-  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(prefix_kernel<D, NT>), C::SMEM));
+  PRA_RETURN_IF_ERROR(prepare(reinterpret_cast<const void*>(prefix_kernel<D, NT>), C::SMEM));
   const int tiles = (rows_of(a) + NT * BM - 1) / (NT * BM);
   const int64_t items = (int64_t)tiles * a.Hkv * (a.packed ? 1 : a.B);
   if (items > INT32_MAX || a.splits > 65535) return cudaErrorInvalidValue;
@@ -1067,7 +1086,7 @@ cudaError_t launch_own(const OwnAttnArgs& a, cudaStream_t st) {
   if (!encode(&k, a.k, width, a.cap, a.k_row, a.B, a.k_batch, OB) || !encode(&v, a.v, width, a.cap, a.v_row, a.B, a.v_batch, OB))
     return cudaErrorInvalidValue;
   const int smem = C::smem(a.T * (a.H / a.Hkv));
-  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(own_kernel<D, NB>), smem));
+  PRA_RETURN_IF_ERROR(prepare(reinterpret_cast<const void*>(own_kernel<D, NB>), smem));
   return pra_launch_pdl(own_kernel<D, NB>, dim3(a.ctas), dim3(C::THREADS), smem, st, k, v, a);
 }
 

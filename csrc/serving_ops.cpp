@@ -463,31 +463,42 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     a.splits = splits_for(a, prefix_blocks);
   }
   if (few) {
-    // Where the prefix part is bound by its products (two tiles a CTA) and the own part by HBM, both run
-    // at once, each on its SMs: those that make the longer of the two shortest.  Times as measured (us): a
-    // prefix CTA 8 + 2 per block of 128 keys (D = 64: 1.6), an own SM 6 + 1 per 75 KB, one after the
-    // other 4 more and 6 KB/ns for the own keys.  The lengths are not known here: half of the capacity.
-    // 64 rows behind 8K with 64 to 1,024 own keys 68 -> 55 us, 128 rows behind 32K 140 -> 124 us.
-    int own_sms = 0;
-    int tiles = 1, slots = 1;
-    if (a.P > 0) pra_prefix_attention_shape(a, &tiles, &slots);
-    const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-    if (a.P > 0 && slots == sms) {
-      const double per_block = head_dim == 128 ? 2.0 : 1.6, own_kb = 2e-3 * B * a.cap * width;
-      const auto prefix_us = [&](int splits) { return 8 + per_block * ceil_div(prefix_blocks, splits); };
-      double best = prefix_us(a.splits) + 4 + own_kb / 6000;
-      for (int s = 4; s <= sms * 3 / 4; s += 4) {
-        const int splits = (sms - s) / tiles;
-        if (splits < 1) break;
-        const double us = std::max(prefix_us(std::min(splits, prefix_blocks)), 6 + own_kb / (75.0 * s));
-        if (us < best) {
-          best = us;
-          own_sms = s;
+    // Both parts at once where that is shorter.  The lengths are not known here: half of the capacity.
+    // Times as measured (us): a prefix CTA 8 + 2 per block of 128 keys (D = 64: 1.6; two CTAs of one tile on an
+    // SM 2.9 and 2), own keys 6 + 1 per 6 MB.
+    int own_ctas = INT32_MAX;
+    if (a.P > 0) {
+      int tiles, slots;
+      pra_prefix_attention_shape(a, &tiles, &slots);
+      const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+      const double own_kb = 2e-3 * B * a.cap * width, alone = head_dim == 128 ? 2.0 : 1.6;
+      const auto prefix_us = [&](int splits, double per_block) { return 8 + per_block * ceil_div(prefix_blocks, splits); };
+      if (slots == sms) {
+        // Two tiles a CTA: the prefix part is bound by its products and the own part by HBM, each takes its SMs
+        // (an own SM reads 75 KB/us).  64 rows behind 8K with 64 to 1,024 own keys 68 -> 45 us, 128 rows behind
+        // 32K 140 -> 117 us.
+        double best = prefix_us(a.splits, alone) + 4 + own_kb / 6000;
+        int own_sms = 0;
+        for (int s = 4; s <= sms * 3 / 4 && (sms - s) / tiles >= 1; s += 4) {
+          const double us = std::max(prefix_us(std::min((sms - s) / tiles, prefix_blocks), alone), 6 + own_kb / (75.0 * s));
+          if (us < best) {
+            best = us;
+            own_sms = s;
+          }
         }
-      }
-      if (own_sms > 0) {
-        a.splits = std::min(prefix_blocks, (sms - own_sms) / tiles);
-        own_sms = sms - a.splits * tiles;
+        if (own_sms > 0) {
+          a.splits = std::min(prefix_blocks, (sms - own_sms) / tiles);
+          own_ctas = 2 * (sms - a.splits * tiles);
+        }
+      } else if (tiles <= sms) {
+        // One tile a CTA: a CTA of each part fits on an SM.
+        const int splits = std::min(prefix_blocks, sms / tiles);
+        const double both = std::max(prefix_us(splits, alone), 6 + own_kb / 6000);
+        const double after = prefix_us(a.splits, a.splits > splits ? (head_dim == 128 ? 2.9 : 2.0) : alone) + 4 + own_kb / 6000;
+        if (both < after) {
+          a.splits = splits;
+          own_ctas = sms;
+        }
       }
     }
     if (a.P > 0) {
@@ -515,7 +526,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     o.status = a.status;
     o.after_prefix = a.P > 0;
     o.ctas = pra_own_attention_ctas(o);
-    if (own_sms > 0) o.ctas = std::min(o.ctas, 2 * own_sms);
+    o.ctas = std::min(o.ctas, own_ctas);
     const int64_t items = B * kv_heads, pieces = (items + o.ctas) * rows;
     // one workspace: the pieces' sums, their (max, sum) pairs, the items' first and last CTAs
     auto work = torch::empty({pieces * (head_dim + 2) + 2 * items}, fo);
