@@ -80,6 +80,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if on
   return m;
 }
 
+// Two weights >= 0 rounded to bf16 (to nearest, a tie upwards) on the integer pipe: the conversion
+// instruction competes with the exponentials (545 -> 530 us for 4 x 512 queries behind 16K).
+__device__ __forceinline__ uint32_t pack_near(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
+}
+
 // Two fp32 values in one 64-bit register pair, and the packed operations on them.
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 pack2(float a, float b) {
@@ -441,7 +447,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
           p0 = ex2(p0);
           p1 = ex2(p1);
           sum[c & 1] = add2(sum[c & 1], pack2(p0, p1));
-          w[c] = pack_bf16(p0, p1);
+          w[c] = pack_near(p0, p1);
         }
         tc::st32(t_s + half * W, w);
         tc::fence_before();

@@ -382,13 +382,22 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   a.scale = (float)scale;
   a.status = pra_attention_status_word(q.device());
   const auto fo = q.options().dtype(at::kFloat);
-  Tensor part_o, part_ml;
-  const auto workspace = [&](int n) {
-    part_o = torch::empty({B * T, heads, n, head_dim}, fo);
-    part_ml = torch::empty({B * T, heads, n, 2}, fo);
-    a.n_slots = n;
-    a.part_o = part_o.data_ptr<float>();
-    a.part_ml = part_ml.data_ptr<float>();
+  // One allocation for the call's parts: n slots of sums and (max, sum) pairs per query, and `more` floats.
+  Tensor work;
+  const auto workspace = [&](int64_t n, int64_t more) {
+    const int64_t queries = B * T * heads, own = (queries * n * (head_dim + 2) + 3) / 4 * 4;  // what follows: 16-byte aligned
+    work = torch::empty({own + more}, fo);
+    a.n_slots = (int)n;
+    a.part_o = n > 0 ? work.data_ptr<float>() : nullptr;
+    a.part_ml = n > 0 ? a.part_o + queries * n * head_dim : nullptr;
+    return work.data_ptr<float>() + own;
+  };
+  // The joined partial that a call for partials returns.
+  Tensor joined_o, joined_ml;
+  const auto joined = [&]() -> std::vector<OptTensor> {
+    joined_o = torch::empty({B * T, heads, 1, head_dim}, fo);
+    joined_ml = torch::empty({B * T, heads, 1, 2}, fo);
+    return {joined_o, joined_ml};
   };
   Tensor out;
   if (!partials) out = torch::empty({B, T, heads * head_dim}, q.options());
@@ -401,9 +410,9 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   }
   if (B == 0 || T == 0 || (a.P == 0 && a.cap == 0)) {
     if (partials) {
-      workspace(1);
-      part_ml.fill_(-INFINITY);
-      return {part_o, part_ml};
+      auto r = joined();
+      joined_ml.fill_(-INFINITY);
+      return r;
     }
     out.zero_();
     if (return_lse) result[1]->fill_(-INFINITY);
@@ -423,14 +432,12 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   m.H = a.H;
   m.Hkv = a.Hkv;
   m.D = a.D;
-  Tensor joined_o, joined_ml;
   const auto merge = [&]() -> std::vector<OptTensor> {
     m.part_o = a.part_o;
     m.part_ml = a.part_ml;
     m.n_slots = a.part_o != nullptr ? a.n_slots : 0;
+    auto r = partials ? joined() : result;
     if (partials) {
-      joined_o = torch::empty({B * T, heads, 1, head_dim}, fo);
-      joined_ml = torch::empty({B * T, heads, 1, 2}, fo);
       m.joined_o = joined_o.data_ptr<float>();
       m.joined_ml = joined_ml.data_ptr<float>();
     } else {
@@ -438,8 +445,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
       m.lse = lse;
     }
     check(pra_prefix_merge(m, stream()), "shared_prefix_attention");
-    if (partials) return {joined_o, joined_ml};
-    return result;
+    return r;
   };
   const int64_t rows = T * G;  // query rows of a (batch row, KV head)
   const bool few = rows <= PRA_OWN_ROWS && a.cap > 0;
@@ -451,11 +457,17 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     a.use_prefix = a.P > 0;
     a.use_own = a.cap > 0;
     a.splits = splits_for(a, prefix_blocks + own_blocks);
-    if (a.splits > 1 || partials) workspace(a.splits);
+    std::vector<OptTensor> r = result;
+    if (a.splits > 1) {
+      workspace(a.splits, 0);
+    } else if (partials) {
+      r = joined();
+      a.part_o = joined_o.data_ptr<float>();
+      a.part_ml = joined_ml.data_ptr<float>();
+      a.n_slots = 1;
+    }
     check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
-    if (a.splits > 1) return merge();
-    if (partials) return {part_o, part_ml};
-    return result;
+    return a.splits > 1 ? merge() : r;
   }
   PrefixAttnArgs own = a;
   if (a.P > 0) {
@@ -501,10 +513,6 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
         }
       }
     }
-    if (a.P > 0) {
-      workspace(a.splits);
-      check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
-    }
     OwnAttnArgs o{};
     o.q = a.q;
     o.q_batch = a.q_batch;
@@ -527,10 +535,9 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     o.after_prefix = a.P > 0;
     o.ctas = pra_own_attention_ctas(o);
     o.ctas = std::min(o.ctas, own_ctas);
+    // behind the slots: the pieces' sums, their (max, sum) pairs, the items' first and last CTAs
     const int64_t items = B * kv_heads, pieces = (items + o.ctas) * rows;
-    // one workspace: the pieces' sums, their (max, sum) pairs, the items' first and last CTAs
-    auto work = torch::empty({pieces * (head_dim + 2) + 2 * items}, fo);
-    o.piece_o = work.data_ptr<float>();
+    o.piece_o = workspace(a.P > 0 ? a.splits : 0, pieces * (head_dim + 2) + 2 * items);
     o.piece_ml = o.piece_o + pieces * head_dim;
     o.first = reinterpret_cast<int*>(o.piece_ml + pieces * 2);
     o.last = o.first + items;
@@ -538,12 +545,13 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     m.piece_ml = o.piece_ml;
     m.first = o.first;
     m.last = o.last;
+    if (a.P > 0) check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
     check(pra_own_attention(o, stream()), "shared_prefix_attention");
     return merge();
   }
   own.use_own = 1;
   own.splits = splits_for(own, own_blocks);
-  workspace(a.splits + own.splits);
+  workspace(a.splits + own.splits, 0);
   own.part_o = a.part_o;
   own.part_ml = a.part_ml;
   own.n_slots = a.n_slots;
@@ -566,6 +574,8 @@ std::vector<OptTensor> merge_attention_partials(Tensor part_o, Tensor part_ml, O
                     o.sizes().slice(0, 3) == ml.sizes().slice(0, 3) && o.size(0) == part_o.size(0) &&
                     o.size(1) == part_o.size(1) && o.size(3) == part_o.size(3),
                 "partials must be contiguous [B * T, H, n, D] and [B * T, H, n, 2]");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(ml.data_ptr()) % 8 == 0,
+                "partials must start on a 16-byte boundary");
   };
   set(part_o, part_ml);
   const int64_t rows = part_o.size(0), H = part_o.size(1), D = part_o.size(3);

@@ -244,6 +244,7 @@ CASES = [
     (7, 5, 333, 90, 12, 12, 64), (4, 3, 260, 17, 32, 4, 128), (2, 70, 400, 150, 8, 2, 128), (3, 129, 77, 200, 4, 4, 64),
     (2, 300, 257, 300, 8, 2, 128), (1, 1, 5000, 10, 32, 8, 128), (1, 513, 900, 600, 4, 1, 64), (2, 40, 130, 64, 64, 2, 64),
     (3, 1, 0, 200, 8, 2, 128), (3, 4, 0, 200, 8, 2, 64), (3, 2, 300, 0, 8, 2, 128), (33, 1, 150, 40, 40, 2, 128),
+    (3, 1, 200, 50, 3, 1, 128), (5, 3, 700, 9, 3, 3, 128), (1, 2, 65, 7, 5, 5, 128),  # odd counts of partials
 ]
 
 
@@ -555,6 +556,33 @@ def test_refusals_of_rotary():
     refused(lambda: ok(k_cache=cache[:, :32]), "caches")
     refused(lambda: ok(v_cache=cache[:4]), "caches")
     refused(lambda: ok(v_cache=cache.float()), "dtype")
+
+
+def test_partials_join_to_the_same_attention():
+    from pdattention_b200.inference.shared_prefix import (merge_attention_partials, shared_prefix_attention,
+                                                          shared_prefix_partials)
+
+    torch.manual_seed(9)
+    for B, T, P, cap, H, Hkv, D in [(5, 1, 300, 40, 8, 2, 128), (2, 300, 200, 300, 4, 2, 64), (3, 20, 130, 30, 8, 2, 64), (2, 1, 0, 0, 4, 4, 64)]:
+        w = Hkv * D
+        q = torch.randn(B, T, H * D, device=DEV).bfloat16()
+        pk, pv = torch.randn(2, P, w, device=DEV).bfloat16()
+        k, v = torch.randn(2, B, cap, w, device=DEV).bfloat16()
+        ln = torch.full((B,), cap, dtype=torch.int32, device=DEV)
+        args = (q, pk, pv, k, v, ln, H, Hkv, D)
+        want = shared_prefix_attention(*args, return_lse=True)
+        parts = shared_prefix_partials(*args)
+        assert parts[0].shape == (B * T, H, 1, D) and parts[1].shape == (B * T, H, 1, 2)
+        out, lse = merge_attention_partials(parts, batch=B, return_lse=True)
+        # the same sums, divided by 1 / l in one place or the other: a last place of fp32 before the rounding
+        assert ((out.double() - want[0].double()).abs() <= half_step(torch.bfloat16) * 2 * want[0].double().abs() + 1e-30).all()
+        assert ((lse - want[1]).nan_to_num().abs() <= 2.0 ** -20 * (1 + want[1].nan_to_num(neginf=0).abs())).all()
+        # keys seen twice weigh twice: the same output, log 2 more
+        twice, lse2 = merge_attention_partials(parts, parts, batch=B, return_lse=True)
+        assert torch.equal(twice, out) and ((lse2 - lse - math.log(2)).nan_to_num().abs() <= 2.0 ** -19 * (1 + lse.nan_to_num(neginf=0).abs())).all()
+    refused(lambda: merge_attention_partials((parts[0], parts[1].double()), batch=2), "dtype")
+    refused(lambda: merge_attention_partials(parts, batch=3), "whole batch rows")
+    refused(lambda: merge_attention_partials((parts[0][..., :32].contiguous(), parts[1]), batch=2), "head_dim")
 
 
 def test_refusals_of_shared_prefix_attention():
