@@ -17,11 +17,15 @@
 // bias names (their ranks by a prefix sum of the bits), and for each such token its id and a word with
 // its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 bias entry + 1).  Integer atomics fill
 // them, so any order gives the same table.  The pass over all logits then only masks and takes
-// maxima, on packed 16-bit pairs, leaving out what is named; the named tokens follow one to a
-// thread.  (Looking the penalties up within the pass over all logits took 107 us for 256 rows of
-// 152,064 logits with 8,192 ids each, a word per token of the slice instead of the table 183 us.)  A
-// thread only remembers which vector held its maximum: the element is looked up at the end, by the
-// warps' winners.  A thread's first logits and mask bytes are loaded before the table is built.
+// maxima, on packed 16-bit pairs, leaving out what is named; the named tokens follow, four logits on
+// their way per thread.  Where the history may name half of a slice, a word per token takes no more
+// room and the history is walked once instead of twice (64 rows of 128,256 logits with 100,000 ids
+// each: 368 -> 138 us).  256 rows of 152,064 bf16 logits with 8,192 ids each take 54 us with cold caches
+// (28 without a history, 12.6 is what their bytes need): the two walks and the scattered logits of the
+// named tokens wait for memory, one after the other.  (Looking the penalties up within the pass over all
+// logits took 107 us, a word per token of the slice instead of the table 183 us.)  A thread only
+// remembers which vector held its maximum: the element is looked up at the end, by the warps' winners.
+// A thread's first logits and mask bytes are loaded before the table is built.
 #include <algorithm>
 #include <type_traits>
 
@@ -121,7 +125,7 @@ __host__ __device__ constexpr int bit_words(int slice) { return (slice + 31) / 3
 
 // T: type of the logits; V: elements of one access; TABLE: a history or biases are given.
 template <typename T, int V, bool TABLE>
-__global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int slice, int table_words) {
+__global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int slice, int table_words, bool direct) {
     constexpr int U = 3;  // accesses of a batch
   extern __shared__ uint32_t smem[];
   __shared__ uint32_t s_scan[NT / 32];
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
   uint32_t* rank = named + bit_words(slice);                    // [bit_words(slice)] table words before
   uint32_t* table = rank + bit_words(slice);                    // [table_words]
   uint32_t* token = table + table_words;                        // [table_words] their elements of the slice
-  int* bias_id = reinterpret_cast<int*>(token + table_words);   // [n_bias]
+  int* bias_id = reinterpret_cast<int*>(direct ? token : token + table_words);  // [n_bias] (direct: word t is token t's)
   float* bias_sum = reinterpret_cast<float*>(bias_id + a.n_bias);
   const int len = a.ids ? max(0, min(a.hist_len[b], a.capacity)) : 0;
   const float rep = a.repetition ? a.repetition[b] : 1.f;
@@ -204,10 +208,11 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
 #pragma unroll 4
       for (int i = done + tid; i < len; i += NT) visit(ids[i], i);
     };
-    walk([&](int id, int) { name(id); });
-    for (int i = tid; i < a.n_bias; i += NT) name(bias_id[i]);
-    __syncthreads();
-    {  // exclusive prefix sum of the words' bit counts, each thread a run of words
+    if (!direct) {
+      walk([&](int id, int) { name(id); });
+      for (int i = tid; i < a.n_bias; i += NT) name(bias_id[i]);
+      __syncthreads();
+      // exclusive prefix sum of the words' bit counts, each thread a run of words
       const int per = (words + NT - 1) / NT, first = min(tid * per, words), last = min(first + per, words);
       uint32_t mine = 0;
       for (int i = first; i < last; ++i) mine += __popc(named[i]);
@@ -228,11 +233,12 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
       for (int w = 0; w < NT / 32; ++w) named_tokens += s_scan[w];
       __syncthreads();
     }
+    auto place = [&](uint32_t t) { return direct ? t : entry_of(t); };
     walk([&](int id, int i) {
       const uint32_t t = (uint32_t)id - base;
       if (t >= (uint32_t)n) return;
-      const uint32_t at = entry_of(t);
-      token[at] = t;  // every occurrence writes the same
+      const uint32_t at = place(t);
+      if (!direct) token[at] = t;  // every occurrence writes the same
       if (i >= prompt) atomicAdd(table + at, 1u);
       else if (!(table[at] & SEEN)) atomicOr(table + at, SEEN);
     });
@@ -247,10 +253,18 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
       for (int j = i; j < a.n_bias; ++j)
         if (bias_id[j] == bias_id[i]) sum += a.bias_values[(int64_t)b * a.n_bias + j];
       bias_sum[i] = sum;
-      token[entry_of(t)] = t;
-      atomicOr(table + entry_of(t), (uint32_t)(i + 1) << 21);
+      if (!direct) token[place(t)] = t;
+      atomicOr(table + place(t), (uint32_t)(i + 1) << 21);
     }
     __syncthreads();
+    if (direct) {
+      for (int i = warp; i < words; i += NT / 32) {
+        const uint32_t bits = __ballot_sync(0xffffffffu, table[i * 32 + lane] != 0);
+        if (lane == 0) named[i] = bits;
+      }
+      named_tokens = n;
+      __syncthreads();
+    }
   }
   const bool choose = a.token != nullptr;
   float best = -INFINITY;  // largest so far, and the first vector that has it
@@ -315,21 +329,30 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
     // the named tokens, after their vectors have been written (in place, an allowed one is still as it came)
     if (y) __syncthreads();
     for (int i0 = tid; i0 < named_tokens; i0 += 4 * NT) {
-      float z4[4];  // four scattered logits on their way
+      float z4[4];  // four scattered logits and mask bytes on their way
+      int e4[4];
+      uint32_t bits4[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (i0 + u * NT < named_tokens) z4[u] = widen(x[token[i0 + u * NT]]);
+      for (int u = 0; u < 4; ++u) {
+        const int i = min(i0 + u * NT, named_tokens - 1);
+        e4[u] = direct ? i : token[i];
+        if (direct && table[i] == 0) continue;
+        z4[u] = widen(x[e4[u]]);
+        bits4[u] = none ? 0u : 0xFFu;
+        if (mask) bits4[u] = mask[e4[u] / 8];
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * NT;
         if (i >= named_tokens) break;
         const uint32_t w = table[i], times = w & COUNT;
-        const int e = token[i];
+        if (w == 0) continue;  // direct: not named
+        const int e = e4[u];
         float z = z4[u];
         if (w & (SEEN | COUNT)) z = z > 0.f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
         if (times) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)times)), pres);
         if (w >> 21) z = __fadd_rn(z, bias_sum[(w >> 21) - 1]);
-        if (!is_allowed(e)) z = -INFINITY;
+        if (!((bits4[u] >> (e & 7)) & 1u)) z = -INFINITY;
         if (choose) {
           const unsigned long long k = choice_key(z, (uint32_t)(a.vocab_start + v0 + e));
           key = k > key ? k : key;
@@ -388,21 +411,21 @@ cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   int cl = 8, slice = 0, table_words = 0;
+  bool direct = false;
   size_t bytes = 0;
   const auto shape = [&](int c) {
     cl = c;
     slice = ((a.V + cl - 1) / cl + 31) / 32 * 32;
-    table_words = TABLE ? (int)std::min<int64_t>(slice, (int64_t)a.capacity + a.n_bias) : 0;
-    bytes = TABLE ? (size_t)bit_words(slice) * 8 + (size_t)table_words * 8 + (size_t)a.n_bias * 8 : 0;
+    const int64_t most = std::min<int64_t>(slice, (int64_t)a.capacity + a.n_bias);  // tokens that may be named
+    direct = TABLE && 2 * most >= slice;
+    table_words = !TABLE ? 0 : direct ? slice : (int)most;
+    bytes = TABLE ? (size_t)bit_words(slice) * 8 + (size_t)table_words * (direct ? 4 : 8) + (size_t)a.n_bias * 8 : 0;
   };
   shape(8);
   while (cl > 1 && (int64_t)a.B * cl > 2 * sms) shape(cl / 2);
   while (cl < 8 && bytes > 110 * 1024) shape(cl * 2);
-  if (bytes > 220 * 1024) shape(16);
   auto kernel = rules_kernel<T, V, TABLE>;
   if (bytes > 48 * 1024) PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), (int)bytes));
-  if (cl > 8)
-    PRA_RETURN_IF_ERROR(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cl, a.B);
   cfg.blockDim = dim3(NT);
@@ -415,7 +438,7 @@ cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a, slice, table_words);
+  return cudaLaunchKernelEx(&cfg, kernel, a, slice, table_words, direct);
 }
 
 template <typename T>
