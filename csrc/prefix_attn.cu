@@ -957,9 +957,13 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const PrefixMer
     const float2* m2;
     const float* o2;
     find(s, m2, o2);
-    M = fmaxf(M, m2->x);
+    M = max3(M, m2->x, m2->x);
   }
-  M = warp_max(M);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) {  // NaN if one part's is: it must not pass for an empty row
+    const float other = __shfl_xor_sync(0xffffffffu, M, x);
+    M = max3(M, other, other);
+  }
   float L = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;

@@ -70,6 +70,7 @@ void rotary_tables(RotaryArgs& a, const Tensor& cos_t, const Tensor& sin_t, cons
   a.cos_t = cos_t.data_ptr<float>();
   a.sin_t = sin_t.data_ptr<float>();
   a.max_pos = cos_t.size(0);
+  TORCH_CHECK(a.max_pos > 0, "cos and sin hold no positions");
   a.rot = (int)(2 * cos_t.size(1));
   TORCH_CHECK(head_dim > 0 && head_dim % 2 == 0 && head_dim <= 4096, "head_dim must be even and at most 4096");
   TORCH_CHECK(a.rot >= 2 && a.rot <= head_dim, "the table rotates ", num(a.rot), " elements of a head of ",
@@ -305,7 +306,8 @@ std::vector<Tensor> choose_tokens(Tensor logits, OptTensor ids, OptTensor hist_l
   c10::cuda::CUDAGuard guard(logits.device());
   const int dtype = dtype_code(logits, "logits");
   LogitsArgs a = rules_args(logits, {ids, hist_len, prompt_len, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows}, vocab_start);
-  TORCH_CHECK(!append || a.ids != nullptr, "append needs a history");
+  TORCH_CHECK(!append || ids.has_value(), "append needs a history");
+  TORCH_CHECK(!append || ids->size(0) <= 1 || ids->stride(0) >= ids->size(1), "rows of an appended history overlap");
   auto token = torch::empty({logits.size(0)}, logits.options().dtype(at::kLong));
   auto value = torch::empty({logits.size(0)}, logits.options().dtype(at::kFloat));
   a.token = token.data_ptr<int64_t>();
@@ -336,7 +338,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   c10::cuda::CUDAGuard guard(q.device());
   TORCH_CHECK(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
   TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
-  TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive");
+  TORCH_CHECK(std::isfinite((float)scale) && (float)scale > 0, "scale must be positive, in 32 bits");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16, "q has dtype ", q.scalar_type(), ", expected bf16");
   TORCH_CHECK(q.dim() == 3 && q.size(2) == heads * head_dim, "q must be [B, T, heads * head_dim]");
   rows_ok(q, heads * head_dim, "q");

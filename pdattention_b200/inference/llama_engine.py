@@ -567,6 +567,7 @@ class PRALlamaEngine:
         memory), each chunk behind the ones before it; prefix tokens read no chunk memory."""
         self.prefix = None
         self.cache = self.cache_len = None  # a cache filled behind another prefix does not fit this one
+        self.release_graph()  # a captured step reads the prefix that has just gone
         if ids is None or ids.numel() == 0:
             return
         cfg = self.cfg
@@ -779,7 +780,7 @@ class PRALlamaEngine:
             return choose_tokens(local, rules, history, append=history is not None)[0]
         token, value = choose_tokens(local, rules, history, vocab_start=self.vocab_start)
         every = self.tp.gather_small(torch.stack([value, token.float()], dim=1)).view(-1, self.tp_size, 2)
-        score, ids = every[..., 0], every[..., 1]
+        score, ids = every[..., 0].nan_to_num(nan=float("inf"), posinf=float("inf"), neginf=float("-inf")), every[..., 1]
         top = score.max(dim=1, keepdim=True).values
         token = torch.where(score == top, ids, torch.full_like(ids, float("inf"))).min(dim=1).values.long()
         if history is not None:

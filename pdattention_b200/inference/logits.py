@@ -17,7 +17,8 @@ from ..ops._ext import require
 @dataclass
 class TokenHistory:
     """Token ids of every row so far: ``ids`` ``[B, capacity]`` int32, of which the first ``lengths[b]``
-    are valid and the first ``prompt_lengths[b]`` (``None``: none) are the prompt's."""
+    are valid (none where it is negative) and the first ``prompt_lengths[b]`` (``None``: none) are the
+    prompt's; the capacity stays under 2^20."""
 
     ids: torch.Tensor
     lengths: torch.Tensor
@@ -33,12 +34,14 @@ class TokenHistory:
 
     def append(self, tokens: torch.Tensor) -> None:
         """Add ``tokens`` ``[B]`` (negative: none); a full row keeps what it has.  No host read."""
-        place = self.lengths.long()
+        if self.ids.shape[1] == 0:
+            return
+        place = self.lengths.long().clamp(min=0)
         room = (place < self.ids.shape[1]) & (tokens >= 0)
         at = place.clamp(max=self.ids.shape[1] - 1)[:, None]
         kept = torch.where(room[:, None], tokens[:, None].to(torch.int32), self.ids.gather(1, at))
         self.ids.scatter_(1, at, kept)
-        self.lengths.add_(room.to(torch.int32))
+        self.lengths.copy_(torch.where(room, (place + 1).to(torch.int32), self.lengths))
 
 
 @dataclass
@@ -54,7 +57,8 @@ class LogitsRules:
       allowed, the others become -inf; ``mask_rows`` ``[B]`` int32 names each row's mask (negative: no
       mask; ``M`` or more: nothing is allowed), by default mask ``b`` for row ``b``.
 
-    Penalties are fp32, absent ones are left out.
+    Penalties are fp32, absent ones are left out.  A history or biases take up to 393,216 columns,
+    a call up to 65,535 rows.
     """
 
     repetition: torch.Tensor | None = None
@@ -70,7 +74,7 @@ def process_logits(logits: torch.Tensor, rules: LogitsRules, history: TokenHisto
                    out: torch.Tensor | None = None, vocab_start: int = 0) -> torch.Tensor:
     """``logits`` ``[B, V]`` (bf16, fp16 or fp32, rows may be strided) after the rules, in a new tensor or
     in ``out`` (which may be ``logits``).  ``vocab_start``: the token id of column 0 when the columns are
-    a slice of the vocabulary (a multiple of 8)."""
+    a slice of the vocabulary (a multiple of 8).  No gradients."""
     h = history
     return require().process_logits(logits, out, h.ids if h else None, h.lengths if h else None,
                                     h.prompt_lengths if h else None, rules.repetition, rules.presence, rules.frequency,

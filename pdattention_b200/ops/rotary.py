@@ -111,8 +111,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, tab
     dimensions; strided views are read in place) rotated by ``positions`` ``[...]`` (int32 or
     int64).  Returns new contiguous tensors ``(q', k')`` (``k'`` is ``None`` without ``k``), with
     gradients for ``q`` and ``k`` (of any order; a backward pass captured into a CUDA graph needs, as
-    with every operator, that no eager graph of the same leaves is alive).  Elements behind ``table.rotary_dim`` pass through; a position
-    outside the table gives NaN in the rotated part of its token."""
+    with every operator, that no eager graph of the same leaves is alive).  Elements behind
+    ``table.rotary_dim`` pass through; a position outside the table gives NaN in the rotated part of its
+    token."""
     return tuple(require().rotary(q, k, positions, table.cos, table.sin, table.interleaved, False))
 
 

@@ -92,6 +92,12 @@ def test_history_appends_on_any_device():
     h.append(torch.tensor([9, 4]))  # row 0 is full
     assert h.ids.tolist() == [[5, 6, 1], [7, 4, 0]] and h.lengths.tolist() == [3, 2]
     assert h.prompt_lengths.tolist() == [2, 1]
+    h.lengths[1] = -3  # a negative length: nothing yet
+    h.append(torch.tensor([2, 8]))
+    assert h.ids.tolist() == [[5, 6, 1], [8, 4, 0]] and h.lengths.tolist() == [3, 1]
+    none = TokenHistory(torch.zeros((2, 0), dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+    none.append(torch.tensor([1, 2]))
+    assert none.lengths.tolist() == [0, 0]
 
 
 @pytest.mark.parametrize("family,scaling", [

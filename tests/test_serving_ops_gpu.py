@@ -428,7 +428,8 @@ def make_rules(B, V, hist, biases, mask, seed=0):
 @pytest.mark.parametrize("B,V,hist,biases,mask", [(1, 1, 3, 0, False), (2, 31, 5, 3, True), (6, 1000, 0, 0, True),
                                                   (5, 4099, 64, 300, True), (3, 32768, 2000, 0, False),
                                                   (4, 50257, 100, 17, True), (7, 128256, 700, 40, True),
-                                                  (2, 5000, 30001, 2047, True), (1, 393216, 60000, 2047, False)])
+                                                  (2, 5000, 30001, 2047, True), (1, 393216, 60000, 2047, False),
+                                                  (150, 2000, 1500, 2, True), (150, 2500, 30, 0, False)])
 def test_process_and_choose(dtype, B, V, hist, biases, mask):
     from pdattention_b200.inference.logits import choose_tokens, process_logits
 
@@ -522,6 +523,11 @@ def test_logits_repeats_exactly_and_appends_in_a_graph():
     assert history.lengths.tolist() == [10, 6, 9] and history.ids[0, 9] == 1
     choose_tokens(logits, rules, history, append=True)
     assert history.lengths.tolist() == [10, 7, 10]
+    i32 = lambda *s: torch.zeros(*s, device=DEV, dtype=torch.int32)  # noqa: E731
+    for rows, capacity in ((0, 4), (2, 0)):  # no rows; no room
+        h = TokenHistory(i32(rows, capacity), i32(rows))
+        token, _ = choose_tokens(logits[:rows], LogitsRules(), h, append=True)
+        assert token.tolist() == logits[:rows].argmax(1).tolist() and h.lengths.tolist() == [0] * rows
 
 
 # ---------------------------------------------------------------------------------- refusals
@@ -545,6 +551,7 @@ def test_refusals_of_rotary():
     refused(lambda: rotary(q, None, pos.float(), t), "int32 or int64")
     refused(lambda: rotary(q, None, pos.cpu(), t), "must be on")
     refused(lambda: rotary(q, None, pos, RotaryTable(t.cos.double(), t.sin)), "dtype")
+    refused(lambda: rotary(q, None, pos, RotaryTable(t.cos[:0], t.sin[:0])), "no positions")
     qkv, cache = torch.zeros(3, 4 * 64, device=DEV).bfloat16(), torch.zeros(8, 64, device=DEV).bfloat16()
     slots = torch.arange(3, device=DEV, dtype=torch.int32)
     ok = lambda **kw: rotary_cache(**{**dict(qkv=qkv, heads=2, kv_heads=1, head_dim=64, positions=pos, table=t,  # noqa: E731
@@ -585,6 +592,48 @@ def test_partials_join_to_the_same_attention():
     refused(lambda: merge_attention_partials((parts[0][..., :32].contiguous(), parts[1]), batch=2), "head_dim")
 
 
+@pytest.mark.parametrize("B,T,P,cap,bad", [(4, 1, 300, 0, "prefix"), (4, 1, 300, 20, "prefix"), (4, 1, 300, 20, "own"),
+                                           (1, 1, 5000, 20, "prefix"), (2, 40, 700, 50, "prefix")])
+def test_a_visible_nan_reaches_its_rows(B, T, P, cap, bad):
+    """A NaN key that a row sees makes that row NaN, its log sum too, and no other row."""
+    from pdattention_b200.inference.shared_prefix import (merge_attention_partials, shared_prefix_attention,
+                                                          shared_prefix_partials)
+
+    torch.manual_seed(5)
+    H, Hkv, D = 4, 2, 64
+    q = torch.randn(B, T, H * D, device=DEV).bfloat16()
+    pk, pv = torch.randn(2, P, Hkv * D, device=DEV).bfloat16()
+    k, v = torch.randn(2, B, cap, Hkv * D, device=DEV).bfloat16()
+    ln = torch.full((B,), cap, dtype=torch.int32, device=DEV)
+    see = torch.full((B,), P, dtype=torch.int32, device=DEV)
+    if bad == "prefix":
+        pk[150:] = float("nan")  # some parts hold nothing but NaN
+        see[1:] = 150
+        if cap:
+            ln[0] = T - 1 if T > 1 else 0
+        hit = torch.arange(B, device=DEV) == 0
+    else:
+        k[-1] = float("nan")
+        hit = torch.arange(B, device=DEV) == B - 1
+    args = (q, pk, pv, k, v, ln, H, Hkv, D)
+    out, lse = shared_prefix_attention(*args, prefix_lengths=see, return_lse=True)
+    assert torch.equal(out.isnan().any(-1).all(-1), hit) and torch.equal(out.isnan().all(-1).any(-1), hit)
+    assert torch.equal(lse.isnan().flatten(1).all(1), hit) and torch.equal(lse.isnan().flatten(1).any(1), hit)
+    o, ml = shared_prefix_partials(*args, prefix_lengths=see)
+    out, lse = merge_attention_partials((o, ml), (torch.zeros_like(o), torch.full_like(ml, NEG)), batch=B, return_lse=True)
+    assert torch.equal(out.isnan().flatten(1).all(1), hit) and torch.equal(lse.isnan().flatten(1).any(1), hit)
+
+
+def test_a_part_of_nan_is_no_empty_part():
+    from pdattention_b200.inference.shared_prefix import merge_attention_partials
+
+    o = torch.zeros(2, 1, 40, 64, device=DEV)
+    ml = torch.full((2, 1, 40, 2), NEG, device=DEV)
+    ml[0, 0, 37] = float("nan")
+    out, lse = merge_attention_partials((o, ml), batch=2, return_lse=True)
+    assert out[0].isnan().all() and lse[0].isnan().all() and (out[1] == 0).all() and (lse[1] == NEG).all()
+
+
 def test_refusals_of_shared_prefix_attention():
     from pdattention_b200.inference.shared_prefix import shared_prefix_attention
 
@@ -607,6 +656,8 @@ def test_refusals_of_shared_prefix_attention():
     refused(lambda: ok(lengths=base["lengths"][:1]), "entries")
     refused(lambda: ok(lengths=base["lengths"].cpu()), "must be on")
     refused(lambda: ok(scale=0.0), "scale")
+    refused(lambda: ok(scale=1e-50), "scale")
+    refused(lambda: ok(scale=1e50), "scale")
     refused(lambda: ok(prefix_lengths=torch.ones(B, device=DEV)), "dtype")
     refused(lambda: ok(prefix_k=z(P, Hkv * D + 4)[:, : Hkv * D]), "multiples of 16 bytes")
     refused(lambda: ok(prefix_k=z(P * Hkv * D + 1)[1:].view(P, Hkv * D)), "16-byte boundary")
@@ -638,3 +689,4 @@ def test_refusals_of_logits_rules():
     refused(lambda: process_logits(x.view(-1)[:100].view(1, 100), LogitsRules(), out=x.view(-1)[10:110].view(1, 100)), "overlap")
     refused(lambda: process_logits(torch.zeros(1, 384 * 1024 + 8, device=DEV), LogitsRules(), TokenHistory(i32(1, 2), i32(1))), "columns")
     refused(lambda: choose_tokens(x, LogitsRules(), append=True), "append")
+    refused(lambda: choose_tokens(x, LogitsRules(), TokenHistory(i32(1, 5).expand(B, -1), i32(B)), append=True), "overlap")
