@@ -12,20 +12,22 @@
 //     (P from TMEM), each committed to an mbarrier;
 //   * a warpgroup per tile does the softmax, one thread per query row (TMEM lane): a block's 128 scores
 //     come into registers once, the running maximum is raised lazily (only when it grows by more
-//     than 2^8, then O is rescaled in TMEM), and P goes back over S's columns as bf16 in two halves, so
-//     that P V of the first begins while the second is computed.
+//     than 2^8, then O is rescaled in TMEM), and P goes back over S's columns as bf16, 96 keys and then 32,
+//     so that P V of the first begins while the rest is computed and little is left to wait for after it.
 // P shares S's columns (S, P and O of two tiles fill TMEM), so S_{j+1} of a tile is issued only after
 // P V_j of that tile has completed; the issuer takes the tiles in turn, which keeps one tile's softmax
 // beside the other's products.  P is rounded to bf16 (one half step, 2^-8 relative, of each weight: the
 // tensor cores take 16-bit operands); the row sums use the unrounded weights, and S, O, maxima and
 // sums stay in fp32.
 //
-// What bounds it: a tile's chain of about 3,800 cycles per block (softmax 2,000, two products of 512,
+// What bounds it: a tile's chain of about 3,200 cycles per block (softmax 1,800, two products of 512,
 // the rest hand-overs of 200 to 300 between the roles), against 2,048 cycles of products and 2,048 of
-// exponentials for both tiles: 1.0 to 1.1 PFLOP/s on long suffixes.  Measured beside it at 4 x 512
-// queries behind 16,384 keys (560 us): an issuer per tile 780 us (the tiles fall into step and compete),
-// two threads per row 573, S in two buffers of 64 columns 777 (an MMA of 64 columns takes 57 cycles, one
-// of 128 takes 65), a quarter of the exponentials as polynomials 557 to 600.
+// exponentials for both tiles: 1.14 to 1.26 PFLOP/s on long suffixes (4 x 512 queries behind 16,384 keys
+// 490 us).  Measured beside it: an issuer per tile, or one that serves whichever tile is ready, half as long
+// again (the tiles fall into step and compete for the tensor cores); two threads per row 2% longer; S in
+// two buffers of 64 columns 40% (an MMA of 64 columns takes 57 cycles, one of 128 takes 65); a quarter of
+// the exponentials as polynomials as long or longer; only one tile in its exponentials at a time 9% longer;
+// 224 registers for the softmax warps (setmaxnreg, with two idle warps) 2% longer.
 //
 // Keys past the ones any query of the CTA may see are never multiplied: their scores are replaced by
 // -inf, and their value rows are zeroed in shared memory (a stale row may hold NaN, and 0 * NaN is
@@ -44,6 +46,8 @@ namespace prefix {
 
 constexpr int BM = 128;  // query rows of a tile
 constexpr int BN = 128;  // keys of a block
+constexpr int HEAD = 96;  // of which P V takes these first
+static_assert(HEAD % 32 == 0 && HEAD < BN, "weights are stored 32 keys at a time");
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_LOG2 = 8.f;
 constexpr long long WAIT_CYCLES = 4000000000LL;
@@ -78,12 +82,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if on
   float m;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
   return m;
-}
-
-// Two weights >= 0 rounded to bf16 (to nearest, a tie upwards) on the integer pipe: the conversion
-// instruction competes with the exponentials (545 -> 530 us for 4 x 512 queries behind 16K).
-__device__ __forceinline__ uint32_t pack_near(float lo, float hi) {
-  return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
 }
 
 // Two fp32 values in one 64-bit register pair, and the packed operations on them.
@@ -189,8 +187,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [R] a ring tile has landed
   uint64_t* empty = full + R;                                        // [R] a ring tile has been read
   uint64_t* s_full = empty + R;                                      // [NT] S_i is in TMEM
-  uint64_t* p_half = s_full + NT;                                    // [NT] half of P_i is in TMEM
-  uint64_t* p_full = p_half + NT;                                    // [NT] all of P_i is
+  uint64_t* p_head = s_full + NT;                                    // [NT] the first HEAD keys' P_i is in TMEM
+  uint64_t* p_full = p_head + NT;                                    // [NT] all of P_i is
   uint64_t* o_full = p_full + NT;                                    // [NT] O_i has P_i V
   uint64_t* q_full = o_full + NT;                                    // [NT] Q_i is in shared memory
   uint64_t* drain = q_full + NT;                                     // [1] every MMA issued has completed
@@ -209,7 +207,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     }
     for (int i = 0; i < NT; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_half + i, 4);
+      mbar_init(p_head + i, 4);
       mbar_init(p_full + i, 4);
       mbar_init(o_full + i, 1);
       mbar_init(q_full + i, 4);
@@ -285,9 +283,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
         tc::mma_bf16(tmem + i * BN, desc_sw128(q_addr + i * C::TILE + off, 16), desc_sw128(ring + r * C::TILE + off, 16), ID_S, kk > 0);
       }
     };
-    auto issue_o = [&](int i, int r, int half, bool acc) {  // 64 keys
+    auto issue_o = [&](int i, int r, bool head, bool acc) {
 #pragma unroll
-      for (int kk = half * (BN / 32); kk < (half + 1) * (BN / 32); ++kk)
+      for (int kk = head ? 0 : HEAD / 16; kk < (head ? HEAD : BN) / 16; ++kk)
         tc::mma_bf16_ts(tmem + C::O_COL + i * D, tmem + i * BN + kk * 8,
                         desc_sw128(ring + r * C::TILE + kk * 2048, C::BOX), ID_O, (acc || kk > 0) ? 1u : 0u);
     };
@@ -305,14 +303,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
         ok = wait(full + vt % R, (uint32_t)((vt / R) & 1), &s_abort);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          ok = ok && wait(p_half + i, (uint32_t)(j & 1), &s_abort);
+          ok = ok && wait(p_head + i, (uint32_t)(j & 1), &s_abort);
           if (!ok) break;
           tc::fence_after();
-          issue_o(i, vt % R, 0, j > 0);
+          issue_o(i, vt % R, true, j > 0);
           ok = wait(p_full + i, (uint32_t)(j & 1), &s_abort);
           if (!ok) break;
           tc::fence_after();
-          issue_o(i, vt % R, 1, true);
+          issue_o(i, vt % R, false, true);
           tc::commit(o_full + i);
           if (j + 1 == n) continue;
           if (i == 0) ok = wait(full + kt % R, (uint32_t)((kt / R) & 1), &s_abort);
@@ -384,38 +382,35 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
         for (int c = 0; c < BN; ++c) s[c] = c < lim ? s[c] : 0xff800000u;
       }
       auto at = [&](int c) { return __uint_as_float(s[c]); };
-      float mx4[4];
+      float m8[8];  // eight chains: their latency would show with four
 #pragma unroll
-      for (int q = 0; q < 4; ++q) mx4[q] = max3(at(q), at(q + 4), at(q + 8));
+      for (int x = 0; x < 8; ++x) m8[x] = max3(at(x), at(x + 8), at(x + 16));
 #pragma unroll
-      for (int c = 12; c + 8 <= BN; c += 8)
+      for (int c = 24; c + 16 <= BN; c += 16)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mx4[q] = max3(mx4[q], at(c + q), at(c + q + 4));
-      float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], at(BN - 4));
-      mx = max3(max3(mx, at(BN - 3), at(BN - 2)), at(BN - 1), mx);
-      // raised lazily; the first maximum costs no rescaling (O has not been written: P V of the
-      // first block overwrites it, and rows that saw nothing so far hold zeros).  A NaN score makes
-      // the maximum, and with it the row's sum and output, NaN.
-      float corr = 1.f;
-      bool rescale = false;
-      if (!(mx <= m_run)) {
-        if (m_run == -INFINITY) {
-          m_run = mx;
-        } else if (!((mx - m_run) * sl2 <= RESCALE_LOG2)) {
-          corr = ex2((m_run - mx) * sl2);
-          l_run *= corr;
-          m_run = mx;
-          rescale = true;
-        }
-      }
-      if (j > 0 && __any_sync(0xffffffffu, rescale)) {  // P V_{j-1} has completed: S_j was issued after it
+        for (int x = 0; x < 8; ++x) m8[x] = max3(m8[x], at(c + x), at(c + x + 8));
 #pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 16) {
-          uint32_t r[16];
-          tc::ld16(t_o + c0, r);
+      for (int x = 0; x < 4; ++x) m8[x] = max3(m8[x], at(BN - 8 + x), at(BN - 4 + x));
+      const float mx = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), max3(m8[6], m8[7], m8[7]));
+      // Raised lazily: where it grew by more than the margin.  The first maximum costs no rescaling (O has
+      // not been written: P V of the first block overwrites it, and rows that saw nothing so far hold
+      // zeros).  A NaN score makes the maximum, and with it the row's sum and output, NaN.  The rescaling
+      // stays a rolled loop: it is rare, and unrolled it cost the loop its registers (534 -> 496 us).
+      const bool rescale = (mx - m_run) * sl2 > RESCALE_LOG2 || mx != mx;
+      const float m_old = m_run;
+      if (rescale) m_run = mx;
+      if (__any_sync(0xffffffffu, rescale)) {
+        const float corr = rescale && m_old != -INFINITY ? ex2((m_old - mx) * sl2) : 1.f;
+        l_run *= corr;
+        if (j > 0) {  // P V_{j-1} has completed: S_j was issued after it
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            uint32_t r[16];
+            tc::ld16(t_o + c0, r);
 #pragma unroll
-          for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * corr);
-          tc::st16(t_o + c0, r);
+            for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * corr);
+            tc::st16(t_o + c0, r);
+          }
         }
       }
       const int seen = block_seen(blk);
@@ -435,24 +430,25 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       const f2 sl2x2 = pack2(sl2, sl2), msx2 = pack2(-ms, -ms);
       f2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        constexpr int W = BN / 4;  // 32-bit words of two weights each
-        uint32_t w[W];
+      for (int c0 = 0; c0 < BN / 2; c0 += 16) {
+        uint32_t w[16];  // two weights each
 #pragma unroll
-        for (int c = 0; c < W; ++c) {
-          const int k = half * 2 * W + 2 * c;
-          const f2 x = fma2(pack2(at(k), at(k + 1)), sl2x2, msx2);
+        for (int c = 0; c < 16; ++c) {
+          const f2 x = fma2(pack2(at(2 * (c0 + c)), at(2 * (c0 + c) + 1)), sl2x2, msx2);
           float p0, p1;
           unpack2(x, p0, p1);
           p0 = ex2(p0);
           p1 = ex2(p1);
           sum[c & 1] = add2(sum[c & 1], pack2(p0, p1));
-          w[c] = pack_near(p0, p1);
+          w[c] = pack_bf16(p0, p1);
         }
-        tc::st32(t_s + half * W, w);
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(half == 0 ? p_half + i : p_full + i);
+        tc::st16_async(t_s + c0, w);
+        if (2 * c0 + 32 == HEAD || 2 * c0 + 32 == BN) {
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(2 * c0 + 32 == HEAD ? p_head + i : p_full + i);
+        }
       }
       float sums[4];
       unpack2(sum[0], sums[0], sums[1]);
