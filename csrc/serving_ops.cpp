@@ -478,37 +478,46 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   }
   if (few) {
     // Both parts at once where that is shorter.  The lengths are not known here: half of the capacity.
-    // Times as measured (us): a prefix CTA 8 + 2 per block of 128 keys (D = 64: 1.6; two CTAs of one tile on an
-    // SM 2.9 and 2), own keys 6 + 1 per 6 MB.
+    // Times in us as measured, for head dim 128 (64).
     int own_ctas = INT32_MAX;
     if (a.P > 0) {
       int tiles, slots;
       pra_prefix_attention_shape(a, &tiles, &slots);
       const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-      const double own_kb = 2e-3 * B * a.cap * width, alone = head_dim == 128 ? 2.0 : 1.6;
-      const auto prefix_us = [&](int splits, double per_block) { return 8 + per_block * ceil_div(prefix_blocks, splits); };
+      const bool wide = head_dim == 128;
+      const double own_kb = 2e-3 * B * a.cap * width;
       if (slots == sms) {
-        // Two tiles a CTA: the prefix part is bound by its products and the own part by HBM, each takes its SMs
-        // (an own SM reads 75 KB/us).  64 rows behind 8K with 64 to 1,024 own keys 68 -> 45 us, 128 rows behind
-        // 32K 140 -> 117 us.
-        double best = prefix_us(a.splits, alone) + 4 + own_kb / 6000;
-        int own_sms = 0;
-        for (int s = 4; s <= sms * 3 / 4 && (sms - s) / tiles >= 1; s += 4) {
-          const double us = std::max(prefix_us(std::min((sms - s) / tiles, prefix_blocks), alone), 6 + own_kb / (75.0 * s));
+        // Two tiles a CTA: the prefix part is bound by its products and the own part by HBM, each takes its SMs.
+        // A prefix CTA takes 13 (4) + 1.85 (1.6) per block; an SM of own CTAs 0.34 (0.26) per block of 64 keys, two
+        // more of them per item, up to HBM's rate, behind which more SMs help little.  64 rows behind 8K with
+        // 64 to 1,024 own keys 68 -> 46 us, 128 rows behind 32K 140 -> 107 us.
+        const auto prefix_us = [&](int splits) { return (wide ? 13 : 4) + (wide ? 1.85 : 1.6) * ceil_div(prefix_blocks, splits); };
+        const double block_kb = 0.256 * head_dim, blocks = (double)B * kv_heads * (a.cap / 128.0 + 2.5);
+        const auto own_us = [&](int s) {
+          const double rate = s * block_kb / (wide ? 0.34 : 0.26);
+          return 6 + blocks * block_kb / (rate < 5800 ? rate : 5800 + 0.25 * (rate - 5800));
+        };
+        double best = prefix_us(a.splits) + 4 + own_kb / 6000;
+        int splits = 0;
+        for (int s = std::min(prefix_blocks, (sms - 4) / tiles); s >= 1 && sms - s * tiles <= sms * 3 / 4; --s) {
+          const double us = std::max(prefix_us(s), own_us(sms - s * tiles));
           if (us < best) {
             best = us;
-            own_sms = s;
+            splits = s;
           }
         }
-        if (own_sms > 0) {
-          a.splits = std::min(prefix_blocks, (sms - own_sms) / tiles);
-          own_ctas = 2 * (sms - a.splits * tiles);
+        if (splits > 0) {
+          a.splits = splits;
+          own_ctas = 2 * (sms - splits * tiles);
         }
       } else if (tiles <= sms) {
         // One tile a CTA: a CTA of each part fits on an SM.
+        // A prefix CTA takes 8 + 2 (1.6) per block, two of them on an SM 2.9 (2).
         const int splits = std::min(prefix_blocks, sms / tiles);
-        const double both = std::max(prefix_us(splits, alone), 6 + own_kb / 6000);
-        const double after = prefix_us(a.splits, a.splits > splits ? (head_dim == 128 ? 2.9 : 2.0) : alone) + 4 + own_kb / 6000;
+        const auto prefix_us = [&](int s, double per_block) { return 8 + per_block * ceil_div(prefix_blocks, s); };
+        const double both = std::max(prefix_us(splits, wide ? 2.0 : 1.6), 6 + own_kb / 6000);
+        const double after =
+            prefix_us(a.splits, a.splits > splits ? (wide ? 2.9 : 2.0) : (wide ? 2.0 : 1.6)) + 4 + own_kb / 6000;
         if (both < after) {
           a.splits = splits;
           own_ctas = sms;
