@@ -16,12 +16,13 @@
 // so each CTA turns its slice of it around in shared memory: a bit per token that the history or a
 // bias names (their ranks by a prefix sum of the bits), and for each such token its id and a word with
 // its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 bias entry + 1).  Integer atomics fill
-// them, so any order gives the same table.  The pass over all logits then only masks and takes
-// maxima, on packed 16-bit pairs, leaving out what is named; the named tokens follow, four logits on
-// their way per thread.  Where the history may name half of a slice, a word per token takes no more
+// them, so any order gives the same table.  The pass over all logits then takes maxima on packed 16-bit
+// pairs and masks and leaves out what is named only where a vector may hold a new largest; the named
+// tokens follow, four logits on their way per thread (half of the warps at them while the others are at
+// all logits: no shorter).  Where the history may name half of a slice, a word per token takes no more
 // room and the history is walked once instead of twice (64 rows of 128,256 logits with 100,000 ids
-// each: 368 -> 138 us).  256 rows of 152,064 bf16 logits with 8,192 ids each take 54 us with cold caches
-// (28 without a history, 12.6 is what their bytes need): the two walks and the scattered logits of the
+// each: 368 -> 136 us).  256 rows of 152,064 bf16 logits with 8,192 ids each take 42 us (17 without a
+// history, 12.6 is what their bytes need): the two walks and the scattered logits of the
 // named tokens wait for memory, one after the other.  (Looking the penalties up within the pass over all
 // logits took 107 us, a word per token of the slice instead of the table 183 us.)  A thread only
 // remembers which vector held its maximum: the element is looked up at the end, by the warps' winners.
@@ -55,6 +56,12 @@ __device__ __forceinline__ unsigned long long choice_key(float z, uint32_t id) {
   const uint32_t u = __float_as_uint(__fadd_rn(z, 0.f));
   const uint32_t k = z != z ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return ((unsigned long long)k << 32) | (0xFFFFFFFFu - id);
+}
+
+// The value of a key's upper half.
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xFFFFFFFFu) return __int_as_float(0x7fffffff);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
 template <typename T, int V>
@@ -123,10 +130,11 @@ __device__ __forceinline__ float max_vec(const Vec<T, V>& x) {
 // 32-bit words of a slice's bits.
 __host__ __device__ constexpr int bit_words(int slice) { return (slice + 31) / 32; }
 
-// T: type of the logits; V: elements of one access; TABLE: a history or biases are given.
-template <typename T, int V, bool TABLE>
+// T: type of the logits; V: elements of one access; TABLE: a history or biases are given; CHOOSE: the
+// greedy token is wanted, else the processed logits.
+template <typename T, int V, bool TABLE, bool CHOOSE>
 __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int slice, int table_words, bool direct) {
-    constexpr int U = 3;  // accesses of a batch
+  constexpr int U = 3;  // accesses of a batch
   extern __shared__ uint32_t smem[];
   __shared__ uint32_t s_scan[NT / 32];
   __shared__ unsigned long long s_best[NT / 32];
@@ -137,7 +145,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
   const int b = blockIdx.y;
   const int v0 = part * slice, n = max(min(a.V, v0 + slice) - v0, 0);
   const T* x = reinterpret_cast<const T*>(a.logits) + (int64_t)b * a.in_stride + v0;
-  T* y = a.out ? reinterpret_cast<T*>(a.out) + (int64_t)b * a.out_stride + v0 : nullptr;
+  T* y = CHOOSE ? nullptr : reinterpret_cast<T*>(a.out) + (int64_t)b * a.out_stride + v0;
   // the row's mask as bytes: element e of the slice is bit (vocab_start + v0 + e) % 8 of its byte
   const uint8_t* mask = nullptr;
   bool none = false;  // a mask row outside the masks allows nothing
@@ -266,42 +274,47 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
       __syncthreads();
     }
   }
-  const bool choose = a.token != nullptr;
-  float best = -INFINITY;  // largest so far, and the first vector that has it
-  int best_i = 0;
   // The bits of the vector's elements that this pass chooses among: allowed, and not named.
   auto choosable = [&](uint32_t bits, int e) {
     if constexpr (TABLE) bits &= ~(named[e >> 5] >> (e & 31));
     return bits;
   };
-  auto apply = [&](Batch& q, int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * NT;
-      if (i >= vecs) continue;
-      if (choose) {
-        if (TABLE || mask || none) mask_vec(q.x[u], choosable(q.allowed[u], i * V));
-        const float m = max_vec(q.x[u]);
-        if (!(m <= best) && best == best) {
-          best = m;
-          best_i = i;
-        }
-      }
-      if (y) {
-        if (mask || none) mask_vec(q.x[u], q.allowed[u]);
-        *reinterpret_cast<Vec<T, V>*>(y + i * V) = q.x[u];
-      }
-    }
-  };
-  for (int i0 = tid; i0 < vecs; i0 += 2 * U * NT) {
-    load(next, i0 + U * NT);
-    apply(here, i0);
-    load(here, i0 + 2 * U * NT);
-    apply(next, i0 + U * NT);
-  }
-  // the warp's largest value; the lanes that have it look for their element
   unsigned long long key = 0;
-  if (choose) {
+  if constexpr (CHOOSE) {
+    // Most vectors hold nothing above the largest that the warp has found: they are only compared, masks
+    // and names are looked up for the others.  A warp's tokens come in rising order, so an equal one later
+    // never wins.
+    float best = -INFINITY, bar = -INFINITY;  // this thread's largest (vector best_i), the warp's
+    int best_i = 0;
+    auto look = [&](Batch& q, int i0) {
+      float m[U];
+      bool above = false;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        m[u] = max_vec(q.x[u]);
+        above = above || (i0 + u * NT < vecs && !(m[u] <= bar));
+      }
+      if (!__any_sync(0xffffffffu, above && bar == bar)) return;  // NaN: nothing is larger
+      float least = bar;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * NT;
+        if (i >= vecs || m[u] <= least || least != least) continue;
+        mask_vec(q.x[u], choosable(q.allowed[u], i * V));
+        const float k = max_vec(q.x[u]);
+        if (k <= least) continue;
+        best = least = k;
+        best_i = i;
+      }
+      bar = key_value(__reduce_max_sync(0xffffffffu, (uint32_t)(choice_key(best, 0) >> 32)));
+    };
+    for (int i0 = tid; i0 - lane < vecs; i0 += 2 * U * NT) {
+      load(next, i0 + U * NT);
+      look(here, i0);
+      load(here, i0 + 2 * U * NT);
+      look(next, i0 + U * NT);
+    }
+    // the lanes that have the warp's largest value look for their element
     const uint32_t mine = (uint32_t)(choice_key(best, 0) >> 32);
     if (mine == __reduce_max_sync(0xffffffffu, mine) && best_i < vecs) {
       Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(x + best_i * V);
@@ -314,20 +327,36 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
         key = k > key ? k : key;
       }
     }
+  } else {
+    auto apply = [&](Batch& q, int i0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * NT;
+        if (i >= vecs) continue;
+        if (mask || none) mask_vec(q.x[u], q.allowed[u]);
+        *reinterpret_cast<Vec<T, V>*>(y + i * V) = q.x[u];
+      }
+    };
+    for (int i0 = tid; i0 < vecs; i0 += 2 * U * NT) {
+      load(next, i0 + U * NT);
+      apply(here, i0);
+      load(here, i0 + 2 * U * NT);
+      apply(next, i0 + U * NT);
+    }
   }
   auto is_allowed = [&](int e) { return !none && (!mask || (mask[e / 8] >> (e & 7) & 1)); };
   for (int e = vecs * V + tid; e < n; e += NT) {  // fewer than V elements at the end of the last slice
     if (TABLE && ((named[e >> 5] >> (e & 31)) & 1u)) continue;
     const float z = is_allowed(e) ? widen(x[e]) : -INFINITY;
-    if (choose) {
+    if constexpr (CHOOSE) {
       const unsigned long long k = choice_key(z, (uint32_t)(a.vocab_start + v0 + e));
       key = k > key ? k : key;
     }
-    if (y) narrow(z, y[e]);
+    if constexpr (!CHOOSE) narrow(z, y[e]);
   }
   if constexpr (TABLE) {
     // the named tokens, after their vectors have been written (in place, an allowed one is still as it came)
-    if (y) __syncthreads();
+    if constexpr (!CHOOSE) __syncthreads();
     for (int i0 = tid; i0 < named_tokens; i0 += 4 * NT) {
       float z4[4];  // four scattered logits and mask bytes on their way
       int e4[4];
@@ -353,15 +382,15 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
         if (times) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)times)), pres);
         if (w >> 21) z = __fadd_rn(z, bias_sum[(w >> 21) - 1]);
         if (!((bits4[u] >> (e & 7)) & 1u)) z = -INFINITY;
-        if (choose) {
+        if constexpr (CHOOSE) {
           const unsigned long long k = choice_key(z, (uint32_t)(a.vocab_start + v0 + e));
           key = k > key ? k : key;
         }
-        if (y) narrow(z, y[e]);
+        if constexpr (!CHOOSE) narrow(z, y[e]);
       }
     }
   }
-  if (choose) {
+  if constexpr (CHOOSE) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
@@ -387,8 +416,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
         other = k > other ? k : other;
       }
       if (lane == 0) {
-        const uint32_t k = (uint32_t)(other >> 32);
-        const float z = k == 0xFFFFFFFFu ? __int_as_float(0x7fffffff) : __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+        const float z = key_value((uint32_t)(other >> 32));
         const int64_t id = 0xFFFFFFFFu - (uint32_t)other;
         const bool any = z != -INFINITY;
         a.token[b] = any ? id : -1;
@@ -403,7 +431,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
   }
 }
 
-template <typename T, int V, bool TABLE>
+template <typename T, int V, bool TABLE, bool CHOOSE>
 cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
   // One wave of two CTAs per SM: rows in 8 slices while few, whole rows (every id then read once, no
   // exchange) when many; more slices again where the table would leave one CTA per SM.
@@ -424,7 +452,7 @@ cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
   shape(8);
   while (cl > 1 && (int64_t)a.B * cl > 2 * sms) shape(cl / 2);
   while (cl < 8 && bytes > 110 * 1024) shape(cl * 2);
-  auto kernel = rules_kernel<T, V, TABLE>;
+  auto kernel = rules_kernel<T, V, TABLE, CHOOSE>;
   if (bytes > 48 * 1024) PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), (int)bytes));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cl, a.B);
@@ -447,8 +475,12 @@ cudaError_t dispatch(const LogitsArgs& a, cudaStream_t st) {
   bool wide = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.in_stride % W == 0;
   if (a.out) wide = wide && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride % W == 0;
   const bool table = a.ids != nullptr || a.bias_ids != nullptr;
-  if (wide) return table ? launch<T, W, true>(a, st) : launch<T, W, false>(a, st);
-  return table ? launch<T, 1, true>(a, st) : launch<T, 1, false>(a, st);
+  const auto choose = [&](auto vec, auto tab) {
+    return a.token != nullptr ? launch<T, vec, tab, true>(a, st) : launch<T, vec, tab, false>(a, st);
+  };
+  using std::integral_constant;
+  if (wide) return table ? choose(integral_constant<int, W>(), std::true_type()) : choose(integral_constant<int, W>(), std::false_type());
+  return table ? choose(integral_constant<int, 1>(), std::true_type()) : choose(integral_constant<int, 1>(), std::false_type());
 }
 
 }  // namespace rules
