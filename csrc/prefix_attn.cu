@@ -150,13 +150,25 @@ struct Item {
   int lo, hi;             // blocks of this split
 };
 
+// The query tile of this CTA and its share of the keys: all of them for the first `whole` tiles, else part
+// `split` of `splits`.
+struct Share {
+  int tile, split, splits;
+};
+__device__ __forceinline__ Share share_of(const PrefixAttnArgs& a) {
+  if (a.whole == 0) return {(int)blockIdx.x, (int)blockIdx.y, a.splits};
+  if ((int)blockIdx.x < a.whole) return {(int)blockIdx.x, 0, 1};
+  const int behind = ((int)gridDim.x - a.whole) / a.splits, c = (int)blockIdx.x - a.whole;
+  return {a.whole + c % behind, c / behind, a.splits};
+}
+
 template <int NT>
-__device__ __forceinline__ Item item_of(const PrefixAttnArgs& a, int seen) {
+__device__ __forceinline__ Item item_of(const PrefixAttnArgs& a, const Share& share, int seen) {
   Item it;
   const int G = a.H / a.Hkv;
   it.rows = (a.packed ? a.B : 1) * a.T * G;
   const int tiles = (it.rows + NT * BM - 1) / (NT * BM);
-  int x = blockIdx.x;
+  int x = share.tile;
   it.row0 = (x % tiles) * NT * BM;
   x /= tiles;
   it.kvh = x % a.Hkv;
@@ -170,8 +182,8 @@ __device__ __forceinline__ Item item_of(const PrefixAttnArgs& a, int seen) {
   }
   it.prefix_blocks = (it.prefix_seen + BN - 1) / BN;
   const int n = it.prefix_blocks + (it.own_seen + BN - 1) / BN;
-  it.lo = (int)((int64_t)n * blockIdx.y / a.splits);
-  it.hi = (int)((int64_t)n * (blockIdx.y + 1) / a.splits);
+  it.lo = (int)((int64_t)n * share.split / share.splits);
+  it.hi = (int)((int64_t)n * (share.split + 1) / share.splits);
   return it;
 }
 
@@ -197,6 +209,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   __shared__ int s_seen;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Share share = share_of(a);
   pdl_launch_dependents();  // the own part, as this grid's CTAs make room, or the merge
   const int G = a.H / a.Hkv;
   constexpr int ISSUER = C::SOFTMAX / 32, PRODUCER = ISSUER + 1;  // warps
@@ -226,7 +239,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   {
     const int rows = (a.packed ? a.B : 1) * a.T * G;
     const int tiles = (rows + NT * BM - 1) / (NT * BM);
-    const int row0 = (blockIdx.x % tiles) * NT * BM, b1 = blockIdx.x / (tiles * a.Hkv);
+    const int row0 = (share.tile % tiles) * NT * BM, b1 = share.tile / (tiles * a.Hkv);
     int seen = 0;
     if (!a.use_prefix) seen = 0;
     else if (a.prefix_len == nullptr) seen = a.P;
@@ -240,7 +253,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const Item it = item_of<NT>(a, s_seen);
+  const Item it = item_of<NT>(a, share, s_seen);
   const uint32_t tmem = s_tmem;
   const uint32_t ring = smem_u32(smem + C::OFF_RING);
   const int n = it.hi - it.lo;
@@ -462,8 +475,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       tc::fence_after();
       const bool any = m_run != -INFINITY;  // else nothing of this range is visible to the row
       const int64_t bt = (int64_t)b * a.T + t;
-      const int64_t slot = (bt * a.H + h) * a.n_slots + a.slot0 + blockIdx.y;
-      const bool partial = a.part_o != nullptr;
+      const int64_t place = a.whole > 0 ? (int64_t)(share.tile - a.whole) * (NT * BM) + i * BM + row : bt * a.H + h;
+      const int64_t slot = place * a.n_slots + a.slot0 + share.split;
+      const bool partial = a.part_o != nullptr && share.tile >= a.whole;
       if (live) {
         if (partial) {
           *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(any ? m_run * a.scale : -INFINITY, l_run);
@@ -948,10 +962,26 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const PrefixMer
   };
   const int64_t at = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  const int64_t bt = at / a.H;
-  const int h = (int)(at - bt * a.H), b = (int)(bt / a.T), t = (int)(bt - (int64_t)b * a.T);
+  int b, t, h;
+  bool ok;
+  if (a.tiles > 0) {  // row `at` of the split tiles
+    const int G = a.H / a.Hkv, rows_all = (a.packed ? a.B : 1) * a.T * G, per = (rows_all + a.tile_rows - 1) / a.tile_rows;
+    const int64_t behind = at / a.tile_rows;
+    const int tile = a.tile0 + (int)behind, x = tile / per;  // x: KV head, or (batch row, KV head)
+    const int64_t qr = (int64_t)(tile - x * per) * a.tile_rows + (at - behind * a.tile_rows);
+    ok = behind < a.tiles && qr < rows_all;
+    const int bt = (int)(qr / G);
+    b = a.packed ? bt / a.T : x / a.Hkv;
+    t = bt % a.T;
+    h = (a.packed ? x : x % a.Hkv) * G + (int)(qr - (int64_t)bt * G);
+  } else {
+    const int64_t bt = at / a.H;
+    h = (int)(at - bt * a.H), b = (int)(bt / a.T), t = (int)(bt - (int64_t)b * a.T);
+    ok = at < (int64_t)a.B * a.T * a.H;
+  }
   pdl_wait();
-  if (at >= (int64_t)a.B * a.T * a.H) return;
+  if (!ok) return;
+  const int64_t query = ((int64_t)b * a.T + t) * a.H + h;  // parts: `at`
   // parts [0, n0) are the first set's, [n0, n1) the second's, [n1, n) the pieces
   const int n0 = a.part_o != nullptr ? a.n_slots : 0, n1 = n0 + (a.more_o != nullptr ? a.n_more : 0);
   int n = n1;
@@ -1031,15 +1061,15 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const PrefixMer
     uint32_t w[E / 2];
 #pragma unroll
     for (int e = 0; e < E; e += 2) w[e / 2] = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + at * D + lane * E);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + query * D + lane * E);
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) dst[e] = w[e];
   }
   if (a.lse != nullptr && lane == 0) a.lse[((int64_t)b * a.H + h) * a.T + t] = any ? M + logf(L) : -INFINITY;
   if (a.joined_o != nullptr) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) a.joined_o[at * D + lane * E + e] = acc[e];
-    if (lane == 0) *reinterpret_cast<float2*>(a.joined_ml + 2 * at) = make_float2(M, L);
+    for (int e = 0; e < E; ++e) a.joined_o[query * D + lane * E + e] = acc[e];
+    if (lane == 0) *reinterpret_cast<float2*>(a.joined_ml + 2 * query) = make_float2(M, L);
   }
 }
 
@@ -1087,8 +1117,9 @@ cudaError_t launch(const PrefixAttnArgs& a, cudaStream_t st) {
   PRA_RETURN_IF_ERROR(prepare(reinterpret_cast<const void*>(prefix_kernel<D, NT>), C::SMEM));
   const int tiles = (rows_of(a) + NT * BM - 1) / (NT * BM);
   const int64_t items = (int64_t)tiles * a.Hkv * (a.packed ? 1 : a.B);
-  if (items > INT32_MAX || a.splits > 65535) return cudaErrorInvalidValue;
-  prefix_kernel<D, NT><<<dim3((unsigned)items, a.splits), C::THREADS, C::SMEM, st>>>(pk, pv, k, v, a);
+  const int64_t ctas = a.whole > 0 ? a.whole + (items - a.whole) * a.splits : items;
+  if (ctas > INT32_MAX || a.splits > 65535 || a.whole < 0 || a.whole > items) return cudaErrorInvalidValue;
+  prefix_kernel<D, NT><<<dim3((unsigned)ctas, a.whole > 0 ? 1 : a.splits), C::THREADS, C::SMEM, st>>>(pk, pv, k, v, a);
   return cudaGetLastError();
 }
 
@@ -1098,9 +1129,10 @@ int tiles_per_cta(const PrefixAttnArgs& a) { return rows_of(a) > BM ? 2 : 1; }
 }  // namespace prefix
 }  // namespace pra
 
-void pra_prefix_attention_shape(const PrefixAttnArgs& a, int* tiles, int* slots) {
+void pra_prefix_attention_shape(const PrefixAttnArgs& a, int* tiles, int* slots, int* tile_rows) {
   using namespace pra::prefix;
   const int nt = tiles_per_cta(a);
+  if (tile_rows != nullptr) *tile_rows = nt * BM;
   *tiles = (rows_of(a) + nt * BM - 1) / (nt * BM) * a.Hkv * (a.packed ? 1 : a.B);
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -1160,7 +1192,7 @@ cudaError_t pra_own_attention(const OwnAttnArgs& a, cudaStream_t st) {
 
 cudaError_t pra_prefix_merge(const PrefixMergeArgs& a, cudaStream_t st) {
   using namespace pra::prefix;
-  const int64_t rows = (int64_t)a.B * a.T * a.H;
+  const int64_t rows = a.tiles > 0 ? (int64_t)a.tiles * a.tile_rows : (int64_t)a.B * a.T * a.H;
   if (rows == 0) return cudaSuccess;
   const int64_t blocks = (rows + MERGE_WARPS - 1) / MERGE_WARPS;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;

@@ -85,16 +85,18 @@ struct PrefixAttnArgs {
   float scale;
   int packed, use_prefix, use_own;
   int splits;                     // CTAs along the keys of one query tile
+  int whole;                      // > 0: that many tiles take all their keys, to out; the tiles behind are split
   int slot0, n_slots;             // partial s of this launch goes to slot slot0 + s of n_slots
-  float* part_o;                  // [B * T, H, n_slots, D] unnormalised, or null: write out / lse
+  float* part_o;                  // [B * T, H, n_slots, D] unnormalised, or null: write out / lse (with `whole`
+                                  // [tiles behind it * tile rows, n_slots, D])
   float* part_ml;                 // [B * T, H, n_slots, 2] (maximum in natural-log units, sum)
   __nv_bfloat16* out;             // [B, T, H * D] contiguous
   float* lse;                     // [B, H, T] or null
   int* status;                    // set to 1 by a CTA that gave up on a bounded wait
 };
 cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t stream);
-// CTAs of a launch before splitting, and how many run at once (for choosing splits).
-void pra_prefix_attention_shape(const PrefixAttnArgs& a, int* tiles, int* slots);
+// Query tiles of a launch (CTAs before splitting), how many run at once (for choosing splits), rows of a tile.
+void pra_prefix_attention_shape(const PrefixAttnArgs& a, int* tiles, int* slots, int* tile_rows = nullptr);
 
 // The own keys of rows with few queries (T * H / Hkv <= PRA_OWN_ROWS per KV head), which a 128-row tile would
 // leave mostly empty: every (batch row, KV head) is an item of ceil(len / 64) blocks (at least one), the
@@ -125,6 +127,8 @@ cudaError_t pra_own_attention(const OwnAttnArgs& a, cudaStream_t stream);
 // out / lse, or the joined partial, from the partials of every (b, t, h).
 struct PrefixMergeArgs {
   int B, T, H, Hkv, D;
+  int tile0, tiles, tile_rows;    // tiles > 0: only the queries of tiles tile0 .. tile0 + tiles - 1 of the attention launch,
+  int packed;                     // whose parts are [tiles * tile_rows, n_slots, D]; its `packed`
   const float* part_o;            // [B * T, H, n_slots, D] and (max, sum) pairs, or null
   const float* part_ml;
   int n_slots;

@@ -384,10 +384,11 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   a.scale = (float)scale;
   a.status = pra_attention_status_word(q.device());
   const auto fo = q.options().dtype(at::kFloat);
-  // One allocation for the call's parts: n slots of sums and (max, sum) pairs per query, and `more` floats.
+  // One allocation for the call's parts: n slots of sums and (max, sum) pairs for each of the queries, and `more`
+  // floats.
   Tensor work;
-  const auto workspace = [&](int64_t n, int64_t more) {
-    const int64_t queries = B * T * heads, own = (queries * n * (head_dim + 2) + 3) / 4 * 4;  // what follows: 16-byte aligned
+  const auto workspace = [&](int64_t n, int64_t more, int64_t queries) {
+    const int64_t own = (queries * n * (head_dim + 2) + 3) / 4 * 4;  // what follows: 16-byte aligned
     work = torch::empty({own + more}, fo);
     a.n_slots = (int)n;
     a.part_o = n > 0 ? work.data_ptr<float>() : nullptr;
@@ -458,10 +459,38 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     a.packed = a.cap == 0;
     a.use_prefix = a.P > 0;
     a.use_own = a.cap > 0;
-    a.splits = splits_for(a, prefix_blocks + own_blocks);
+    const int blocks = prefix_blocks + own_blocks;
+    a.splits = splits_for(a, blocks);
     std::vector<OptTensor> r = result;
+    int tiles, slots, tile_rows;
+    pra_prefix_attention_shape(a, &tiles, &slots, &tile_rows);
+    if (a.splits == 1 && tiles % slots != 0 && prefix_blocks >= own_blocks && !partials) {
+      // The tiles behind the last full wave are split among all SMs (where their keys are mostly the prefix, alike
+      // for all: causal tiles of all lengths fill the last wave anyway, 4,096 queries without a prefix took 3%
+      // longer).  In blocks of 128 keys: a CTA takes 5 more than its keys, the join 2 and what it writes and reads.
+      // 3, 4 and 5 x 512 queries behind 16K (192, 256 and 320 tiles on 148 SMs) 544 -> 405, 485 -> 480 and
+      // 731 -> 656 us.
+      const int behind = tiles % slots;
+      double best = blocks + 5;
+      for (int s = 2; s <= std::min(16, blocks); ++s) {
+        const double cost = ceil_div((int64_t)behind * s, slots) * (ceil_div(blocks, s) + 5.0) + 2 +
+                            behind * s * (tile_rows * head_dim / 32768.0) * 0.014;
+        if (cost < best) {
+          best = cost;
+          a.splits = s;
+        }
+      }
+      a.whole = a.splits > 1 ? tiles - behind : 0;
+      if (a.whole > 0) {
+        m.tile0 = a.whole;
+        m.tiles = behind;
+        m.tile_rows = tile_rows;
+        m.packed = a.packed;
+      }
+    }
     if (a.splits > 1) {
-      workspace(a.splits, 0);
+      if (a.whole > 0) workspace(a.splits, 0, (int64_t)m.tiles * tile_rows);
+      else workspace(a.splits, 0, B * T * heads);
     } else if (partials) {
       r = joined();
       a.part_o = joined_o.data_ptr<float>();
@@ -548,7 +577,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     o.ctas = std::min(o.ctas, own_ctas);
     // behind the slots: the pieces' sums, their (max, sum) pairs, the items' first and last CTAs
     const int64_t items = B * kv_heads, pieces = (items + o.ctas) * rows;
-    o.piece_o = workspace(a.P > 0 ? a.splits : 0, pieces * (head_dim + 2) + 2 * items);
+    o.piece_o = workspace(a.P > 0 ? a.splits : 0, pieces * (head_dim + 2) + 2 * items, B * T * heads);
     o.piece_ml = o.piece_o + pieces * head_dim;
     o.first = reinterpret_cast<int*>(o.piece_ml + pieces * 2);
     o.last = o.first + items;
@@ -562,7 +591,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   }
   own.use_own = 1;
   own.splits = splits_for(own, own_blocks);
-  workspace(a.splits + own.splits, 0);
+  workspace(a.splits + own.splits, 0, B * T * heads);
   own.part_o = a.part_o;
   own.part_ml = a.part_ml;
   own.n_slots = a.n_slots;

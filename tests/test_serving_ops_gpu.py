@@ -245,6 +245,8 @@ CASES = [
     (2, 300, 257, 300, 8, 2, 128), (1, 1, 5000, 10, 32, 8, 128), (1, 513, 900, 600, 4, 1, 64), (2, 40, 130, 64, 64, 2, 64),
     (3, 1, 0, 200, 8, 2, 128), (3, 4, 0, 200, 8, 2, 64), (3, 2, 300, 0, 8, 2, 128), (33, 1, 150, 40, 40, 2, 128),
     (3, 1, 200, 50, 3, 1, 128), (5, 3, 700, 9, 3, 3, 128), (1, 2, 65, 7, 5, 5, 128),  # odd counts of partials
+    # more tiles than fit in whole waves of CTAs, or less than one: those behind are split
+    (20, 300, 700, 300, 8, 8, 64), (4, 300, 7000, 300, 16, 8, 128), (300, 64, 500, 0, 4, 2, 64),
 ]
 
 
