@@ -538,11 +538,45 @@ def gemm_train_shapes(iters: int = 20) -> None:
     print(f"{'wgrad lm_head ' + f'{v}x{k}x{m}':44s} {ours:8.1f} {ref:9.1f} {fl / ours / 1e6:9.0f} {ref / ours:6.2f}")
 
 
+def serving_ops(iters: int = 3) -> None:
+    """The serving operators: rotary into the cache, attention behind a shared prefix (a decode batch, then
+    the prefill of suffixes), greedy tokens after the rules, processed logits."""
+    from .inference.logits import LogitsRules, TokenHistory, choose_tokens, process_logits
+    from .inference.shared_prefix import shared_prefix_attention
+    from .ops.rotary import rotary_cache, rotary_table
+
+    dev = torch.device("cuda", torch.cuda.current_device())
+    gen = torch.Generator(device=dev).manual_seed(0)
+    bf = lambda *s: torch.randn(*s, generator=gen, device=dev).bfloat16()  # noqa: E731
+    H, Hkv, D, M, V, B, L = 32, 8, 128, 16384, 152064, 256, 8192
+    table = rotary_table(D, 8192)
+    qkv, kc, vc = bf(M, (H + 2 * Hkv) * D), bf(M, Hkv * D), bf(M, Hkv * D)
+    slots = torch.arange(M, device=dev, dtype=torch.int32)
+    pk, pv = bf(16384, Hkv * D), bf(16384, Hkv * D)
+    q1, k1, v1 = bf(64, 1, H * D), bf(64, 1280, Hkv * D), bf(64, 1280, Hkv * D)
+    n1 = torch.randint(64, 1025, (64,), generator=gen, device=dev).int()
+    q2, k2, v2 = bf(4, 512, H * D), bf(4, 512, Hkv * D), bf(4, 512, Hkv * D)
+    n2 = torch.full((4,), 512, device=dev, dtype=torch.int32)
+    logits = bf(B, V)
+    history = TokenHistory((V * torch.rand(B, L, generator=gen, device=dev) ** 4).int(),
+                           torch.full((B,), L, device=dev, dtype=torch.int32))
+    rules = LogitsRules(repetition=torch.full((B,), 1.1, device=dev),
+                        mask=torch.randint(-2 ** 31, 2 ** 31, (B, (V + 31) // 32), generator=gen, device=dev).int())
+    for _ in range(iters):
+        rotary_cache(qkv, H, Hkv, D, slots % 8192, table, kc, vc, slots)
+        shared_prefix_attention(q1, pk[:8192], pv[:8192], k1, v1, n1, H, Hkv, D)
+        shared_prefix_attention(q2, pk, pv, k2, v2, n2, H, Hkv, D)
+        choose_tokens(logits, rules, history)
+        process_logits(logits, rules, history)
+    torch.cuda.synchronize()
+    print("ok")
+
+
 CASES = {"attention-fwd": attention_fwd, "decode-gemm-one": decode_gemm_one, "gemm-train-shapes": gemm_train_shapes,
          "decode-overlap-probe": decode_overlap_probe, "sweep-table": sweep_table, "train-small": train_small, "decode-small": decode_small, "train-table": train_table,
          "decode-table": decode_table, "decode-table-tp": decode_table_tp,
          "decode-attention-sweep": decode_attention_sweep, "route-topk-bench": route_topk_bench,
-         "decode-gemm-sweep": decode_gemm_sweep}
+         "decode-gemm-sweep": decode_gemm_sweep, "serving-ops": serving_ops}
 
 
 def main(argv=None) -> None:
