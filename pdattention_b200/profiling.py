@@ -8,6 +8,7 @@ profiler and then under ``ncu`` on one GPU with the same arguments::
     python -m pdattention_b200.profiling train-table       # torch.profiler kernel table of one step (8 rows)
     python -m pdattention_b200.profiling decode-table      # kernel table of one decode step (64 rows)
     python -m pdattention_b200.profiling attention-fwd     # forward attention kernels, tcgen05 vs mma.sync
+    python -m pdattention_b200.profiling serving-ops       # rotary, shared-prefix attention, rules on logits
     torchrun --nproc-per-node N -m pdattention_b200.profiling decode-table-tp   # TP decode step table
 
 The ``*-small`` cases keep device memory to a few GB so full ``ncu`` captures of one
