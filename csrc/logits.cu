@@ -15,8 +15,10 @@
 // 1 to 8 CTAs owns a row, one slice of the vocabulary each.  The history cannot be looked up per logit,
 // so each CTA turns its slice of it around in shared memory: a bit per token that the history or a
 // bias names (their ranks by a prefix sum of the bits), and for each such token its id and a word with
-// its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 bias entry + 1).  Integer atomics fill
-// them, so any order gives the same table.  The pass over all logits then takes maxima on packed 16-bit
+// its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 2,047 less the first bias entry, or
+// 0).  Integer atomics fill
+// them, so any order gives the same table; a token's first bias entry sums all of its entries (looking for earlier
+// entries from each one took 203 us for 2,047 biases, now 21).  The pass over all logits then takes maxima on packed 16-bit
 // pairs and masks and leaves out what is named only where a vector may hold a new largest; the named
 // tokens follow, four logits on their way per thread (half of the warps at them while the others are at
 // all logits: no shorter).  Where the history may name half of a slice, a word per token takes no more
@@ -192,7 +194,10 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
     const int words = bit_words(slice);
     for (int i = tid; i < words; i += NT) named[i] = 0;
     for (int i = tid; i < table_words; i += NT) table[i] = 0;
-    for (int i = tid; i < a.n_bias; i += NT) bias_id[i] = a.bias_ids[(int64_t)b * a.n_bias + i];
+    for (int i = tid; i < a.n_bias; i += NT) {
+      bias_id[i] = a.bias_ids[(int64_t)b * a.n_bias + i];
+      bias_sum[i] = 0.f;
+    }
     __syncthreads();
     auto name = [&](int id) {
       const uint32_t t = (uint32_t)id - base, bit = 1u << (t & 31);
@@ -242,6 +247,14 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
       __syncthreads();
     }
     auto place = [&](uint32_t t) { return direct ? t : entry_of(t); };
+    // the table words of biased tokens, before anything else is in them: the smallest entry wins
+    for (int i = tid; i < a.n_bias; i += NT) {
+      const uint32_t t = (uint32_t)bias_id[i] - base;
+      if (t >= (uint32_t)n) continue;
+      if (!direct) token[place(t)] = t;
+      atomicMax(table + place(t), (uint32_t)(PRA_RULES_MAX_BIASES - i) << 21);
+    }
+    if (a.n_bias > 0) __syncthreads();
     walk([&](int id, int i) {
       const uint32_t t = (uint32_t)id - base;
       if (t >= (uint32_t)n) return;
@@ -250,19 +263,35 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
       if (i >= prompt) atomicAdd(table + at, 1u);
       else if (!(table[at] & SEEN)) atomicOr(table + at, SEEN);
     });
-    // an entry whose id no earlier entry has owns the token and sums all its entries in list order
-    for (int i = tid; i < a.n_bias; i += NT) {
-      const uint32_t t = (uint32_t)bias_id[i] - base;
-      if (t >= (uint32_t)n) continue;
-      bool first = true;
-      for (int j = 0; j < i && first; ++j) first = bias_id[j] != bias_id[i];
-      if (!first) continue;
-      float sum = 0.f;
-      for (int j = i; j < a.n_bias; ++j)
-        if (bias_id[j] == bias_id[i]) sum += a.bias_values[(int64_t)b * a.n_bias + j];
-      bias_sum[i] = sum;
-      if (!direct) token[place(t)] = t;
-      atomicOr(table + place(t), (uint32_t)(i + 1) << 21);
+    // a token's first entry owns it and sums all its entries in list order
+    if (a.n_bias > 0) {
+      for (int i = tid; i < a.n_bias; i += NT) {
+        const uint32_t t = (uint32_t)bias_id[i] - base;
+        if (t >= (uint32_t)n) continue;
+        const int first = PRA_RULES_MAX_BIASES - (int)(table[place(t)] >> 21);
+        if (first != i) bias_sum[first] = 1.f;  // there are more of it
+      }
+      __syncthreads();
+      const float* values = a.bias_values + (int64_t)b * a.n_bias;
+      for (int i0 = warp * 32; i0 < a.n_bias; i0 += NT) {
+        const int i = i0 + lane;
+        const uint32_t t = i < a.n_bias ? (uint32_t)bias_id[i] - base : 0xFFFFFFFFu;
+        const bool owns = t < (uint32_t)n && PRA_RULES_MAX_BIASES - (int)(table[place(t)] >> 21) == i;
+        float sum = owns ? 0.f + values[i] : 0.f;
+        // the warp looks for the other entries of one token after the other
+        for (uint32_t more = __ballot_sync(0xffffffffu, owns && bias_sum[i] != 0.f); more; more &= more - 1) {
+          const int of = __ffs(more) - 1, id = bias_id[i0 + of];
+          for (int c = i0; c < a.n_bias; c += 32) {
+            const int j = c + lane;
+            uint32_t found = __ballot_sync(0xffffffffu, j > i0 + of && j < a.n_bias && bias_id[j] == id);
+            for (; found; found &= found - 1) {
+              const float v = values[c + __ffs(found) - 1];
+              if (lane == of) sum += v;
+            }
+          }
+        }
+        if (owns) bias_sum[i] = sum;
+      }
     }
     __syncthreads();
     if (direct) {
@@ -380,7 +409,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
         float z = z4[u];
         if (w & (SEEN | COUNT)) z = z > 0.f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
         if (times) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)times)), pres);
-        if (w >> 21) z = __fadd_rn(z, bias_sum[(w >> 21) - 1]);
+        if (w >> 21) z = __fadd_rn(z, bias_sum[PRA_RULES_MAX_BIASES - (w >> 21)]);
         if (!((bits4[u] >> (e & 7)) & 1u)) z = -INFINITY;
         if constexpr (CHOOSE) {
           const unsigned long long k = choice_key(z, (uint32_t)(a.vocab_start + v0 + e));
