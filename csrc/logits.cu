@@ -15,20 +15,20 @@
 // 1 to 8 CTAs owns a row, one slice of the vocabulary each.  The history cannot be looked up per logit,
 // so each CTA turns its slice of it around in shared memory: a bit per token that the history or a
 // bias names (their ranks by a prefix sum of the bits), and for each such token its id and a word with
-// its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 2,047 less the first bias entry, or
-// 0).  Integer atomics fill
-// them, so any order gives the same table; a token's first bias entry sums all of its entries (looking for earlier
-// entries from each one took 203 us for 2,047 biases, now 21).  The pass over all logits then takes maxima on packed 16-bit
-// pairs and masks and leaves out what is named only where a vector may hold a new largest; the named
-// tokens follow, four logits on their way per thread (half of the warps at them while the others are at
-// all logits: no shorter).  Where the history may name half of a slice, a word per token takes no more
-// room and the history is walked once instead of twice (64 rows of 128,256 logits with 100,000 ids
-// each: 368 -> 136 us).  256 rows of 152,064 bf16 logits with 8,192 ids each take 42 us (17 without a
-// history, 12.6 is what their bytes need): the two walks and the scattered logits of the
-// named tokens wait for memory, one after the other.  (Looking the penalties up within the pass over all
-// logits took 107 us, a word per token of the slice instead of the table 183 us.)  A thread only
-// remembers which vector held its maximum: the element is looked up at the end, by the warps' winners.
-// A thread's first logits and mask bytes are loaded before the table is built.
+// its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 2,047 less its first bias entry, or
+// 0).  Integer atomics fill them, so any order gives the same table; a token's first bias entry sums all
+// of its entries (looking for earlier ones from each entry took 203 us for 2,047 biases, now 21).
+//
+// The pass over all logits then takes maxima on packed 16-bit pairs, and masks and leaves out what is
+// named only where a vector may hold a new largest; the named tokens follow, four logits on their way per
+// thread (half of the warps at them while the others are at all logits: no shorter).  Where the history
+// may name half of a slice, a word per token takes no more room and the history is walked once instead
+// of twice (64 rows of 128,256 logits with 100,000 ids each: 368 -> 136 us).  256 rows of 152,064 bf16
+// logits with 8,192 ids each take 40 us (17 without a history, 12.6 is what their bytes need): the two
+// walks and the scattered logits of the named tokens wait for memory, one after the other.  (Looking the
+// penalties up within the pass over all logits took 107 us, a word per token of the slice instead of the
+// table 183 us.)  A thread only remembers which vector held its maximum: the element is looked up at the
+// end, by the warps' winners.  A thread's first logits and mask bytes are loaded before the table is built.
 #include <algorithm>
 #include <type_traits>
 
@@ -133,8 +133,9 @@ __device__ __forceinline__ float max_vec(const Vec<T, V>& x) {
 __host__ __device__ constexpr int bit_words(int slice) { return (slice + 31) / 32; }
 
 // T: type of the logits; V: elements of one access; TABLE: a history or biases are given; CHOOSE: the
-// greedy token is wanted, else the processed logits.
-template <typename T, int V, bool TABLE, bool CHOOSE>
+// greedy token is wanted, else the processed logits; PEEL: rows may begin at any element (vectors then
+// start at the first aligned one, and their mask bits straddle bytes).
+template <typename T, int V, bool TABLE, bool CHOOSE, bool PEEL>
 __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int slice, int table_words, bool direct) {
   constexpr int U = 3;  // accesses of a batch
   extern __shared__ uint32_t smem[];
@@ -157,7 +158,16 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
     if (r >= 0 && !none)
       mask = reinterpret_cast<const uint8_t*>(a.mask + r * a.mask_words) + (a.vocab_start + v0) / 8;
   }
-  const int vecs = n / V;
+  // elements in front of the first aligned vector (rows of an odd length begin anywhere), then vectors
+  const int head = !PEEL ? 0 : min(n, (int)((0 - reinterpret_cast<uintptr_t>(x)) / sizeof(T) % V));
+  const int vecs = (n - head) / V;
+  // mask bits of the V elements from e, and named ones
+  auto mask_bits = [&](int e) {
+    const int s = e & 7;
+    uint32_t bits = mask[e >> 3] >> s;
+    if constexpr (PEEL) bits |= (uint32_t)mask[(e + V - 1) >> 3] << 8 >> s;  // the same byte again does no harm
+    return bits;
+  };
   struct Batch {
     Vec<T, V> x[U];
     uint32_t allowed[U];
@@ -168,8 +178,8 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
       const int i = i0 + u * NT;
       q.allowed[u] = none ? 0u : 0xFFu;
       if (i < vecs) {
-        q.x[u] = *reinterpret_cast<const Vec<T, V>*>(x + i * V);
-        if (mask) q.allowed[u] = mask[i * V / 8] >> (i * V & 7);
+        q.x[u] = *reinterpret_cast<const Vec<T, V>*>(x + head + i * V);
+        if (mask) q.allowed[u] = mask_bits(head + i * V);
       }
     }
   };
@@ -305,7 +315,8 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
   }
   // The bits of the vector's elements that this pass chooses among: allowed, and not named.
   auto choosable = [&](uint32_t bits, int e) {
-    if constexpr (TABLE) bits &= ~(named[e >> 5] >> (e & 31));
+    if constexpr (TABLE && PEEL) bits &= ~__funnelshift_r(named[e >> 5], named[(e + V - 1) >> 5], e & 31);
+    else if constexpr (TABLE) bits &= ~(named[e >> 5] >> (e & 31));
     return bits;
   };
   unsigned long long key = 0;
@@ -329,7 +340,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * NT;
         if (i >= vecs || m[u] <= least || least != least) continue;
-        mask_vec(q.x[u], choosable(q.allowed[u], i * V));
+        mask_vec(q.x[u], choosable(q.allowed[u], head + i * V));
         const float k = max_vec(q.x[u]);
         if (k <= least) continue;
         best = least = k;
@@ -346,13 +357,14 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
     // the lanes that have the warp's largest value look for their element
     const uint32_t mine = (uint32_t)(choice_key(best, 0) >> 32);
     if (mine == __reduce_max_sync(0xffffffffu, mine) && best_i < vecs) {
-      Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(x + best_i * V);
+      const int e = head + best_i * V;
+      Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(x + e);
       uint32_t bits = none ? 0u : 0xFFu;
-      if (mask) bits = mask[best_i * V / 8] >> (best_i * V & 7);
-      mask_vec(raw, choosable(bits, best_i * V));
+      if (mask) bits = mask_bits(e);
+      mask_vec(raw, choosable(bits, e));
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const unsigned long long k = choice_key(widen(raw.v[j]), (uint32_t)(a.vocab_start + v0 + best_i * V + j));
+        const unsigned long long k = choice_key(widen(raw.v[j]), (uint32_t)(a.vocab_start + v0 + e + j));
         key = k > key ? k : key;
       }
     }
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
         const int i = i0 + u * NT;
         if (i >= vecs) continue;
         if (mask || none) mask_vec(q.x[u], q.allowed[u]);
-        *reinterpret_cast<Vec<T, V>*>(y + i * V) = q.x[u];
+        *reinterpret_cast<Vec<T, V>*>(y + head + i * V) = q.x[u];
       }
     };
     for (int i0 = tid; i0 < vecs; i0 += 2 * U * NT) {
@@ -374,7 +386,9 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
     }
   }
   auto is_allowed = [&](int e) { return !none && (!mask || (mask[e / 8] >> (e & 7) & 1)); };
-  for (int e = vecs * V + tid; e < n; e += NT) {  // fewer than V elements at the end of the last slice
+  // fewer than V elements in front of the vectors and behind them
+  for (int r = tid; r < n - vecs * V; r += NT) {
+    const int e = r < head ? r : r + vecs * V;
     if (TABLE && ((named[e >> 5] >> (e & 31)) & 1u)) continue;
     const float z = is_allowed(e) ? widen(x[e]) : -INFINITY;
     if constexpr (CHOOSE) {
@@ -460,7 +474,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
   }
 }
 
-template <typename T, int V, bool TABLE, bool CHOOSE>
+template <typename T, int V, bool TABLE, bool CHOOSE, bool PEEL>
 cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
   // One wave of two CTAs per SM: rows in 8 slices while few, whole rows (every id then read once, no
   // exchange) when many; more slices again where the table would leave one CTA per SM.
@@ -481,7 +495,7 @@ cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
   shape(8);
   while (cl > 1 && (int64_t)a.B * cl > 2 * sms) shape(cl / 2);
   while (cl < 8 && bytes > 110 * 1024) shape(cl * 2);
-  auto kernel = rules_kernel<T, V, TABLE, CHOOSE>;
+  auto kernel = rules_kernel<T, V, TABLE, CHOOSE, PEEL>;
   if (bytes > 48 * 1024) PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), (int)bytes));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cl, a.B);
@@ -501,15 +515,20 @@ cudaError_t launch(const LogitsArgs& a, cudaStream_t st) {
 template <typename T>
 cudaError_t dispatch(const LogitsArgs& a, cudaStream_t st) {
   constexpr int W = 16 / sizeof(T);
-  bool wide = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.in_stride % W == 0;
-  if (a.out) wide = wide && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride % W == 0;
+  // Vectors need rows of input and output that begin alike.  Rows that begin anywhere have their own variant: in
+  // one for all, aligned rows took longer (256 rows of 152,064 13.3 -> 20.8 us), and with single elements these do
+  // (75 rows of 50,257 bf16: the choice 14.0 us, now 7.3, processed with 300 ids 17.3, now 9.4).
   const bool table = a.ids != nullptr || a.bias_ids != nullptr;
-  const auto choose = [&](auto vec, auto tab) {
-    return a.token != nullptr ? launch<T, vec, tab, true>(a, st) : launch<T, vec, tab, false>(a, st);
+  const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.in_stride % W == 0;
+  const bool alike = !a.out || ((reinterpret_cast<uintptr_t>(a.out) - reinterpret_cast<uintptr_t>(a.logits)) % 16 == 0 &&
+                                (a.out_stride - a.in_stride) % W == 0);
+  const auto choose = [&](auto vec, auto peel) {
+    if (table) return a.token ? launch<T, vec, true, true, peel>(a, st) : launch<T, vec, true, false, peel>(a, st);
+    return a.token ? launch<T, vec, false, true, peel>(a, st) : launch<T, vec, false, false, peel>(a, st);
   };
   using std::integral_constant;
-  if (wide) return table ? choose(integral_constant<int, W>(), std::true_type()) : choose(integral_constant<int, W>(), std::false_type());
-  return table ? choose(integral_constant<int, 1>(), std::true_type()) : choose(integral_constant<int, 1>(), std::false_type());
+  if (!alike) return choose(integral_constant<int, 1>(), std::false_type());
+  return aligned ? choose(integral_constant<int, W>(), std::false_type()) : choose(integral_constant<int, W>(), std::true_type());
 }
 
 }  // namespace rules
