@@ -529,6 +529,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     tc::fence_after();
     tc::dealloc(tmem, C::COLS);
   }
+  if (a.after_prefix) pdl_wait();  // what waits for this grid waits for the one before, too
 }
 
 // ---------------------------------------------------------------- own keys of few queries
@@ -1103,7 +1104,9 @@ cudaError_t launch(const PrefixAttnArgs& a, cudaStream_t st) {
   const int64_t items = (int64_t)tiles * a.Hkv * (a.packed ? 1 : a.B);
   const int64_t ctas = a.whole > 0 ? a.whole + (items - a.whole) * a.splits : items;
   if (ctas > INT32_MAX || a.splits > 65535 || a.whole < 0 || a.whole > items) return cudaErrorInvalidValue;
-  prefix_kernel<D, NT><<<dim3((unsigned)ctas, a.whole > 0 ? 1 : a.splits), C::THREADS, C::SMEM, st>>>(pk, pv, k, v, a);
+  const dim3 grid((unsigned)ctas, a.whole > 0 ? 1 : a.splits);
+  if (a.after_prefix) return pra_launch_pdl(prefix_kernel<D, NT>, grid, dim3(C::THREADS), C::SMEM, st, pk, pv, k, v, a);
+  prefix_kernel<D, NT><<<grid, C::THREADS, C::SMEM, st>>>(pk, pv, k, v, a);
   return cudaGetLastError();
 }
 

@@ -93,6 +93,7 @@ struct PrefixAttnArgs {
   __nv_bfloat16* out;             // [B, T, H * D] contiguous
   float* lse;                     // [B, H, T] or null
   int* status;                    // set to 1 by a CTA that gave up on a bounded wait
+  int after_prefix;               // the launch before it on the stream is such a one, on whose results it does not wait
 };
 cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t stream);
 // Query tiles of a launch (CTAs before splitting), how many run at once (for choosing splits), rows of a tile.

@@ -596,6 +596,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   own.part_ml = a.part_ml;
   own.n_slots = a.n_slots;
   own.slot0 = a.splits;
+  own.after_prefix = 1;
   check(pra_prefix_attention(a, stream()), "shared_prefix_attention");
   check(pra_prefix_attention(own, stream()), "shared_prefix_attention");
   return merge();
