@@ -301,7 +301,8 @@ def test_shared_prefix_attention_views_lengths_and_scale(T):
 
 
 @pytest.mark.parametrize("B,T,P,lo,hi,H,Hkv,D", [(78, 1, 2170, 1, 66, 28, 4, 128), (64, 1, 8192, 64, 700, 32, 8, 128),
-                                                 (150, 1, 900, 1, 64, 16, 8, 128), (48, 3, 1500, 3, 90, 8, 2, 64)])
+                                                 (150, 1, 900, 1, 64, 16, 8, 128), (48, 3, 1500, 3, 90, 8, 2, 64),
+                                                 (40, 5, 3000, 5, 200, 32, 8, 64), (3, 512, 5000, 512, 600, 32, 8, 128)])
 def test_shared_prefix_attention_repeats_exactly(B, T, P, lo, hi, H, Hkv, D):
     """Both parts at once, many short rows to a CTA: every call gives the same bits, and the right ones."""
     from pdattention_b200.inference.shared_prefix import shared_prefix_attention
@@ -319,12 +320,13 @@ def test_shared_prefix_attention_repeats_exactly(B, T, P, lo, hi, H, Hkv, D):
     assert all(torch.equal(a, b) for r in again for a, b in zip(r, first))
 
 
-def test_shared_prefix_attention_streams_and_graphs():
+@pytest.mark.parametrize("B,T,H", [(6, 1, 8), (6, 9, 8), (50, 1, 8), (40, 260, 4)])
+def test_shared_prefix_attention_streams_and_graphs(B, T, H):
     from pdattention_b200.inference.shared_prefix import shared_prefix_attention
 
     torch.manual_seed(5)
-    B, P, cap, H, Hkv, D = 6, 400, 64, 8, 2, 128
-    mk = lambda s: (torch.randn(B, 1, H * D, device=DEV).bfloat16(), *torch.randn(2, P, Hkv * D, device=DEV).bfloat16(),  # noqa: E731
+    P, cap, Hkv, D = 400, 64, 2, 128
+    mk = lambda s: (torch.randn(B, T, H * D, device=DEV).bfloat16(), *torch.randn(2, P, Hkv * D, device=DEV).bfloat16(),  # noqa: E731
                     *torch.randn(2, B, cap, Hkv * D, device=DEV).bfloat16(),
                     torch.randint(1, cap + 1, (B,), device=DEV, dtype=torch.int32))
     one, two = mk(0), mk(1)
