@@ -424,10 +424,25 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   if (!partials) a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.lse = lse;
   const int prefix_blocks = ceil_div(a.P, 128), own_blocks = ceil_div(a.cap, 128);
-  const auto splits_for = [](const PrefixAttnArgs& p, int blocks) {
+  // Up to `most` parts of a tile's blocks.  In us: 2 (1.6) per block of a part, and each part costs the merge 0.1, more
+  // than 30 of them another 3 (a second round).  One row behind 32K with 2 KV heads: 64 parts 22.8 us, all 148 that
+  // run at once 27.4; 2 x 4 drafts behind 6,877 keys, head dim 64: 24 parts 17.7 us, 54 23.4.
+  const auto best_splits = [head_dim](int blocks, int most) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= std::min(blocks, most); ++s) {
+      const double us = (head_dim == 128 ? 2.0 : 1.6) * ceil_div(blocks, s) + 0.1 * s + (s > 30 ? 3 : 0);
+      if (us < least) {
+        least = us;
+        best = s;
+      }
+    }
+    return best;
+  };
+  const auto splits_for = [&](const PrefixAttnArgs& p, int blocks) {
     int tiles, slots;
     pra_prefix_attention_shape(p, &tiles, &slots);
-    return std::max(1, std::min(blocks, slots / tiles));
+    return best_splits(blocks, slots / tiles);
   };
   PrefixMergeArgs m{};
   m.B = a.B;
@@ -542,7 +557,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
       } else if (tiles <= sms) {
         // One tile a CTA: a CTA of each part fits on an SM.
         // A prefix CTA takes 8 + 2 (1.6) per block, two of them on an SM 2.9 (2).
-        const int splits = std::min(prefix_blocks, sms / tiles);
+        const int splits = best_splits(prefix_blocks, sms / tiles);
         const auto prefix_us = [&](int s, double per_block) { return 8 + per_block * ceil_div(prefix_blocks, s); };
         const double both = std::max(prefix_us(splits, wide ? 2.0 : 1.6), 6 + own_kb / 6000);
         const double after =
