@@ -1110,8 +1110,18 @@ cudaError_t launch(const PrefixAttnArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Two tiles per CTA read every key block once for 256 queries; one tile leaves room for two CTAs per SM.
-int tiles_per_cta(const PrefixAttnArgs& a) { return rows_of(a) > BM ? 2 : 1; }
+// Two tiles per CTA read every key block once for 256 queries; one tile leaves room for two CTAs per SM.  Row by
+// row two are 2 to 16% faster where they are full, or where there is less than a wave of them (4 x 600 query rows
+// behind 16K 112 us, with one 137); one is where the second of the last pair would be empty (122 x 324, head dim 64:
+// 472 -> 344 us).
+int tiles_per_cta(const PrefixAttnArgs& a) {
+  const int64_t rows = rows_of(a), ones = (rows + BM - 1) / BM, pairs = (ones + 1) / 2;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (!a.packed && ones * 115 < 2 * pairs * 100 && pairs * a.Hkv * a.B > sms) return 1;
+  return rows > BM ? 2 : 1;
+}
 
 }  // namespace prefix
 }  // namespace pra
