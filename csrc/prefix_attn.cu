@@ -32,7 +32,8 @@
 // Keys past the ones any query of the CTA may see are never multiplied: their scores are replaced by
 // -inf, and their value rows are zeroed in shared memory (a stale row may hold NaN, and 0 * NaN is
 // not 0).  Every wait is bounded; a CTA that times out sets *status, waits (bounded) for its copies
-// and MMAs in flight, frees its TMEM and returns.
+// and MMAs in flight, frees its TMEM and returns.  What it leaves unwritten the merge reads all the same, as
+// numbers without meaning: every index it takes from memory is written by CTAs that gave up, too.
 #include <algorithm>
 #include <map>
 #include <mutex>
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       mbar_init(q_full + i, 4);
     }
     mbar_init(drain, 1);
-    s_abort = 0;
+    s_abort = a.give_up;
     s_seen = 0;
     tc::fence_mbarrier_init();
   }
@@ -599,7 +600,7 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, OWARPS);
     }
-    s_abort = 0;
+    s_abort = a.give_up;
     s_row[0] = s_row[1] = -1;
     tc::fence_mbarrier_init();
   }
@@ -914,7 +915,7 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
         }
         asm volatile("bar.sync 1, %0;\n" ::"n"(OWARPS * 32) : "memory");
       }
-      if (tid == 0 && ok) {
+      if (tid == 0) {  // after a wait that gave up, too: the merge reads the pieces in this range
         if (u >= at.blk) a.first[item] = blockIdx.x;  // the run began at or before the item's first block
         if (at.blk + 1 == at.blocks) a.last[item] = blockIdx.x;
       }

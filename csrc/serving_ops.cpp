@@ -328,6 +328,9 @@ void rows_ok(const Tensor& t, int64_t width, const char* name) {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// Launches from here on take the way of CTAs whose waits ran out (set by tests of that way).
+bool give_up = false;
+
 // {out [like q], lse [B, H, T] or none}, or with `partials` {unnormalised o [B * T, H, 1, D], (max, sum)
 // [B * T, H, 1, 2]}.
 std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k, Tensor v, Tensor lengths,
@@ -383,6 +386,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   a.D = (int)head_dim;
   a.scale = (float)scale;
   a.status = pra_attention_status_word(q.device());
+  a.give_up = give_up;
   const auto fo = q.options().dtype(at::kFloat);
   // One allocation for the call's parts: n slots of sums and (max, sum) pairs for each of the queries, and `more`
   // floats.
@@ -587,6 +591,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     o.D = a.D;
     o.scale = a.scale;
     o.status = a.status;
+    o.give_up = a.give_up;
     o.after_prefix = a.P > 0;
     o.ctas = pra_own_attention_ctas(o);
     o.ctas = std::min(o.ctas, own_ctas);
@@ -672,4 +677,5 @@ void pra_bind_serving_ops(pybind11::module_& m) {
   m.def("choose_tokens", &choose_tokens);
   m.def("shared_prefix_attention", &prefix_attention);
   m.def("merge_attention_partials", &merge_attention_partials);
+  m.def("prefix_attention_give_up", [](bool on) { give_up = on; });
 }

@@ -1,0 +1,47 @@
+"""Corner calls of the serving operators on the GPU: waits that ran out, unusual views, empty tables, lifetimes."""
+
+import math
+
+import pytest
+import torch
+
+from test_serving_ops_gpu import half_step, prefix64, prefix_close, rotary_close, rotate64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _device():
+    if not torch.cuda.is_available():
+        pytest.skip("CUDA device required")
+
+
+@pytest.mark.parametrize("B,T,P,cap,H,Hkv,D", [(5, 1, 0, 200, 8, 2, 128), (9, 2, 300, 130, 8, 2, 64), (64, 1, 700, 100, 32, 8, 128),
+                                               (3, 40, 300, 90, 8, 2, 128), (1, 300, 500, 300, 8, 2, 64)])
+def test_waits_that_ran_out_end_in_the_status_word(B, T, P, cap, H, Hkv, D):
+    """Every CTA takes the way of one that gave up: the call ends, the status word says so, and the next
+    call is right again.  The workspace holds large integers beforehand."""
+    from pdattention_b200.inference.shared_prefix import shared_prefix_attention
+    from pdattention_b200.ops import _ext
+
+    torch.manual_seed(B)
+    ext, w = _ext.require(), Hkv * D
+    q = torch.randn(B, T, H * D, device=DEV).bfloat16()
+    pk, pv = torch.randn(2, P, w, device=DEV).bfloat16()
+    k, v = torch.randn(2, B, cap, w, device=DEV).bfloat16()
+    lengths = torch.randint(T, cap + 1, (B,), device=DEV, dtype=torch.int32)
+    run = lambda: shared_prefix_attention(q, pk, pv, k, v, lengths, H, Hkv, D, return_lse=True)  # noqa: E731
+    status = ext.attention_status(0)
+    junk = [torch.full((1 << n,), 0x7F7F7F7F, dtype=torch.int32, device=DEV) for n in range(8, 24)]
+    del junk
+    ext.prefix_attention_give_up(True)
+    try:
+        run()
+    finally:
+        ext.prefix_attention_give_up(False)
+    torch.cuda.synchronize()
+    assert int(status) == 1
+    status.zero_()
+    prefix_close(*run(), prefix64(q, pk, pv, k, v, lengths, None, H, Hkv, D, 1 / math.sqrt(D)), D)
+    assert int(status) == 0
