@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       mbar_init(q_full + i, 4);
     }
     mbar_init(drain, 1);
-    s_abort = a.give_up;
+    s_abort = 0;
     s_seen = 0;
     tc::fence_mbarrier_init();
   }
@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
         for (int kv = 0; kv < 2 && ok; ++kv) {
           const int r = issued % R;
           if (issued >= R) ok = wait(empty + r, (uint32_t)((issued / R - 1) & 1), &s_abort);
+          if (issued + 1 == a.give_up) s_abort = 1, ok = false;
           if (!ok) break;
           const CUtensorMap* map = kv == 0 ? (own ? &map_k : &map_pk) : (own ? &map_v : &map_pv);
           expect_tx(full + r, C::TILE);
@@ -336,10 +337,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
           tc::commit(s_full + i);
           if (i == NT - 1) mbar_arrive(empty + vt % R);
         }
-      }
-      if (!ok) {
-        tc::commit(drain);
-        tc::mbar_wait_cycles(drain, 0, WAIT_CYCLES);
       }
     }
   } else {
@@ -520,10 +517,16 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   __syncwarp();
   tc::fence_before();
   __syncthreads();
-  if (s_abort) {  // nothing may land in shared memory after the CTA has gone: wait for the copies in flight
+  if (s_abort) {
+    // Nothing may land in shared memory, and no MMA may read it or TMEM, after the CTA has gone: wait for both.
+    // Here and not where the issuer gives up: its own waits may all have been answered while another role's ran out.
     if (tid == 0 && a.status != nullptr) atomicExch(a.status, 1);
     for (int x = max(0, issued - R); x < issued; ++x)
       tc::mbar_wait_cycles(full + x % R, (uint32_t)((x / R) & 1), WAIT_CYCLES);
+    if (tid == ISSUER * 32) {  // the thread whose MMAs they are
+      tc::commit(drain);
+      tc::mbar_wait_cycles(drain, 0, WAIT_CYCLES);
+    }
     __syncthreads();
   }
   if (warp == PRODUCER) {
@@ -600,7 +603,7 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, OWARPS);
     }
-    s_abort = a.give_up;
+    s_abort = 0;
     s_row[0] = s_row[1] = -1;
     tc::fence_mbarrier_init();
   }
@@ -707,6 +710,10 @@ __global__ void __launch_bounds__(OwnCfg<D>::THREADS, 2)
         }
         const int st = issued % C::STAGES;
         if (issued >= C::STAGES && !wait(empty + st, (uint32_t)((issued / C::STAGES - 1) & 1), &s_abort)) break;
+        if (issued + 1 == a.give_up) {
+          s_abort = 1;
+          break;
+        }
         expect_tx(full + st, C::STAGE);
         const uint32_t to = smem_u32(smem + st * C::STAGE);
 #pragma unroll

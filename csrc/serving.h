@@ -93,7 +93,7 @@ struct PrefixAttnArgs {
   __nv_bfloat16* out;             // [B, T, H * D] contiguous
   float* lse;                     // [B, H, T] or null
   int* status;                    // set to 1 by a CTA that gave up on a bounded wait
-  int give_up;                    // 1: every CTA takes the way of one that gave up (nothing is loaded)
+  int give_up;                    // > 0: the producer of every CTA gives up in front of its give_up-th copy
   int after_prefix;               // the launch before it on the stream is such a one, on whose results it does not wait
 };
 cudaError_t pra_prefix_attention(const PrefixAttnArgs& a, cudaStream_t stream);

@@ -328,8 +328,9 @@ void rows_ok(const Tensor& t, int64_t width, const char* name) {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Launches from here on take the way of CTAs whose waits ran out (set by tests of that way).
-bool give_up = false;
+// > 0: launches from here on give up in front of a CTA's copy of that number, as if its wait had run out (set by tests
+// of that way).
+int give_up = 0;
 
 // {out [like q], lse [B, H, T] or none}, or with `partials` {unnormalised o [B * T, H, 1, D], (max, sum)
 // [B * T, H, 1, 2]}.
@@ -677,5 +678,5 @@ void pra_bind_serving_ops(pybind11::module_& m) {
   m.def("choose_tokens", &choose_tokens);
   m.def("shared_prefix_attention", &prefix_attention);
   m.def("merge_attention_partials", &merge_attention_partials);
-  m.def("prefix_attention_give_up", [](bool on) { give_up = on; });
+  m.def("prefix_attention_give_up", [](int64_t copy) { give_up = (int)copy; });
 }

@@ -45,3 +45,34 @@ def test_waits_that_ran_out_end_in_the_status_word(B, T, P, cap, H, Hkv, D):
     status.zero_()
     prefix_close(*run(), prefix64(q, pk, pv, k, v, lengths, None, H, Hkv, D, 1 / math.sqrt(D)), D)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("copy", [2, 3, 4, 5, 8])
+@pytest.mark.parametrize("B,T,P,cap,H,Hkv,D", [(64, 1, 4000, 700, 32, 8, 128), (64, 8, 4000, 700, 8, 2, 64), (5, 300, 3000, 300, 8, 2, 128),
+                                               (200, 300, 700, 300, 2, 1, 64)])
+def test_giving_up_with_copies_and_products_in_flight(copy, B, T, P, cap, H, Hkv, D):
+    """The wait that runs out is the producer's, behind some copies: the other roles still work on what came.
+    The CTAs end with nothing in flight, so the next call, on the same SMs, is right."""
+    from pdattention_b200.inference.shared_prefix import shared_prefix_attention
+    from pdattention_b200.ops import _ext
+
+    torch.manual_seed(copy)
+    ext, w = _ext.require(), Hkv * D
+    q = torch.randn(B, T, H * D, device=DEV).bfloat16()
+    pk, pv = torch.randn(2, P, w, device=DEV).bfloat16()
+    k, v = torch.randn(2, B, cap, w, device=DEV).bfloat16()
+    lengths = torch.full((B,), cap, device=DEV, dtype=torch.int32)
+    run = lambda: shared_prefix_attention(q, pk, pv, k, v, lengths, H, Hkv, D, return_lse=True)  # noqa: E731
+    first = run()
+    status = ext.attention_status(0)
+    assert int(status) == 0
+    ext.prefix_attention_give_up(copy)
+    try:
+        run()
+    finally:
+        ext.prefix_attention_give_up(0)
+    again = run()  # right behind it
+    torch.cuda.synchronize()
+    assert int(status) == 1
+    status.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(again, first))
