@@ -88,18 +88,30 @@ void rotary_positions(RotaryArgs& a, const Tensor& positions, const Tensor& firs
   a.pos64 = positions.scalar_type() == at::kLong;
 }
 
+// The one stride with which the leading dimensions of [..., heads, head_dim] walk its tokens in order; -1: there is
+// none.  Dimensions of size 1 are never walked: their strides say nothing.
+int64_t token_stride(at::IntArrayRef sizes, at::IntArrayRef strides) {
+  int64_t stride = 0, next = -1;  // the innermost walked dimension's stride; what the dimension around it has to have
+  for (int64_t d = (int64_t)sizes.size() - 3; d >= 0; --d) {
+    if (sizes[d] == 1) continue;
+    if (next < 0) stride = strides[d];
+    else if (strides[d] != next) return -1;
+    next = strides[d] * sizes[d];
+  }
+  return stride;
+}
+
 // The segment of x [..., heads, head_dim] (read in place where its tokens have one stride) and its new output.
 Tensor rotary_segment(RotarySegment& s, Tensor& x, int64_t head_dim) {
   TORCH_CHECK(x.dim() >= 2 && x.size(-1) == head_dim, "queries and keys must be [..., heads, head_dim] of one head_dim");
   auto out = torch::empty(x.sizes(), x.options());
   const int64_t heads = x.size(-2);
   TORCH_CHECK(heads <= 4096, "at most 4096 heads");
-  bool strided = x.stride(-1) == 1 || x.numel() == 0;
-  for (int64_t d = 0; d + 3 < x.dim(); ++d)  // the leading dimensions collapse to one token dimension
-    if (x.size(d) != 1 && x.stride(d) != x.stride(d + 1) * x.size(d + 1)) strided = false;
+  const int64_t token = token_stride(x.sizes(), x.strides());
+  const bool strided = (x.stride(-1) == 1 && token >= 0) || x.numel() == 0;
   if (!strided) x = x.contiguous();
   s.src = x.data_ptr();
-  s.src_token = x.dim() > 2 ? x.stride(-3) : heads * head_dim;
+  s.src_token = strided && x.numel() > 0 ? token : heads * head_dim;
   s.src_head = x.stride(-2);
   s.dst = out.data_ptr();
   s.dst_token = heads * head_dim;
@@ -674,6 +686,7 @@ std::vector<OptTensor> merge_attention_partials(Tensor part_o, Tensor part_ml, O
 void pra_bind_serving_ops(pybind11::module_& m) {
   m.def("rotary", &rotary);
   m.def("rotary_cache", &rotary_cache);
+  m.def("token_stride", [](const std::vector<int64_t>& sizes, const std::vector<int64_t>& strides) { return token_stride(sizes, strides); });
   m.def("process_logits", &process_logits);
   m.def("choose_tokens", &choose_tokens);
   m.def("shared_prefix_attention", &prefix_attention);

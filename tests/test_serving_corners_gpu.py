@@ -76,3 +76,18 @@ def test_giving_up_with_copies_and_products_in_flight(copy, B, T, P, cap, H, Hkv
     assert int(status) == 1
     status.zero_()
     assert all(torch.equal(a, b) for a, b in zip(again, first))
+
+
+def test_rotary_of_views_with_dimensions_of_one():
+    """Sizes of 1 among the leading dimensions, their strides those of a slice or of a permuted tensor."""
+    from pdattention_b200.ops.rotary import rotary, rotary_table
+
+    torch.manual_seed(0)
+    base = torch.randn(3, 2, 3, 4, 64, device=DEV).bfloat16()
+    table = rotary_table(64, 50)
+    for x in (base[:, ::2], base[:1].permute(1, 2, 0, 3, 4), base[:, :, ::3], base[:, :1, :1].transpose(0, 2), base.transpose(0, 2)):
+        pos = torch.randint(0, 50, x.shape[:-2], device=DEV)
+        rotary_close(rotary(x, None, pos, table)[0], rotate64(x, pos, table), x, 64)
+        leaf = torch.randn(x.shape, device=DEV).bfloat16().requires_grad_()
+        (grad,) = torch.autograd.grad(rotary(leaf, None, pos, table)[0], leaf, x)  # the incoming gradient is such a view
+        rotary_close(grad, rotate64(x, pos, table, inverse=True), x, 64)
