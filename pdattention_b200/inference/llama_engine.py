@@ -883,7 +883,8 @@ class PRALlamaEngine:
     def capture_decode(self, sample: bool = False, rules: LogitsRules | None = None,
                        history: TokenHistory | None = None) -> None:
         """Capture one ``decode_step`` into a CUDA graph (after at least one eager step).  ``rules`` and
-        ``history`` are read from their tensors at every replay.
+        ``history`` are read from (and the history written to) the tensors they hold now, which the engine
+        keeps for as long as the graph.
 
         Replays run the whole step (32 layers of GEMMs, routing, attention and the
         tensor-parallel collectives) as one graph launch; the collectives take their
@@ -906,6 +907,8 @@ class PRALlamaEngine:
                                     or (self.tp.epoch_dg - dg0) % 2):
             raise RuntimeError("a captured step must use both halves of each double buffer equally often")
         self._graph = graph
+        # the replayed kernels' addresses: another rule or history put in their place is not seen
+        self._graph_holds = [t for o in (rules, history) if o is not None for t in vars(o).values() if t is not None]
 
     def decode_step_graphed(self, token_ids: torch.Tensor) -> torch.Tensor:
         """``decode_step`` through the captured graph (returns the graph's static output: logits, or
@@ -917,6 +920,7 @@ class PRALlamaEngine:
     def release_graph(self) -> None:
         self._graph = None
         self._graph_out = None
+        self._graph_holds = None
 
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, lengths: torch.Tensor, max_new_tokens: int,

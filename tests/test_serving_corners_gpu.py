@@ -91,3 +91,28 @@ def test_rotary_of_views_with_dimensions_of_one():
         leaf = torch.randn(x.shape, device=DEV).bfloat16().requires_grad_()
         (grad,) = torch.autograd.grad(rotary(leaf, None, pos, table)[0], leaf, x)  # the incoming gradient is such a view
         rotary_close(grad, rotate64(x, pos, table, inverse=True), x, 64)
+
+
+def test_a_captured_step_keeps_its_rules_and_history():
+    """The caller's objects may go, or get other tensors: the graph's are alive until it is released."""
+    import weakref
+
+    from test_serving_engine_gpu import setup
+
+    from pdattention_b200.inference.logits import LogitsRules, TokenHistory
+
+    cfg, model, engine = setup(6)
+    ids, n = torch.randint(0, cfg.vocab_size, (2, 6)), torch.tensor([6, 3])
+    rules = LogitsRules(repetition=torch.full((2,), 1.5, device=DEV), bias_ids=torch.tensor([[3], [5]], device=DEV).int(),
+                        bias_values=torch.ones(2, 1, device=DEV))
+    history = TokenHistory.start(ids.to(DEV), n, 6)
+    tok = engine.prefill(ids, n, 6).float().argmax(-1)
+    engine.decode_step(tok, sample=True, rules=rules, history=history)
+    engine.capture_decode(sample=True, rules=rules, history=history)
+    held = [weakref.ref(t) for t in (rules.repetition, rules.bias_ids, rules.bias_values, history.ids, history.lengths,
+                                     history.prompt_lengths)]
+    rules.repetition = torch.full((2,), 9.0, device=DEV)
+    del rules, history
+    assert all(r() is not None for r in held)
+    engine.release_graph()
+    assert all(r() is None for r in held)
