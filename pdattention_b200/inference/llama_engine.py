@@ -620,6 +620,8 @@ class PRALlamaEngine:
                            else torch.zeros(B, device=self.device, dtype=torch.int32))
         if self.prefix is not None:  # the rows' own tokens follow the shared prefix
             self.pos_offset = self.pos_offset + self.prefix_tokens
+            # here and not in the first step that routes: a captured one would fill it at its replays only
+            self._no_len = torch.zeros(B, device=self.device, dtype=torch.int32)
         self._max_pos = int(self.pos_offset.max()) + max_len if B else max_len
         step = row_batch or B
         outs = [self._prefill_rows(ids[r: r + step], lengths[r: r + step], r) for r in range(0, B, step)]
@@ -796,8 +798,6 @@ class PRALlamaEngine:
         args = (q.unsqueeze(1), *self._prefix_kv(li), kc, vc, new_len, H, Hkv, D)
         if not routed:
             return shared_prefix_attention(*args).view(B, H * D)
-        if self._no_len is None or self._no_len.shape[0] != B:
-            self._no_len = torch.zeros(B, device=self.device, dtype=torch.int32)
         n_mem = max(1, -(-cfg.memory_tokens_per_row // 256))
         more = (torch.empty((B, H, n_mem, D), device=self.device, dtype=torch.float32),
                 torch.empty((B, H, n_mem, 2), device=self.device, dtype=torch.float32))

@@ -116,3 +116,29 @@ def test_a_captured_step_keeps_its_rules_and_history():
     assert all(r() is not None for r in held)
     engine.release_graph()
     assert all(r() is None for r in held)
+
+
+def test_a_capture_before_the_first_routed_step_leaves_eager_steps_right():
+    """Memory that comes after the first step, a capture, then an eager step: the same logits as without the capture."""
+    from test_serving_engine_gpu import setup
+
+    outs = []
+    for capture in (False, True):
+        cfg, model, engine = setup(7)
+        gen = torch.Generator().manual_seed(7)
+        draw = lambda *s: torch.randint(0, cfg.vocab_size, s, generator=gen)  # noqa: E731
+        engine.set_shared_prefix(draw(70))
+        engine.prefill(draw(2, 9), torch.tensor([9, 4]), 6)
+        engine.decode_step(draw(2))
+        engine.build_memory(draw(12, 16), torch.full((12,), 16, dtype=torch.int32))
+        engine.set_namespace(torch.zeros(2, dtype=torch.int32), torch.full((2,), 12, dtype=torch.int32))
+        if capture:
+            engine.capture_decode()
+            assert engine._no_len.tolist() == [0, 0]
+            kept = engine._no_len
+        outs.append(engine.decode_step(draw(2)))
+        if capture:
+            assert engine._no_len is kept  # made with the cache, not while the step was captured
+            engine.prefill(draw(2, 9), torch.tensor([9, 4]), 6)
+            assert engine._no_len is not kept
+    assert torch.equal(*outs)
