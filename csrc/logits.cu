@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(NT, 2) rules_kernel(const LogitsArgs a, int sl
   // the row's mask as bytes: element e of the slice is bit (vocab_start + v0 + e) % 8 of its byte
   const uint8_t* mask = nullptr;
   bool none = false;  // a mask row outside the masks allows nothing
-  if (a.mask) {
+  if (a.mask_words > 0) {  // (an empty set of masks has no address)
     const int r = a.mask_rows ? a.mask_rows[b] : b;
     none = r >= a.mask_count;
     if (r >= 0 && !none)

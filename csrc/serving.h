@@ -52,9 +52,9 @@ struct LogitsArgs {
   const int* bias_ids;     // [B, n_bias] or null; ids outside the vocabulary are skipped
   const float* bias_values;
   int n_bias;
-  const uint32_t* mask;    // [mask_count, mask_words] bit t: token id t is allowed, or null
+  const uint32_t* mask;    // [mask_count, mask_words] bit t: token id t is allowed
   int mask_count;
-  int64_t mask_words;
+  int64_t mask_words;      // 0: no mask
   const int* mask_rows;    // [B] mask of each row (negative: no mask) or null: mask b
   int64_t* token;          // [B] greedy token ids or null
   float* value;            // [B] their processed logits

@@ -142,3 +142,21 @@ def test_a_capture_before_the_first_routed_step_leaves_eager_steps_right():
             engine.prefill(draw(2, 9), torch.tensor([9, 4]), 6)
             assert engine._no_len is not kept
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("biases", [False, True])
+def test_an_empty_set_of_masks_allows_nothing(biases):
+    """mask [0, words] with mask_rows: every row that names a mask names one that is not there."""
+    from pdattention_b200.inference.logits import LogitsRules, choose_tokens, process_logits
+
+    x = torch.randn(3, 100, device=DEV)
+    more = dict(bias_ids=torch.tensor([[4]] * 3, device=DEV).int(), bias_values=torch.full((3, 1), 50.0, device=DEV)) if biases else {}
+    rules = LogitsRules(mask=torch.empty(0, 4, dtype=torch.int32, device=DEV),
+                        mask_rows=torch.tensor([0, -1, 7], dtype=torch.int32, device=DEV), **more)
+    want = x.clone()
+    if biases:
+        want[:, 4] += 50.0
+    want[0::2] = float("-inf")
+    assert torch.equal(process_logits(x, rules), want)
+    token, value = choose_tokens(x, rules)
+    assert token.tolist() == [-1, int(want[1].argmax()), -1] and torch.equal(value, want.amax(1))
