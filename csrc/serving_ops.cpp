@@ -431,7 +431,9 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   if (B == 0 || T == 0 || (a.P == 0 && a.cap == 0)) {
     if (partials) {
       auto r = joined();
-      joined_ml.fill_(-INFINITY);
+      joined_o.zero_();
+      joined_ml.zero_();
+      joined_ml.select(-1, 0).fill_(-INFINITY);
       return r;
     }
     out.zero_();

@@ -160,3 +160,22 @@ def test_an_empty_set_of_masks_allows_nothing(biases):
     assert torch.equal(process_logits(x, rules), want)
     token, value = choose_tokens(x, rules)
     assert token.tolist() == [-1, int(want[1].argmax()), -1] and torch.equal(value, want.amax(1))
+
+
+@pytest.mark.parametrize("P,cap,n", [(0, 0, 0), (0, 5, 0), (3, 0, 0), (300, 40, 0)])
+def test_partials_of_queries_that_see_nothing(P, cap, n):
+    """Sums 0, maximum -inf, sum of the weights 0, whether keys are there or not."""
+    from pdattention_b200.inference.shared_prefix import merge_attention_partials, shared_prefix_partials
+
+    B, T, H, Hkv, D = 2, 3, 4, 2, 64
+    junk = torch.full((1 << 16,), float("nan"), device=DEV)
+    del junk
+    q = torch.randn(B, T, H * D, device=DEV).bfloat16()
+    pk, pv = torch.randn(2, P, Hkv * D, device=DEV).bfloat16()
+    k, v = torch.randn(2, B, cap, Hkv * D, device=DEV).bfloat16()
+    none = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    o, ml = shared_prefix_partials(q, pk, pv, k, v, none, H, Hkv, D, prefix_lengths=none)
+    assert o.shape == (B * T, H, 1, D) and (o == 0).all()
+    assert (ml[..., 0] == float("-inf")).all() and (ml[..., 1] == 0).all()
+    out, lse = merge_attention_partials((o, ml), batch=B, return_lse=True)
+    assert (out == 0).all() and (lse == float("-inf")).all()
