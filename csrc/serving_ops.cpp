@@ -369,6 +369,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   if (pk.size(0) > 0) rows_ok(pk, width, "prefix keys"), rows_ok(pv, width, "prefix values");
   if (k.size(1) > 0 && B > 0) {
     rows_ok(k, width, "own keys"), rows_ok(v, width, "own values");
+    // tensor maps are specified with outer strides that are multiples of the inner ones
     for (const Tensor* t : {&k, &v})
       TORCH_CHECK(B == 1 || k.size(1) == 1 || t->stride(0) % t->stride(1) == 0,
                   "the batch stride of own keys and values must be a multiple of their row stride");
@@ -387,8 +388,9 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
   a.k = reinterpret_cast<const __nv_bfloat16*>(k.data_ptr());
   a.v = reinterpret_cast<const __nv_bfloat16*>(v.data_ptr());
   a.cap = (int)k.size(1);
-  a.k_row = k.size(1) > 1 ? k.stride(1) : width;
-  a.v_row = v.size(1) > 1 ? v.stride(1) : width;
+  // (and of a single own row the batch stride is a multiple)
+  a.k_row = k.size(1) > 1 ? k.stride(1) : B > 1 ? k.stride(0) : width;
+  a.v_row = v.size(1) > 1 ? v.stride(1) : B > 1 ? v.stride(0) : width;
   a.k_batch = B > 1 ? k.stride(0) : a.cap * a.k_row;
   a.v_batch = B > 1 ? v.stride(0) : a.cap * a.v_row;
   a.len = per_row<int>(lengths, at::kInt, q, B, "lengths");

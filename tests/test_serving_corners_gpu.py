@@ -179,3 +179,31 @@ def test_partials_of_queries_that_see_nothing(P, cap, n):
     assert (ml[..., 0] == float("-inf")).all() and (ml[..., 1] == 0).all()
     out, lse = merge_attention_partials((o, ml), batch=B, return_lse=True)
     assert (out == 0).all() and (lse == float("-inf")).all()
+
+
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("P", [0, 90])
+def test_one_own_key_at_any_batch_stride(T, P):
+    """A capacity of one row: the batch stride is no multiple of the row's width."""
+    from pdattention_b200.inference.shared_prefix import shared_prefix_attention
+
+    torch.manual_seed(T)
+    B, H, Hkv, D = 5, 8, 2, 64
+    w = Hkv * D
+    q = torch.randn(B, T, H * D, device=DEV).bfloat16()
+    pk, pv = torch.randn(2, P, w, device=DEV).bfloat16()
+    k = torch.randn(B, w + 40, device=DEV).bfloat16()[:, None, 8: 8 + w]
+    v = torch.randn(B, 2 * w + 8, device=DEV).bfloat16()[:, None, 16: 16 + w]
+    lengths = torch.tensor([1, 0, 1, 1, 1], dtype=torch.int32, device=DEV)
+    out, lse = shared_prefix_attention(q, pk, pv, k, v, lengths, H, Hkv, D, return_lse=True)
+    prefix_close(out, lse, prefix64(q, pk, pv, k, v, lengths, None, H, Hkv, D, 1 / math.sqrt(D)), D)
+
+
+def test_batch_strides_that_no_tensor_map_takes_are_refused():
+    from pdattention_b200.inference.shared_prefix import shared_prefix_attention
+
+    w = 64
+    k = torch.zeros(2 * (3 * w + 8), device=DEV).bfloat16().as_strided((2, 3, w), (3 * w + 8, w, 1))
+    with pytest.raises(RuntimeError, match="batch stride"):
+        shared_prefix_attention(torch.zeros(2, 1, w, device=DEV).bfloat16(), k[0], k[0], k, k,
+                                torch.ones(2, dtype=torch.int32, device=DEV), 1, 1, 64)
