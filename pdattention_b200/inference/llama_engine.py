@@ -30,7 +30,7 @@ import torch
 
 from ..models.llama import PRALlamaConfig, PRALlamaReference
 from ..ops import _ext
-from ..ops.rotary import RotaryTable, rotary_cache, rotary_frequencies
+from ..ops.rotary import RotaryTable, dynamic_window, rotary_angles, rotary_cache
 from ..tracing import traced
 from .logits import LogitsRules, TokenHistory, choose_tokens
 from .routing import select_chunks
@@ -308,17 +308,32 @@ class PRALlamaEngine:
 
     # -- helpers ----------------------------------------------------------------
     def rope_tables(self, max_pos: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """fp32 cos/sin ``[max_pos, Dh/2]`` computed in fp64 (cached, grown on demand)."""
+        """fp32 cos/sin ``[max_pos, Dh/2]`` computed in fp64 (cached, grown on demand).  Under dynamic scaling
+        row p is that of a sequence which ends at p: what a decode step, or anything within the window, takes."""
         have = max(self._rope_cache) if self._rope_cache else 0
         if have < max_pos:
             cfg = self.cfg
             n = max(max_pos, 2 * have)
-            freq, scale = rotary_frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling,
-                                             cfg.max_position_embeddings)
-            ang = torch.arange(n, dtype=torch.float64)[:, None] * freq[None]
+            ang, scale = rotary_angles(torch.arange(n), cfg.head_dim, cfg.rope_theta, cfg.rope_scaling)
             self._rope_cache = {n: ((ang.cos() * scale).float().to(self.device),
                                     (ang.sin() * scale).float().to(self.device))}
         return next(iter(self._rope_cache.values()))
+
+    def _rotary(self, pos: torch.Tensor, lengths, longest: int,
+                max_pos: int | None = None) -> tuple[RotaryTable, torch.Tensor]:
+        """Table and rows of it (flat) for tokens at ``pos`` ``[rows, T]`` of sequences of ``lengths`` ``[rows]``
+        (or one) tokens, ``longest`` at most.  Past the window of dynamic scaling the angles go by a
+        sequence's length, whatever it shares a batch with: there token m has row m of a table of its own."""
+        cfg = self.cfg
+        window = dynamic_window(cfg.rope_scaling)
+        if window is None or longest <= window:
+            return RotaryTable(*self.rope_tables(max_pos or longest)), pos.reshape(-1)
+        if torch.is_tensor(lengths):
+            lengths = lengths[:, None]
+        ang, scale = rotary_angles(pos, cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, lengths)
+        ang = ang.flatten(0, 1)
+        return (RotaryTable((ang.cos() * scale).float(), (ang.sin() * scale).float()),
+                torch.arange(pos.numel(), device=self.device, dtype=torch.int32))
 
     def _norm(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
         return self.ext.norm_fwd(x, w, None, self.cfg.rms_norm_eps, True)[0]
@@ -493,31 +508,29 @@ class PRALlamaEngine:
         if n == 0:
             return
         mem.chunk_len[first: first + n].copy_(lengths.to(self.device, torch.int32))
-        cos, sin = self.rope_tables(tc)
         if self.tp is not None:  # each row-parallel partial must fit the peer buffer
             batch_chunks = max(1, min(batch_chunks, self.tp.max_partial // (tc * cfg.hidden_size)))
         for c0 in range(0, n, batch_chunks):
             c1 = min(n, c0 + batch_chunks)
             self._encode_chunk_batch(mem, chunks[c0:c1].to(self.device), mem.chunk_len[first + c0: first + c1],
-                                     first + c0, cos, sin)
+                                     first + c0)
         if self.tp is not None:  # gists are computed per KV-head slice; every rank gets all of them
             self.tp.gather_gists(mem, first, n)
         # bf16 routing copy for the tensor-core scoring GEMM
         sl = slice(first, first + n)
         mem.gn_bf16[:, sl].copy_(mem.gn.view(cfg.num_hidden_layers, mem.C_pad, -1)[:, sl])
 
-    def _encode_chunk_batch(self, mem: ChunkMemory, ids, lengths, c0, cos, sin):
+    def _encode_chunk_batch(self, mem: ChunkMemory, ids, lengths, c0):
         cfg, ext = self.cfg, self.ext
         n, tc = ids.shape
         M = n * tc
-        pos = torch.arange(tc, device=self.device, dtype=torch.int32).repeat(n)
+        table, pos = self._rotary(torch.arange(tc, device=self.device, dtype=torch.int32).expand(n, tc), lengths, tc)
         rows = (torch.arange(M, device=self.device, dtype=torch.int32) + c0 * tc)
         valid = (torch.arange(tc, device=self.device)[None] < lengths[:, None]).to(torch.uint8).contiguous()
         dest = torch.arange(c0, c0 + n, device=self.device, dtype=torch.int32)
         starts = rows.view(n, tc)[:, 0].contiguous()
         x = self._embed(ids)
         qd, kd = self.q_dim, self.kv_dim
-        table = RotaryTable(cos, sin)
         for li, lw in enumerate(self.w.layers):
             h = self._norm(x, self._ln(lw.ln_in))
             qkv = self._gemm(h, lw.qkv, lw.qkv_bias)
@@ -564,7 +577,8 @@ class PRALlamaEngine:
         """Every row of the following prefills starts with ``ids`` ``[P]`` (``None``: none): a prompt encoded
         once, whose keys and values all rows attend over.  Prompts given to ``prefill`` are what
         follows it, at positions ``P, P + 1, ...``.  Encoded ``chunk_tokens`` at a time (activation
-        memory), each chunk behind the ones before it; prefix tokens read no chunk memory."""
+        memory), each chunk behind the ones before it; prefix tokens read no chunk memory.  Under dynamic
+        scaling its keys keep the angles of a sequence of ``P`` tokens, as a cached prompt's do."""
         self.prefix = None
         self.cache = self.cache_len = None  # a cache filled behind another prefix does not fit this one
         self.release_graph()  # a captured step reads the prefix that has just gone
@@ -578,18 +592,18 @@ class PRALlamaEngine:
         ids = ids.to(self.device)
         P, qd, kd = ids.shape[0], self.q_dim, self.kv_dim
         self.prefix = torch.empty((cfg.num_hidden_layers, P, 2 * kd), device=self.device, dtype=torch.bfloat16)
-        table = RotaryTable(*self.rope_tables(P))
         if self.tp is not None:  # each row-parallel partial must fit the peer buffer
             chunk_tokens = max(1, min(chunk_tokens, self.tp.max_partial // cfg.hidden_size))
         for p0 in range(0, P, chunk_tokens):
             n = min(chunk_tokens, P - p0)
             rows = torch.arange(p0, p0 + n, device=self.device, dtype=torch.int32)
+            table, pos = self._rotary(rows[None], P, P)
             length = torch.full((1,), n, device=self.device, dtype=torch.int32)
             x = self._embed(ids[p0: p0 + n])
             for li, lw in enumerate(self.w.layers):
                 qkv = self._gemm(self._norm(x, self._ln(lw.ln_in)), lw.qkv, lw.qkv_bias)
                 k, v = self._prefix_kv(li)
-                q = rotary_cache(qkv, self.heads, self.kv_heads, cfg.head_dim, rows, table, k, v, rows)
+                q = rotary_cache(qkv, self.heads, self.kv_heads, cfg.head_dim, pos, table, k, v, rows)
                 if li == len(self.w.layers) - 1:
                     break  # the last layer's output is never read
                 pk, pv = self._prefix_kv(li, p0)
@@ -632,16 +646,15 @@ class PRALlamaEngine:
         B, T = ids.shape
         max_len = self.max_len
         qd, kd = self.q_dim, self.kv_dim
-        cos, sin = self.rope_tables(self._max_pos)
         M = B * T
-        pos = (torch.arange(T, device=self.device, dtype=torch.int32)[None]
-               + self.pos_offset[r0: r0 + B, None]).reshape(-1)
+        offset = self.pos_offset[r0: r0 + B]
+        table, pos = self._rotary(torch.arange(T, device=self.device, dtype=torch.int32)[None] + offset[:, None],
+                                  offset + lengths, self._max_pos - max_len + T, self._max_pos)
         rows = ((torch.arange(B, device=self.device, dtype=torch.int32)[:, None] + r0) * max_len
                 + torch.arange(T, device=self.device, dtype=torch.int32)[None]).reshape(-1)
         valid = (torch.arange(T, device=self.device)[None] < lengths[:, None]).to(torch.uint8).contiguous()
         last = (torch.arange(B, device=self.device) * T + lengths.long() - 1)
         x = self._embed(ids)
-        table = RotaryTable(cos, sin)
         full = torch.full((B,), T, device=self.device, dtype=torch.int32)  # token t sees own tokens 0 .. t
         use_memory = self.memory is not None and self.namespace is not None and cfg.top_k_chunks > 0
         namespace = None

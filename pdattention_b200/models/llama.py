@@ -35,7 +35,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops.rotary import rotary_frequencies
+from ..ops.rotary import rotary_angles, rotary_frequencies
 
 _FAMILIES = ("llama", "mistral", "qwen2")
 
@@ -61,7 +61,9 @@ class PRALlamaConfig:
     direct_window: int = 4096
     pra_layers: tuple | None = None   # layer ids that read memory (None: every layer)
     memory_budget_tokens: int | None = None  # cap on materialised memory tokens per row and layer
-    rope_scaling: dict | None = None  # long-context scaling of the rotary angles (ops.rotary.rotary_frequencies)
+    # long-context scaling of the rotary angles (ops.rotary.rotary_frequencies); dynamic: past the window each row
+    # by its own length, what is cached keeps the angles of its forward
+    rope_scaling: dict | None = None
 
     def __post_init__(self):
         if self.family not in _FAMILIES:
@@ -143,10 +145,10 @@ PRESETS = {"llama3-8b": llama3_8b, "mistral-7b": mistral_7b, "qwen2-7b": qwen2_7
 # Rotary positions
 # ---------------------------------------------------------------------------
 
-def rope_tables(cfg: PRALlamaConfig, positions: torch.Tensor, dtype=torch.float32):
-    """cos/sin ``[..., Dh]`` for integer ``positions`` (HF ``rotate_half`` layout)."""
-    freq, scale = rotary_frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, cfg.max_position_embeddings)
-    ang = positions.to(torch.float64)[..., None] * freq.to(positions.device)
+def rope_tables(cfg: PRALlamaConfig, positions: torch.Tensor, dtype=torch.float32, lengths=None):
+    """cos/sin ``[..., Dh]`` for integer ``positions`` (HF ``rotate_half`` layout) of sequences of
+    ``lengths`` (``ops.rotary.rotary_angles``)."""
+    ang, scale = rotary_angles(positions, cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, lengths)
     ang = torch.cat([ang, ang], dim=-1)
     return (ang.cos() * scale).to(dtype), (ang.sin() * scale).to(dtype)
 
@@ -295,7 +297,7 @@ class PRALlamaReference(nn.Module):
         cfg = self.cfg
         c, tc = chunks.shape
         pos = torch.arange(tc, device=chunks.device).expand(c, tc)
-        cos, sin = rope_tables(cfg, pos)
+        cos, sin = rope_tables(cfg, pos, lengths=lengths.to(chunks.device)[:, None])
         valid = torch.arange(tc, device=chunks.device)[None] < lengths[:, None]
         x = self.model.embed_tokens(chunks).float()
         mem = LlamaChunkMemory(length=lengths.clone())
@@ -353,9 +355,9 @@ class PRALlamaReference(nn.Module):
         cfg = self.cfg
         b, t = input_ids.shape
         pos = torch.arange(t, device=input_ids.device).expand(b, t)
-        cos, sin = rope_tables(cfg, pos)
         valid = attention_mask.bool() if attention_mask is not None else None
         last = (valid.long().sum(1) - 1) if valid is not None else torch.full((b,), t - 1, device=input_ids.device)
+        cos, sin = rope_tables(cfg, pos, lengths=last[:, None] + 1)
         x = self.model.embed_tokens(input_ids).float()
         selections = []
         for li, layer in enumerate(self.model.layers):
@@ -389,7 +391,7 @@ def reference_step(model: PRALlamaReference, ids: torch.Tensor, cache: list, mem
     t0 = cache[0][0].shape[0] if cache and cache[0][0] is not None else 0
     T = ids.shape[0]
     pos = torch.arange(t0, t0 + T, device=ids.device)[None] + int(position_offset)
-    cos, sin = rope_tables(cfg, pos)
+    cos, sin = rope_tables(cfg, pos, lengths=t0 + T + int(position_offset))
     x = model.model.embed_tokens(ids[None]).float()
     picks = []
     scale = 1.0 / math.sqrt(cfg.head_dim)

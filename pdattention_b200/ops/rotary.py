@@ -38,7 +38,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
 
     * ``linear``: every angle divided by ``factor``;
     * ``ntk``: the base raised to ``theta * factor^(d / (d - 2))``; ``dynamic``: the same with the
-      factor grown with ``max_positions`` over ``original_max_position_embeddings``;
+      factor grown with ``max_positions`` over ``original_max_position_embeddings``: the angles of a
+      sequence of that length (``rotary_angles`` takes sequences of several lengths);
     * ``llama3``: wavelengths over ``original / low_freq_factor`` divided by ``factor``, those under
       ``original / high_freq_factor`` kept, a linear blend between;
     * ``yarn``: pairs that turn less than ``beta_slow`` times over the original window are divided by
@@ -96,6 +97,34 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
         m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
         scale = mscale(float(m)) / mscale(float(m_all)) if m and m_all else mscale(1.0)
     return freq * (1 - ramp) + freq / factor * ramp, float(scale)
+
+
+def dynamic_window(scaling: dict | None) -> int | None:
+    """The window of ``dynamic`` scaling, past which angles go by the length of the sequence; ``None`` for others."""
+    if not scaling or scaling.get("rope_type", scaling.get("type")) != "dynamic":
+        return None
+    return int(scaling["original_max_position_embeddings"])
+
+
+def rotary_angles(positions: torch.Tensor, rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None,
+                  lengths: torch.Tensor | int | None = None) -> tuple[torch.Tensor, float]:
+    """fp64 angles ``[..., rotary_dim / 2]`` of integer ``positions`` ``[...]`` and the factor on cosines and
+    sines.  ``lengths`` (broadcast against ``positions``): the length of the sequence that a position is rotated
+    in, which only ``dynamic`` scaling goes by; by default the sequence ends at the position, as in a decode
+    step."""
+    freq, scale = rotary_frequencies(rotary_dim, theta, scaling)
+    window = dynamic_window(scaling)
+    positions = positions.to(torch.float64)[..., None]
+    if window is None or rotary_dim == 2:
+        return positions * freq.to(positions.device), scale
+    if lengths is None:
+        lengths = positions + 1
+    else:
+        lengths = torch.as_tensor(lengths, device=positions.device).to(torch.float64)[..., None]
+    factor = float(scaling.get("factor", 1.0))
+    grown = factor * lengths.clamp(min=window) / window - (factor - 1.0)
+    pair = torch.arange(0, rotary_dim // 2, dtype=torch.float64, device=positions.device) / (rotary_dim // 2)
+    return positions * (float(theta) * grown ** (rotary_dim / (rotary_dim - 2))) ** -pair, scale
 
 
 def rotary_table(rotary_dim: int, max_positions: int, *, theta: float = 10000.0, scaling: dict | None = None,

@@ -44,3 +44,57 @@ def test_token_stride_ignores_dimensions_of_one():
             steps = first.diff()
             assert not (steps == steps[0]).all()  # there is none
     assert found > 50
+
+
+def test_dynamic_scaling_matches_hugging_face_past_the_window():
+    """A prompt behind the window, decode steps on its cache, and a prompt within the window."""
+    import transformers
+
+    from pdattention_b200.hf.convert import reference_from_hf
+    from pdattention_b200.models.llama import hf_config, reference_step, tiny_llama
+    from pdattention_b200.models.llama import PRALlamaReference
+
+    source = PRALlamaReference(tiny_llama(max_position_embeddings=32)).eval()
+    source.reset_parameters(seed=0, std=0.2)
+    hcfg = hf_config(source.cfg)
+    hcfg.rope_parameters = {"rope_type": "dynamic", "factor": 4.0, "rope_theta": source.cfg.rope_theta}
+    hcfg._attn_implementation = "eager"
+    fresh = lambda: transformers.LlamaForCausalLM(hcfg).eval()  # noqa: E731 (it keeps the longest length that it saw)
+    hf = fresh()
+    hf.load_state_dict(source.state_dict(), strict=False)
+    ours = reference_from_hf(hf)
+    assert ours.cfg.rope_scaling["rope_type"] == "dynamic"
+    ids = torch.randint(0, source.cfg.vocab_size, (1, 103), generator=torch.Generator().manual_seed(1))
+    # tolerance as in the comparison of the other scalings: the other side's angles are fp32
+    close = lambda a, b: torch.allclose(a, b, atol=2e-3, rtol=1e-3)  # noqa: E731
+    with torch.no_grad():
+        within = hf(ids[:, :32]).logits
+        assert close(ours(ids[:, :32]), within) and close(source(ids[:, :32]), within)  # not yet scaled
+        out = hf(ids[:, :100], use_cache=True)
+        assert close(ours(ids[:, :100]), out.logits)
+        assert not torch.allclose(source(ids[:, :100]), out.logits, atol=2e-2, rtol=1e-2)
+        cache = [[None, None] for _ in range(source.cfg.num_hidden_layers)]
+        assert close(reference_step(ours, ids[0, :100], cache, None, None)[0], out.logits[0])
+        for t in range(100, 103):
+            out = hf(ids[:, t: t + 1], past_key_values=out.past_key_values, use_cache=True)
+            assert close(reference_step(ours, ids[0, t: t + 1], cache, None, None)[0], out.logits[0])
+
+
+def test_angles_of_sequences_of_several_lengths():
+    from pdattention_b200.ops.rotary import rotary_angles, rotary_frequencies
+
+    d = {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 100}
+    pos = torch.arange(300).expand(3, 300)
+    lengths = torch.tensor([300, 101, 60])
+    got, one = rotary_angles(pos, 8, 10000.0, d, lengths[:, None])
+    assert got.shape == (3, 300, 4) and one == 1.0
+    for row, n in enumerate(lengths.tolist()):
+        assert torch.allclose(got[row], torch.arange(300.0, dtype=torch.float64)[:, None] * rotary_frequencies(8, 10000.0, d, n)[0],
+                              rtol=1e-13)
+    steps, _ = rotary_angles(torch.arange(300), 8, 10000.0, d)  # each position the end of its sequence
+    for p in (0, 50, 99, 100, 101, 299):
+        assert torch.allclose(steps[p], p * rotary_frequencies(8, 10000.0, d, p + 1)[0], rtol=1e-13)
+    for scaling in (None, {"type": "linear", "factor": 3.0}):  # lengths do not matter
+        freq, _ = rotary_frequencies(8, 10000.0, scaling)
+        assert torch.equal(rotary_angles(pos, 8, 10000.0, scaling, lengths[:, None])[0], pos.double()[..., None] * freq)
+    assert torch.equal(rotary_angles(pos, 2, 10000.0, d, 300)[0][..., 0], pos.double())  # a single pair has no base

@@ -207,3 +207,77 @@ def test_batch_strides_that_no_tensor_map_takes_are_refused():
     with pytest.raises(RuntimeError, match="batch stride"):
         shared_prefix_attention(torch.zeros(2, 1, w, device=DEV).bfloat16(), k[0], k[0], k, k,
                                 torch.ones(2, dtype=torch.int32, device=DEV), 1, 1, 64)
+
+
+class Routing:
+    """The oracle takes the chunks that the engine took, so that a tie decided by bf16 activations changes no
+    logits; each of them must be one of the oracle's best, up to the bound of the engine's tests (a cosine of
+    0.995 to the fp32 activations: a query and a gist turned by at most sqrt(2 * 0.005) each)."""
+
+    def __init__(self, engine, monkeypatch):
+        from pdattention_b200.models import llama
+
+        self.engine, self.taken, self.row, self.layer = engine, {}, 0, 0
+        route, F = engine._route, torch.nn.functional
+
+        def recording(layer, *args, **kw):
+            out = route(layer, *args, **kw)
+            self.taken.setdefault(layer, []).append(engine.last_selection[layer])
+            return out
+
+        def select(cfg, query, gist, namespace):
+            taken = [c for c in torch.cat(self.taken[self.layer])[self.row].tolist() if c >= 0]
+            score = F.normalize(gist.float(), dim=-1) @ F.normalize(query[0].float(), dim=-1)
+            best = score[namespace[0]].topk(cfg.top_k_chunks).values
+            assert sorted(set(taken)) == taken and len(taken) == cfg.top_k_chunks
+            assert (score[taken] >= best[-1] - 2 * 2 * math.sqrt(2 * 0.005)).all()
+            self.layer += 1
+            return [taken]
+
+        engine._route = recording
+        monkeypatch.setattr(llama, "select_chunks", select)
+
+    def step(self, row):
+        self.row, self.layer = row, 0
+
+
+@pytest.mark.parametrize("prefix,memory,row_batch", [(0, False, None), (0, True, 1), (20, False, None), (60, True, None)])
+def test_dynamic_scaling_past_the_window(prefix, memory, row_batch, monkeypatch):
+    """Rows of several lengths, each scaled by its own; prefill, eager and replayed steps, against the fp32 oracle."""
+    from test_serving_engine_gpu import close, setup
+
+    from pdattention_b200.models.llama import reference_step
+
+    cfg, model, engine = setup(8, chunk_tokens=48,
+                               rope_scaling={"rope_type": "dynamic", "factor": 4.0, "original_max_position_embeddings": 32})
+    L, B = cfg.num_hidden_layers, 3
+    ids, n = torch.randint(0, cfg.vocab_size, (B, 90)), torch.tensor([90, 41, 7])
+    ref_mem = ns = None
+    if memory:
+        chunks, lengths = torch.randint(0, cfg.vocab_size, (12, 48)), torch.randint(20, 49, (12,))
+        engine.build_memory(chunks, lengths)  # chunks on both sides of the window
+        engine.set_namespace(torch.zeros(B), torch.full((B,), 12))
+        ref_mem, ns = model.encode_chunks(chunks, lengths), list(range(12))
+    routing = Routing(engine, monkeypatch)
+    caches = [[[None, None] for _ in range(L)] for _ in range(B)]
+    if prefix:
+        head = torch.randint(0, cfg.vocab_size, (prefix,))
+        engine.set_shared_prefix(head, chunk_tokens=25)
+        for b in range(B):
+            reference_step(model, head, caches[b], None, None)
+    logits = engine.prefill(ids, n, 8, row_batch=row_batch)
+    for b in range(B):
+        routing.step(b)
+        close(logits[b], reference_step(model, ids[b, : n[b]], caches[b], ref_mem, ns)[0][-1], 0.995)
+    for step in range(4):
+        routing.taken.clear()
+        if step == 2:
+            engine.capture_decode()
+        tok = torch.randint(0, cfg.vocab_size, (B,))
+        got = engine.decode_step(tok) if step < 2 else engine.decode_step_graphed(tok)
+        if step == 3:  # nothing is recorded at a replay: the graph's own outputs
+            routing.taken.update({layer: [sel] for layer, sel in engine.last_selection.items()})
+        for b in range(B):
+            routing.step(b)
+            close(got[b], reference_step(model, tok[b: b + 1], caches[b], ref_mem, ns)[0][-1], 0.99)
+    engine.release_graph()
