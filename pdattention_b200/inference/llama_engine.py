@@ -213,6 +213,7 @@ class PRALlamaEngine:
         self.page_table: torch.Tensor | None = None  # [B, P] pages per row (paged chunk cache)
         self._row0 = 0  # first row of the prefill row batch being routed
         self.prefix: torch.Tensor | None = None  # [L, P, 2 * kv_dim] keys and values of the shared prefix
+        self.prefix_ids: torch.Tensor | None = None  # [P] its token ids
         self._no_len: torch.Tensor | None = None  # zero local lengths (memory-only decode attention)
         self.last_selection: dict[int, torch.Tensor] = {}
         # Vocabulary-parallel LM head: under tensor parallelism each rank holds rows
@@ -579,7 +580,7 @@ class PRALlamaEngine:
         follows it, at positions ``P, P + 1, ...``.  Encoded ``chunk_tokens`` at a time (activation
         memory), each chunk behind the ones before it; prefix tokens read no chunk memory.  Under dynamic
         scaling its keys keep the angles of a sequence of ``P`` tokens, as a cached prompt's do."""
-        self.prefix = None
+        self.prefix = self.prefix_ids = None
         self.cache = self.cache_len = None  # a cache filled behind another prefix does not fit this one
         self.release_graph()  # a captured step reads the prefix that has just gone
         if ids is None or ids.numel() == 0:
@@ -589,7 +590,7 @@ class PRALlamaEngine:
             raise ValueError("a shared prefix is one row of token ids")
         if cfg.head_dim not in (64, 128):
             raise ValueError("a shared prefix needs head dim 64 or 128")
-        ids = ids.to(self.device)
+        self.prefix_ids = ids = ids.to(self.device, copy=True)
         P, qd, kd = ids.shape[0], self.q_dim, self.kv_dim
         self.prefix = torch.empty((cfg.num_hidden_layers, P, 2 * kd), device=self.device, dtype=torch.bfloat16)
         if self.tp is not None:  # each row-parallel partial must fit the peer buffer
@@ -729,7 +730,8 @@ class PRALlamaEngine:
         """One token per row at position ``cache_len[b]``; returns logits ``[B, V]``, or with
         ``sample=True`` the greedy next token ids ``[B]`` (no full-vocabulary logits are formed
         under tensor parallelism).  With ``rules`` the choice is made after them, -1 where they
-        leave a row nothing, and joins ``history``."""
+        leave a row nothing, and joins ``history`` (which begins with ``prefix_ids`` behind a shared prefix:
+        ``TokenHistory.start``)."""
         cfg, ext = self.cfg, self.ext
         B = token_ids.shape[0]
         qd, kd = self.q_dim, self.kv_dim
@@ -939,14 +941,16 @@ class PRALlamaEngine:
     def generate(self, ids: torch.Tensor, lengths: torch.Tensor, max_new_tokens: int,
                  rules: LogitsRules | None = None) -> torch.Tensor:
         """Greedy decoding: ``[B, max_new_tokens]`` new token ids, each chosen after ``rules`` when given
-        (penalties see the row's prompt and what it has generated; a row whose rules leave nothing
+        (penalties see the row's prompt, a shared prefix in front of it, and what it has generated; a row whose rules leave nothing
         gives -1 and goes on with token 0)."""
         logits = self.prefill(ids, lengths, max_new_tokens)
         out = []
         if rules is None:
             tok = logits.float().argmax(-1)
         else:
-            history = TokenHistory.start(ids.to(self.device), lengths, max_new_tokens)
+            # (only repetition looks at what is not output: the walk over a long prefix is left out otherwise)
+            history = TokenHistory.start(ids.to(self.device), lengths, max_new_tokens,
+                                         self.prefix_ids if rules.repetition is not None else None)
             tok = choose_tokens(logits.contiguous(), rules, history, append=True)[0]
         for _ in range(max_new_tokens):
             out.append(tok)

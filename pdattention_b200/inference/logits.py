@@ -25,11 +25,16 @@ class TokenHistory:
     prompt_lengths: torch.Tensor | None = None
 
     @classmethod
-    def start(cls, prompts: torch.Tensor, lengths: torch.Tensor, new_tokens: int) -> "TokenHistory":
-        """History of left-aligned ``prompts`` ``[B, T]`` with room for ``new_tokens`` more."""
-        n = lengths.to(prompts.device, torch.int32).contiguous()
-        ids = torch.zeros((prompts.shape[0], prompts.shape[1] + new_tokens), dtype=torch.int32, device=prompts.device)
-        ids[:, : prompts.shape[1]] = prompts
+    def start(cls, prompts: torch.Tensor, lengths: torch.Tensor, new_tokens: int,
+              prefix: torch.Tensor | None = None) -> "TokenHistory":
+        """History of left-aligned ``prompts`` ``[B, T]`` with room for ``new_tokens`` more; ``prefix`` ``[P]``: a
+        prompt that every row has in front of its own."""
+        P = 0 if prefix is None else prefix.shape[0]
+        n = lengths.to(prompts.device, torch.int32).contiguous() + P
+        ids = torch.zeros((prompts.shape[0], P + prompts.shape[1] + new_tokens), dtype=torch.int32, device=prompts.device)
+        if P:
+            ids[:, :P] = prefix.to(prompts.device)
+        ids[:, P: P + prompts.shape[1]] = prompts
         return cls(ids, n.clone(), n)
 
     def append(self, tokens: torch.Tensor) -> None:

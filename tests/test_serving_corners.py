@@ -98,3 +98,15 @@ def test_angles_of_sequences_of_several_lengths():
         freq, _ = rotary_frequencies(8, 10000.0, scaling)
         assert torch.equal(rotary_angles(pos, 8, 10000.0, scaling, lengths[:, None])[0], pos.double()[..., None] * freq)
     assert torch.equal(rotary_angles(pos, 2, 10000.0, d, 300)[0][..., 0], pos.double())  # a single pair has no base
+
+
+def test_history_behind_a_shared_prefix():
+    from pdattention_b200.inference.logits import TokenHistory
+
+    h = TokenHistory.start(torch.tensor([[5, 6], [7, 0]]), torch.tensor([2, 1]), 1, torch.tensor([8, 9, 8]))
+    assert h.ids.tolist() == [[8, 9, 8, 5, 6, 0], [8, 9, 8, 7, 0, 0]]
+    assert h.lengths.tolist() == h.prompt_lengths.tolist() == [5, 4]
+    h.append(torch.tensor([1, 2]))
+    assert h.ids.tolist() == [[8, 9, 8, 5, 6, 1], [8, 9, 8, 7, 2, 0]] and h.prompt_lengths.tolist() == [5, 4]
+    alone = TokenHistory.start(torch.tensor([[5, 6]]), torch.tensor([2]), 1, torch.zeros(0, dtype=torch.long))
+    assert alone.ids.tolist() == [[5, 6, 0]] and alone.lengths.tolist() == [2]

@@ -281,3 +281,33 @@ def test_dynamic_scaling_past_the_window(prefix, memory, row_batch, monkeypatch)
             routing.step(b)
             close(got[b], reference_step(model, tok[b: b + 1], caches[b], ref_mem, ns)[0][-1], 0.99)
     engine.release_graph()
+
+
+def test_penalties_see_the_shared_prefix():
+    """Repetition that rules a token out for good: what the prefix says is not said again.  Every token is the best
+    of the engine's own logits after the penalties of prefix, prompt and output."""
+    from test_serving_engine_gpu import setup
+
+    from pdattention_b200.inference.logits import LogitsRules
+
+    cfg, model, engine = setup(9)
+    B, new, V = 2, 10, cfg.vocab_size
+    ids, n = torch.randint(0, V, (B, 7)), torch.tensor([7, 3])
+    engine.set_shared_prefix(torch.arange(0, 40))
+    logits = engine.prefill(ids, n, new)
+    prefix = torch.cat([torch.arange(0, 40), logits.float().topk(20, dim=-1).indices.flatten().cpu()])  # and the likeliest
+    engine.set_shared_prefix(prefix)
+    rules = LogitsRules(repetition=torch.full((B,), 1e30, device=DEV))
+    out = engine.generate(ids, n, new, rules=rules).cpu()
+    logits = engine.prefill(ids, n, new)
+    seen = [set(prefix.tolist()) | set(ids[b, : n[b]].tolist()) for b in range(B)]
+    for step in range(new):
+        z = logits.float().cpu()
+        for b in range(B):
+            said = torch.tensor(sorted(seen[b]))
+            z[b, said] = torch.where(z[b, said] > 0, z[b, said] / 1e30, z[b, said] * 1e30)
+            assert int(out[b, step]) == int(z[b].argmax()) and int(out[b, step]) not in seen[b]
+            seen[b].add(int(out[b, step]))
+        logits = engine.decode_step(out[:, step].to(DEV))
+    engine.set_shared_prefix(None)
+    assert engine.prefix_ids is None
