@@ -568,9 +568,8 @@ class PRALlamaEngine:
     def prefix_tokens(self) -> int:
         return 0 if self.prefix is None else self.prefix.shape[1]
 
-    def _prefix_kv(self, layer: int, end: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        rows = self.prefix[layer, : self.prefix_tokens if end is None else end]
-        return rows[:, : self.kv_dim], rows[:, self.kv_dim:]
+    def _prefix_kv(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
+        return self.prefix[layer, :, : self.kv_dim], self.prefix[layer, :, self.kv_dim:]
 
     @torch.no_grad()
     @traced("pra.llama.shared_prefix")
@@ -590,9 +589,9 @@ class PRALlamaEngine:
             raise ValueError("a shared prefix is one row of token ids")
         if cfg.head_dim not in (64, 128):
             raise ValueError("a shared prefix needs head dim 64 or 128")
-        self.prefix_ids = ids = ids.to(self.device, copy=True)
+        ids = ids.to(self.device, copy=True)
         P, qd, kd = ids.shape[0], self.q_dim, self.kv_dim
-        self.prefix = torch.empty((cfg.num_hidden_layers, P, 2 * kd), device=self.device, dtype=torch.bfloat16)
+        prefix = torch.empty((cfg.num_hidden_layers, P, 2 * kd), device=self.device, dtype=torch.bfloat16)
         if self.tp is not None:  # each row-parallel partial must fit the peer buffer
             chunk_tokens = max(1, min(chunk_tokens, self.tp.max_partial // cfg.hidden_size))
         for p0 in range(0, P, chunk_tokens):
@@ -603,15 +602,15 @@ class PRALlamaEngine:
             x = self._embed(ids[p0: p0 + n])
             for li, lw in enumerate(self.w.layers):
                 qkv = self._gemm(self._norm(x, self._ln(lw.ln_in)), lw.qkv, lw.qkv_bias)
-                k, v = self._prefix_kv(li)
+                k, v = prefix[li, :, :kd], prefix[li, :, kd:]
                 q = rotary_cache(qkv, self.heads, self.kv_heads, cfg.head_dim, pos, table, k, v, rows)
                 if li == len(self.w.layers) - 1:
                     break  # the last layer's output is never read
-                pk, pv = self._prefix_kv(li, p0)
-                a = shared_prefix_attention(q.view(1, n, qd), pk, pv, k[None, p0: p0 + n], v[None, p0: p0 + n], length,
-                                            self.heads, self.kv_heads, cfg.head_dim)
+                a = shared_prefix_attention(q.view(1, n, qd), k[:p0], v[:p0], k[None, p0: p0 + n], v[None, p0: p0 + n],
+                                            length, self.heads, self.kv_heads, cfg.head_dim)
                 x = self._row_parallel(a.view(n, qd), lw.o, x)
                 x = self._mlp(lw, x)
+        self.prefix, self.prefix_ids = prefix, ids  # only a whole one
 
     @torch.no_grad()
     @traced("pra.llama.prefill")

@@ -110,3 +110,41 @@ def test_history_behind_a_shared_prefix():
     assert h.ids.tolist() == [[8, 9, 8, 5, 6, 1], [8, 9, 8, 7, 2, 0]] and h.prompt_lengths.tolist() == [5, 4]
     alone = TokenHistory.start(torch.tensor([[5, 6]]), torch.tensor([2]), 1, torch.zeros(0, dtype=torch.long))
     assert alone.ids.tolist() == [[5, 6, 0]] and alone.lengths.tolist() == [2]
+
+
+def test_a_prefix_that_was_not_finished_is_none(monkeypatch):
+    """An exception while the second chunk is encoded: the engine has no prefix, not half of one."""
+    from types import SimpleNamespace
+
+    from pdattention_b200.inference import llama_engine
+    from pdattention_b200.models.llama import tiny_llama
+
+    engine = llama_engine.PRALlamaEngine.__new__(llama_engine.PRALlamaEngine)
+    cfg = tiny_llama(head_dim=64)
+    engine.cfg, engine.device, engine.tp = cfg, torch.device("cpu"), None
+    engine.heads, engine.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
+    engine.q_dim, engine.kv_dim = cfg.q_dim, cfg.kv_dim
+    engine.prefix = engine.prefix_ids = engine.cache = None
+    engine._rope_cache = {}
+    engine.w = SimpleNamespace(layers=[SimpleNamespace(ln_in=None, qkv=None, qkv_bias=None, o=None)] * cfg.num_hidden_layers)
+    calls = []
+
+    def rotary_cache(qkv, heads, kv_heads, head_dim, pos, table, k, v, rows):
+        calls.append(int(rows[0]))
+        if rows[0] >= 10:
+            raise torch.OutOfMemoryError("no room")
+        return qkv[:, : cfg.q_dim]
+
+    monkeypatch.setattr(llama_engine, "rotary_cache", rotary_cache)
+    monkeypatch.setattr(llama_engine, "shared_prefix_attention", lambda q, *a: q)
+    rows = lambda x, *a, **kw: torch.zeros(x.shape[0], cfg.q_dim + 2 * cfg.kv_dim)  # noqa: E731
+    for name in ("_norm", "_gemm", "_row_parallel", "_mlp"):
+        setattr(engine, name, (lambda x, *a, **kw: x) if name != "_gemm" else rows)
+    engine._mlp = lambda lw, x: x
+    engine._ln = lambda w: None
+    engine._embed = lambda ids: torch.zeros(ids.numel(), cfg.hidden_size)
+    with pytest.raises(torch.OutOfMemoryError):
+        engine.set_shared_prefix(torch.arange(25), chunk_tokens=10)
+    assert max(calls) == 10 and engine.prefix is None and engine.prefix_ids is None and engine.prefix_tokens == 0
+    engine.set_shared_prefix(torch.arange(9), chunk_tokens=10)
+    assert engine.prefix_tokens == 9 and engine.prefix_ids.tolist() == list(range(9))
