@@ -182,6 +182,11 @@ struct Rotary : torch::autograd::Function<Rotary> {
 
 std::vector<OptTensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& cos_t,
                               const Tensor& sin_t, bool interleaved, bool inverse) {
+  const auto dual = [](const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); };
+  TORCH_CHECK(!dual(q) && !(k.has_value() && dual(*k)) && !dual(cos_t) && !dual(sin_t),
+              "rotary has no forward-mode derivatives (the map is linear: rotate the tangents)");
+  TORCH_CHECK(!torch::GradMode::is_enabled() || !(cos_t.requires_grad() || sin_t.requires_grad()),
+              "rotary has no gradients for its table: detach cos and sin");
   if (!torch::GradMode::is_enabled() || !(q.requires_grad() || (k.has_value() && k->requires_grad())))
     return rotate(q, k, positions, cos_t, sin_t, interleaved, inverse);
   auto y = Rotary::apply(q, k, positions, cos_t, sin_t, interleaved, inverse);

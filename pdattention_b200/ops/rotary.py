@@ -139,7 +139,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, tab
     """``q`` ``[..., H, D]`` and ``k`` ``[..., Hkv, D]`` (bf16, fp16 or fp32; the same leading
     dimensions; strided views are read in place) rotated by ``positions`` ``[...]`` (int32 or
     int64).  Returns new contiguous tensors ``(q', k')`` (``k'`` is ``None`` without ``k``), with
-    gradients for ``q`` and ``k`` (of any order; a backward pass captured into a CUDA graph needs, as
+    gradients for ``q`` and ``k`` (of any order; none for the table and none in forward mode, which are
+    refused; a backward pass captured into a CUDA graph needs, as
     with every operator, that no eager graph of the same leaves is alive).  Elements behind
     ``table.rotary_dim`` pass through; a position outside the table gives NaN in the rotated part of its
     token."""

@@ -148,3 +148,28 @@ def test_a_prefix_that_was_not_finished_is_none(monkeypatch):
     assert max(calls) == 10 and engine.prefix is None and engine.prefix_ids is None and engine.prefix_tokens == 0
     engine.set_shared_prefix(torch.arange(9), chunk_tokens=10)
     assert engine.prefix_tokens == 9 and engine.prefix_ids.tolist() == list(range(9))
+
+
+@needs_ext
+def test_derivatives_that_rotary_does_not_have_are_refused():
+    import torch.autograd.forward_ad as fwad
+
+    from pdattention_b200.ops.rotary import RotaryTable, rotary, rotary_table
+
+    t = rotary_table(8, 4, device="cpu")
+    q, pos = torch.randn(3, 2, 8), torch.zeros(3, dtype=torch.long)
+    with fwad.dual_level():
+        dual = fwad.make_dual(q, torch.ones_like(q))
+        for args in ((dual, None), (q, dual), (dual.clone().requires_grad_(), None)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                rotary(*args, pos, t)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            rotary(q, None, pos, RotaryTable(fwad.make_dual(t.cos, t.cos), t.sin))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            rotary(dual, None, pos, t)
+    learned = RotaryTable(t.cos.clone().requires_grad_(), t.sin)
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="gradients for its table"):
+            rotary(x, None, pos, learned)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):  # without gradients any table serves
+        rotary(q, None, pos, learned)
