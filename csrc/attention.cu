@@ -143,7 +143,7 @@ __device__ __forceinline__ uint64_t drop_elem(const Params& p, int b, int h, int
   return (((uint64_t)b * p.H + h) * p.T + q) * p.T + t;
 }
 
-template <int D>
+template <int D, bool PARTS>
 __global__ void __launch_bounds__(NT) fwd_kernel(Params p) {
   constexpr int LD = Smem<D>::LD;
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -260,6 +260,17 @@ __global__ void __launch_bounds__(NT) fwd_kernel(Params p) {
     const int t = row_a + r * 8;
     if (t >= p.T) continue;
     const float inv = l_run[r] > 0.f ? 1.f / l_run[r] : 0.f;
+    if constexpr (PARTS) {
+      const int64_t at = ((int64_t)b * p.T + t) * p.H + h;
+#pragma unroll
+      for (int nb = 0; nb < D / 8; ++nb)
+        *reinterpret_cast<float2*>(p.part_o + at * D + nb * 8 + (lane & 3) * 2) =
+            make_float2(o_acc[nb][2 * r] * inv, o_acc[nb][2 * r + 1] * inv);
+      if ((lane & 3) == 0)
+        reinterpret_cast<float2*>(p.part_ml)[at] =
+            make_float2(l_run[r] > 0.f ? m_run[r] * p.scale + logf(l_run[r]) : -INFINITY, 1.f);
+      continue;
+    }
     __nv_bfloat16* dst = p.o + b * p.o_batch + t * p.o_row + h * D;
 #pragma unroll
     for (int nb = 0; nb < D / 8; ++nb) {
@@ -550,13 +561,13 @@ __global__ void __launch_bounds__(NT) bwd_dkdv_kernel(Params p) {
   }
 }
 
-template <int D>
+template <int D, bool PARTS = false>
 cudaError_t launch_fwd(const Params& p, cudaStream_t st) {
   constexpr int LD = Smem<D>::LD;
   const size_t smem = (size_t)(BM + 4 * BN) * LD * sizeof(__nv_bfloat16) + 2 * BN;
-  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(fwd_kernel<D>), (int)smem));
+  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(fwd_kernel<D, PARTS>), (int)smem));
   dim3 grid(p.H * p.B, (p.T + BM - 1) / BM);
-  fwd_kernel<D><<<grid, NT, smem, st>>>(p);
+  fwd_kernel<D, PARTS><<<grid, NT, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -614,6 +625,10 @@ cudaError_t pra_attention_fwd(const AttnParams& p, int head_dim, cudaStream_t st
   if (g_attn_tcgen05 && (p.T > 64 || head_dim == 64) && p.drop_thresh == 0) {
     const cudaError_t e = pra_attention_fwd_tc(p, head_dim, st);
     if (e != cudaErrorNotSupported) return e;
+  }
+  if (p.part_o != nullptr) {
+    if (head_dim == 64) return launch_fwd<64, true>(p, st);
+    return head_dim == 128 ? launch_fwd<128, true>(p, st) : cudaErrorInvalidValue;
   }
   switch (head_dim) {
     case 16: return launch_fwd<16>(p, st);

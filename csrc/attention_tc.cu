@@ -178,7 +178,17 @@ __device__ __forceinline__ void load_query_rows(uint8_t* tile, const __nv_bfloat
   }
 }
 
-template <int D>
+// 32 columns of a query's part.
+__device__ __forceinline__ void store_part(float* dst, const uint32_t (&r)[32], float inv) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4)
+    *reinterpret_cast<float4*>(dst + i) =
+        make_float4(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv, __uint_as_float(r[i + 2]) * inv,
+                    __uint_as_float(r[i + 3]) * inv);
+}
+
+// PARTS: the result goes to p.part_o / p.part_ml (instantiations of their own: the others stay as they are).
+template <int D, bool PARTS>
 __global__ void __launch_bounds__(NT, 2) fwd_kernel(AttnParams p) {
   using C = Cfg<D>;
   constexpr int BN = C::BN, HB = C::HB, HD = C::HD;
@@ -394,7 +404,9 @@ __global__ void __launch_bounds__(NT, 2) fwd_kernel(AttnParams p) {
     for (int c0 = 0; c0 < HD; c0 += 32) {
       uint32_t r[32];
       tc::ld32(t_o + c0, r);
-      if (q < p.T) {
+      if constexpr (PARTS) {
+        if (q < p.T) store_part(p.part_o + (((int64_t)b * p.T + q) * p.H + h) * D + half * HD + c0, r, inv);
+      } else if (q < p.T) {
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           uint4 w;
@@ -406,8 +418,11 @@ __global__ void __launch_bounds__(NT, 2) fwd_kernel(AttnParams p) {
         }
       }
     }
-    if (q < p.T && half == 0)
-      p.lse[((int64_t)b * p.H + h) * p.T + q] = l_tot > 0.f ? m_run * p.scale + logf(l_tot) : -INFINITY;
+    if (q < p.T && half == 0) {
+      const float lse = l_tot > 0.f ? m_run * p.scale + logf(l_tot) : -INFINITY;
+      if constexpr (PARTS) reinterpret_cast<float2*>(p.part_ml)[((int64_t)b * p.T + q) * p.H + h] = make_float2(lse, 1.f);
+      else p.lse[((int64_t)b * p.H + h) * p.T + q] = lse;
+    }
   } else {
     // Stop: record the failure, give the MMAs in flight a bounded time to finish, free TMEM.
     if (tid == 0 && p.status != nullptr) atomicExch(p.status, 1);
@@ -845,6 +860,7 @@ struct PackCfg {
   static constexpr int O_COL = BN, P_COL = BN + D;  // as Cfg<64>
 };
 
+template <bool PARTS>
 __global__ void __launch_bounds__(NT, 2) fwd_packed_kernel(AttnParams p) {
   using C = PackCfg;
   constexpr int D = C::D, BN = C::BN, KB = C::KB, HB = C::HB;
@@ -1073,7 +1089,15 @@ __global__ void __launch_bounds__(NT, 2) fwd_packed_kernel(AttnParams p) {
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
     uint32_t o[32];
     tc::ld32(t_o, o);
-    if (row_seq && t < p.T) {
+    if constexpr (PARTS) {
+      if (row_seq && t < p.T) {
+        const int64_t at = ((int64_t)b * p.T + t) * p.H + h;
+        store_part(p.part_o + at * D + half * (D / 2), o, inv);
+        if (half == 0)
+          reinterpret_cast<float2*>(p.part_ml)[at] =
+              make_float2(l_tot > 0.f ? m_run * p.scale + logf(l_tot) : -INFINITY, 1.f);
+      }
+    } else if (row_seq && t < p.T) {
       __nv_bfloat16* dst = p.o + b * p.o_batch + (int64_t)t * p.o_row + h * D + half * (D / 2);
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
@@ -1100,12 +1124,12 @@ __global__ void __launch_bounds__(NT, 2) fwd_packed_kernel(AttnParams p) {
   }
 }
 
-template <int D>
+template <int D, bool PARTS>
 cudaError_t launch(const AttnParams& p, cudaStream_t st) {
   constexpr int smem = Cfg<D>::SMEM;
-  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(fwd_kernel<D>), smem));
+  PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(fwd_kernel<D, PARTS>), smem));
   dim3 grid(p.H * p.B, (p.T + BM - 1) / BM);
-  fwd_kernel<D><<<grid, NT, smem, st>>>(p);
+  fwd_kernel<D, PARTS><<<grid, NT, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -1164,14 +1188,15 @@ cudaError_t pra_attention_fwd_tc(const AttnParams& p, int head_dim, cudaStream_t
     return cudaErrorNotSupported;
   if (head_dim == 64 && p.T <= 64) {  // two sequences per 128-query tile
     constexpr int smem = PackCfg::SMEM;
-    PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(fwd_packed_kernel), smem));
+    auto kernel = p.part_o != nullptr ? fwd_packed_kernel<true> : fwd_packed_kernel<false>;
+    PRA_RETURN_IF_ERROR(pra::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
     dim3 grid(p.H, (p.B + 1) / 2);
-    fwd_packed_kernel<<<grid, NT, smem, st>>>(p);
+    kernel<<<grid, NT, smem, st>>>(p);
     return cudaGetLastError();
   }
   switch (head_dim) {
-    case 64: return launch<64>(p, st);
-    case 128: return launch<128>(p, st);
+    case 64: return p.part_o != nullptr ? launch<64, true>(p, st) : launch<64, false>(p, st);
+    case 128: return p.part_o != nullptr ? launch<128, true>(p, st) : launch<128, false>(p, st);
     default: return cudaErrorNotSupported;
   }
 }

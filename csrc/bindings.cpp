@@ -153,6 +153,24 @@ std::vector<torch::Tensor> attention_fwd(torch::Tensor q, torch::Tensor k, torch
   return {out, lse};
 }
 
+// The same attention as one part of a larger softmax, unrounded: {o [B * T, H, 1, D] fp32, (max, sum) [B * T, H, 1, 2]}.
+std::vector<torch::Tensor> attention_partials(torch::Tensor q, torch::Tensor k, torch::Tensor v, int64_t heads,
+                                              int64_t kv_heads, int64_t head_dim, c10::optional<torch::Tensor> mem_k,
+                                              c10::optional<torch::Tensor> mem_v, c10::optional<torch::Tensor> mem_idx,
+                                              c10::optional<torch::Tensor> mem_len,
+                                              c10::optional<torch::Tensor> key_valid, double scale) {
+  c10::cuda::CUDAGuard guard(q.device());
+  TORCH_CHECK(head_dim == 64 || head_dim == 128, "partials need head dim 64 or 128");
+  auto p = attn_params(q, k, v, heads, kv_heads, mem_k, mem_v, mem_idx, mem_len, key_valid, scale);
+  const auto fp32 = q.options().dtype(at::kFloat);
+  auto o = torch::empty({(int64_t)p.B * p.T, heads, 1, head_dim}, fp32);
+  auto ml = torch::empty({(int64_t)p.B * p.T, heads, 1, 2}, fp32);
+  p.part_o = ptr<float>(o);
+  p.part_ml = ptr<float>(ml);
+  check(pra_attention_fwd(p, (int)head_dim, stream()), "attention_partials");
+  return {o, ml};
+}
+
 std::vector<torch::Tensor> attention_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
                                          torch::Tensor out, torch::Tensor lse, int64_t heads, int64_t head_dim,
                                          c10::optional<torch::Tensor> mem_k, c10::optional<torch::Tensor> mem_v,
@@ -1585,6 +1603,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kv_heads"), py::arg("head_dim"), py::arg("mem_k"), py::arg("mem_v"), py::arg("mem_idx"),
         py::arg("mem_len"), py::arg("key_valid"), py::arg("scale"), py::arg("drop_p") = 0.0,
         py::arg("drop_seed") = 0, py::arg("drop_offset") = 0);
+  m.def("attention_partials", &attention_partials);
   m.def("dropout", &dropout);
   m.def("dropout_add", &dropout_add);
   m.def("attention_status", [](int64_t device) { return attention_status_buffer(torch::Device(torch::kCUDA, device)); });

@@ -13,6 +13,11 @@ struct AttnParams {
   const __nv_bfloat16* v;
   __nv_bfloat16* o;
   float* lse;                  // [B, H, T] natural-log LSE of the scaled scores
+  // A forward whose result is one part of a larger softmax, in fp32 for the join: instead of o and lse the
+  // normalised output [B * T, H, D] and (lse, 1) pairs [B * T, H, 2] ((-inf, 1): nothing visible); or null.
+  // Head dims 64 and 128.
+  float* part_o;
+  float* part_ml;
   const __nv_bfloat16* mem_k;  // pool rows [tokens, Hkv * D]
   const __nv_bfloat16* mem_v;
   const int* mem_idx;          // [B, mem_max] pool row of each memory key

@@ -680,10 +680,8 @@ class PRALlamaEngine:
                 a = shared_prefix_attention(q, *self._prefix_kv(li), k_rows, v_rows, full, *heads)
             else:  # the routed memory on its own (no local key is valid), joined with [prefix ; local]
                 parts = shared_prefix_partials(q, *self._prefix_kv(li), k_rows, v_rows, full, *heads)
-                o, lse = ext.attention_fwd(q, k_rows, v_rows, *heads, *mem_args, torch.zeros_like(valid),
-                                           1.0 / math.sqrt(cfg.head_dim))[:2]
-                lse = lse.transpose(1, 2).reshape(M, self.heads, 1)
-                more = (o.view(M, self.heads, 1, cfg.head_dim).float(), torch.stack([lse, torch.ones_like(lse)], -1))
+                more = ext.attention_partials(q, k_rows, v_rows, *heads, *mem_args, torch.zeros_like(valid),
+                                              1.0 / math.sqrt(cfg.head_dim))
                 a = merge_attention_partials(parts, more, batch=B)
             x = self._row_parallel(a.view(M, qd), lw.o, x)
             x = self._mlp(lw, x)

@@ -9,6 +9,7 @@ from test_serving_ops_gpu import half_step, prefix64, prefix_close, rotary_close
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+NEG_INF = float("-inf")
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -311,3 +312,62 @@ def test_penalties_see_the_shared_prefix():
         logits = engine.decode_step(out[:, step].to(DEV))
     engine.set_shared_prefix(None)
     assert engine.prefix_ids is None
+
+
+@pytest.mark.parametrize("impl", ["tcgen05", "mma"])
+@pytest.mark.parametrize("T,H,Hkv,D", [(3, 4, 2, 64), (64, 8, 2, 64), (65, 8, 8, 64), (300, 4, 1, 64), (5, 8, 2, 128), (200, 8, 2, 128)])
+def test_attention_over_memory_as_an_unrounded_part(impl, T, H, Hkv, D):
+    """Alone it joins to attention_fwd's own bits; beside another part nothing is rounded before the join."""
+    from pdattention_b200.inference.shared_prefix import merge_attention_partials
+    from pdattention_b200.ops import _ext
+
+    torch.manual_seed(T)
+    ext, B, w, n = _ext.require(), 3, Hkv * D, 70
+    q = torch.randn(B, T, H * D, device=DEV).bfloat16()
+    k, v = torch.randn(2, B, T, w, device=DEV).bfloat16()
+    pool = torch.randn(500, 2 * w, device=DEV).bfloat16()
+    idx = torch.randint(0, 500, (B, n), device=DEV, dtype=torch.int32)
+    mem_len = torch.tensor([n, 0, 33], dtype=torch.int32, device=DEV)
+    valid = torch.zeros(B, T, dtype=torch.uint8, device=DEV)  # the memory only
+    args = (q, k, v, H, Hkv, D, pool[:, :w], pool[:, w:], idx, mem_len, valid, 1 / math.sqrt(D))
+    ext.set_attention_impl(impl)
+    try:
+        o, ml = ext.attention_partials(*args)
+        out, lse = ext.attention_fwd(*args)
+    finally:
+        ext.set_attention_impl("tcgen05")
+    assert o.shape == (B * T, H, 1, D) and ml.shape == (B * T, H, 1, 2) and (ml[..., 1] == 1).all()
+    alone, alone_lse = merge_attention_partials((o, ml), batch=B, return_lse=True)
+    assert torch.equal(alone, out) and torch.equal(alone_lse, lse)
+    assert (lse[1] == NEG_INF).all() and (out[1] == 0).all()
+    o = o.view(B, T, H, D)
+    seen = o[0::2]
+    assert (seen.bfloat16().float() != seen).float().mean() > 0.9  # fp32 values
+    keys = [pool[idx[b, : int(mem_len[b])].long()].double().view(-1, 2, Hkv, D).repeat_interleave(H // Hkv, 2) for b in (0, 2)]
+    for b, kv in zip((0, 2), keys):
+        x = q[b].double().view(T, H, D)
+        s = torch.einsum("thd,nhd->htn", x, kv[:, 0]) / math.sqrt(D)
+        p = torch.softmax(s, -1)
+        want, mass = torch.einsum("htn,nhd->thd", p, kv[:, 1]), torch.einsum("htn,nhd->thd", p, kv[:, 1].abs())
+        size = torch.einsum("thd,nhd->htn", x.abs(), kv[:, 0].abs()).amax() / math.sqrt(D)
+        slack = D * 2.0 ** -24 * size + 2.0 ** -20 * (1 + size + torch.logsumexp(s, -1).abs().amax())
+        # every weight half a step of bf16 and the score's error; no rounding of the result
+        assert ((o[b].double() - want).abs() <= (half_step(torch.bfloat16) + 2 * slack) * mass).all()
+
+
+def test_a_prefill_joins_its_memory_unrounded(monkeypatch):
+    from test_serving_engine_gpu import setup
+
+    from pdattention_b200.inference import llama_engine
+
+    cfg, model, engine = setup(10)
+    engine.build_memory(torch.randint(0, cfg.vocab_size, (12, 16)), torch.full((12,), 16, dtype=torch.int32))
+    engine.set_namespace(torch.zeros(2, dtype=torch.int32), torch.full((2,), 12, dtype=torch.int32))
+    engine.set_shared_prefix(torch.arange(30))
+    parts = []
+    join = llama_engine.merge_attention_partials
+    monkeypatch.setattr(llama_engine, "merge_attention_partials", lambda a, b, **kw: (parts.append(b[0]), join(a, b, **kw))[1])
+    engine.prefill(torch.randint(0, cfg.vocab_size, (2, 9)), torch.tensor([9, 4]), 2)
+    assert len(parts) == cfg.num_hidden_layers
+    for o in parts:
+        assert o.dtype == torch.float32 and (o.bfloat16().float() != o).float().mean() > 0.9
