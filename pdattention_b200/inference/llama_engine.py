@@ -32,7 +32,7 @@ from ..models.llama import PRALlamaConfig, PRALlamaReference
 from ..ops import _ext
 from ..ops.rotary import RotaryTable, dynamic_window, rotary_angles, rotary_cache
 from ..tracing import traced
-from .logits import LogitsRules, TokenHistory, choose_tokens
+from .logits import LogitsRules, TokenHistory, choose_tokens, join_choices
 from .routing import select_chunks
 from .shared_prefix import merge_attention_partials, shared_prefix_attention, shared_prefix_partials
 
@@ -794,9 +794,7 @@ class PRALlamaEngine:
             return choose_tokens(local, rules, history, append=history is not None)[0]
         token, value = choose_tokens(local, rules, history, vocab_start=self.vocab_start)
         every = self.tp.gather_small(torch.stack([value, token.float()], dim=1)).view(-1, self.tp_size, 2)
-        score, ids = every[..., 0].nan_to_num(nan=float("inf"), posinf=float("inf"), neginf=float("-inf")), every[..., 1]
-        top = score.max(dim=1, keepdim=True).values
-        token = torch.where(score == top, ids, torch.full_like(ids, float("inf"))).min(dim=1).values.long()
+        token = join_choices(every[..., 0], every[..., 1])
         if history is not None:
             history.append(token)
         return token

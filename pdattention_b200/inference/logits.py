@@ -86,6 +86,16 @@ def process_logits(logits: torch.Tensor, rules: LogitsRules, history: TokenHisto
                                     rules.bias_ids, rules.bias_values, rules.mask, rules.mask_rows, vocab_start)
 
 
+def join_choices(values: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
+    """Tokens ``[B]`` int64 over the whole vocabulary from the choices of its slices (``choose_tokens``): processed
+    logits ``values`` and ids ``tokens`` ``[B, slices]``.  As within a slice: NaN is the largest, ties go to the
+    lowest id, -1 where no slice has anything."""
+    nan = values.isnan()
+    score = values.masked_fill(nan.any(1, keepdim=True), float("-inf")).masked_fill(nan, 0.0)
+    worse = score < score.amax(1, keepdim=True)
+    return tokens.double().masked_fill(worse, float("inf")).amin(1).long()
+
+
 def choose_tokens(logits: torch.Tensor, rules: LogitsRules, history: TokenHistory | None = None, *,
                   vocab_start: int = 0, append: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """Greedy token of each row after the rules: ``(ids [B] int64, their processed logits [B] fp32)``.

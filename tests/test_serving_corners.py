@@ -173,3 +173,78 @@ def test_derivatives_that_rotary_does_not_have_are_refused():
             rotary(x, None, pos, learned)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):  # without gradients any table serves
         rotary(q, None, pos, learned)
+
+
+def test_choices_of_vocabulary_slices_are_joined():
+    from pdattention_b200.inference.logits import join_choices
+
+    nan, inf = float("nan"), float("inf")
+    cases = [  # (value, id) of each slice: the choice over all of them
+        ([(1.0, 3), (2.0, 40), (0.5, 99)], 40),
+        ([(2.0, 3), (2.0, 40), (2.0, 99)], 3),        # ties: the lowest id
+        ([(-inf, -1), (-5.0, 40), (-inf, -1)], 40),   # slices with nothing left
+        ([(-inf, -1), (-inf, -1), (-inf, -1)], -1),
+        ([(inf, 3), (nan, 40), (1.0, 99)], 40),       # NaN is larger than +inf
+        ([(nan, 17), (inf, 40), (nan, 99)], 17),
+        ([(inf, 3), (inf, 40), (-inf, -1)], 3),
+        ([(-0.0, 7), (0.0, 40), (-1.0, 99)], 7),      # -0 counts as 0
+        ([(-3.4e38, 7), (-inf, -1), (-3.4e38, 393215)], 7),
+    ]
+    values = torch.tensor([[v for v, _ in c] for c, _ in cases])
+    tokens = torch.tensor([[t for _, t in c] for c, _ in cases])
+    for ids in (tokens, tokens.float()):  # ids travel as fp32, exact under 2^24
+        got = join_choices(values, ids)
+        assert got.dtype == torch.int64 and got.tolist() == [t for _, t in cases]
+
+
+def test_tensor_parallel_ranks_choose_alike(monkeypatch):
+    """``_choose`` of two ranks (each with half of the columns) gives what one rank with all of them gives, and the
+    same histories.  The kernel's place is taken by the operator's definition."""
+    from types import SimpleNamespace
+
+    from pdattention_b200.inference import llama_engine
+    from pdattention_b200.inference.logits import LogitsRules, TokenHistory
+
+    torch.manual_seed(0)
+    B, V = 6, 32
+    logits = torch.randn(B, V)
+    logits[1, 20] = logits[1].amax() + 1
+    logits[1, 5] = logits[1, 20]            # a tie across the ranks
+    logits[2] = float("-inf")               # nothing left
+    logits[3, 3], logits[3, 30] = float("inf"), float("nan")
+    logits[4, 16:] = float("-inf")          # one rank with nothing left
+
+    def choose(local, rules, history, vocab_start=0, append=False):
+        key = torch.where(local.isnan(), float("inf"), local)
+        key = torch.where(local.isnan().any(1, keepdim=True) & ~local.isnan(), float("-inf"), key)
+        value, at = key.max(1)
+        value = local.gather(1, at[:, None])[:, 0]
+        token = torch.where(value == float("-inf"), -1, at + vocab_start)
+        if append:
+            history.append(token)
+        return token, value
+
+    monkeypatch.setattr(llama_engine, "choose_tokens", choose)
+
+    def engine(start, tp, size):
+        e = llama_engine.PRALlamaEngine.__new__(llama_engine.PRALlamaEngine)
+        e.vocab_start, e.tp, e.tp_size = start, tp, size
+        return e
+
+    fresh = lambda: TokenHistory(torch.zeros(B, 3, dtype=torch.int32), torch.tensor([0, 1, 2, 0, 3, 0], dtype=torch.int32))  # noqa: E731
+    rules, want_history = LogitsRules(), fresh()
+    want = engine(0, None, 1)._choose(logits, rules, want_history)
+    assert want[1:5].tolist() == [5, -1, 30, int(logits[4].argmax())]
+    pairs = []
+    for half in range(2):
+        part = logits[:, half * 16: half * 16 + 16]
+        token, value = choose(part, rules, None, vocab_start=half * 16)
+        pairs.append(torch.stack([value, token.float()], 1))
+    for half in range(2):
+        sent = []
+        tp = SimpleNamespace(gather_small=lambda x: (sent.append(x), torch.cat(pairs, 1))[1])
+        history = fresh()
+        got = engine(half * 16, tp, 2)._choose(logits[:, half * 16: half * 16 + 16], rules, history)
+        assert torch.equal(got, want) and got.dtype == want.dtype
+        assert torch.equal(sent[0].nan_to_num(nan=7.0), pairs[half].nan_to_num(nan=7.0))
+        assert torch.equal(history.ids, want_history.ids) and torch.equal(history.lengths, want_history.lengths)
