@@ -728,7 +728,11 @@ class PRALlamaEngine:
         ``sample=True`` the greedy next token ids ``[B]`` (no full-vocabulary logits are formed
         under tensor parallelism).  With ``rules`` the choice is made after them, -1 where they
         leave a row nothing, and joins ``history`` (which begins with ``prefix_ids`` behind a shared prefix:
-        ``TokenHistory.start``)."""
+        ``TokenHistory.start``); both are for choices, so ``rules`` need ``sample`` and a history rules."""
+        if rules is not None and not sample:
+            raise ValueError("rules choose a token: they need sample=True (process_logits serves a sampler of its own)")
+        if history is not None and rules is None:
+            raise ValueError("a history without rules would not be appended to (LogitsRules() has none)")
         cfg, ext = self.cfg, self.ext
         B = token_ids.shape[0]
         qd, kd = self.q_dim, self.kv_dim
@@ -936,8 +940,8 @@ class PRALlamaEngine:
     def generate(self, ids: torch.Tensor, lengths: torch.Tensor, max_new_tokens: int,
                  rules: LogitsRules | None = None) -> torch.Tensor:
         """Greedy decoding: ``[B, max_new_tokens]`` new token ids, each chosen after ``rules`` when given
-        (penalties see the row's prompt, a shared prefix in front of it, and what it has generated; a row whose rules leave nothing
-        gives -1 and goes on with token 0)."""
+        (penalties see the row's prompt, a shared prefix in front of it, and what it has generated; a row
+        whose rules leave nothing gives -1 and goes on with token 0)."""
         logits = self.prefill(ids, lengths, max_new_tokens)
         out = []
         if rules is None:

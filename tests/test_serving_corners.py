@@ -248,3 +248,15 @@ def test_tensor_parallel_ranks_choose_alike(monkeypatch):
         assert torch.equal(got, want) and got.dtype == want.dtype
         assert torch.equal(sent[0].nan_to_num(nan=7.0), pairs[half].nan_to_num(nan=7.0))
         assert torch.equal(history.ids, want_history.ids) and torch.equal(history.lengths, want_history.lengths)
+
+
+def test_rules_and_histories_that_a_step_would_ignore_are_refused():
+    from pdattention_b200.inference.llama_engine import PRALlamaEngine
+    from pdattention_b200.inference.logits import LogitsRules, TokenHistory
+
+    engine = PRALlamaEngine.__new__(PRALlamaEngine)
+    history = TokenHistory(torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="sample=True"):
+        engine.decode_step(torch.zeros(1, dtype=torch.long), rules=LogitsRules())
+    with pytest.raises(ValueError, match="history without rules"):
+        engine.decode_step(torch.zeros(1, dtype=torch.long), sample=True, history=history)
