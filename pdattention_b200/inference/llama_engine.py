@@ -729,10 +729,7 @@ class PRALlamaEngine:
         under tensor parallelism).  With ``rules`` the choice is made after them, -1 where they
         leave a row nothing, and joins ``history`` (which begins with ``prefix_ids`` behind a shared prefix:
         ``TokenHistory.start``); both are for choices, so ``rules`` need ``sample`` and a history rules."""
-        if rules is not None and not sample:
-            raise ValueError("rules choose a token: they need sample=True (process_logits serves a sampler of its own)")
-        if history is not None and rules is None:
-            raise ValueError("a history without rules would not be appended to (LogitsRules() has none)")
+        self._check_choice(sample, rules, history)
         cfg, ext = self.cfg, self.ext
         B = token_ids.shape[0]
         qd, kd = self.q_dim, self.kv_dim
@@ -790,6 +787,13 @@ class PRALlamaEngine:
         if not sample:
             return self._logits(x)
         return self._greedy(x) if rules is None else self._choose(self._local_logits(x), rules, history)
+
+    @staticmethod
+    def _check_choice(sample: bool, rules: LogitsRules | None, history: TokenHistory | None) -> None:
+        if rules is not None and not sample:
+            raise ValueError("rules choose a token: they need sample=True (process_logits serves a sampler of its own)")
+        if history is not None and rules is None:
+            raise ValueError("a history without rules would not be appended to (LogitsRules() has none)")
 
     def _choose(self, local: torch.Tensor, rules: LogitsRules, history: TokenHistory | None) -> torch.Tensor:
         """Greedy tokens after ``rules`` from this rank's vocabulary slice of the logits, merged
@@ -903,6 +907,7 @@ class PRALlamaEngine:
         Replays run the whole step (32 layers of GEMMs, routing, attention and the
         tensor-parallel collectives) as one graph launch; the collectives take their
         epochs from device counters, so replays stay in lockstep across ranks."""
+        self._check_choice(sample, rules, history)  # before the capture begins
         B = self.cache_len.shape[0]
         self._graph_ids = torch.zeros(B, dtype=torch.long, device=self.device)
         ar0 = self.tp.epoch_ar if self.tp is not None else 0

@@ -260,3 +260,5 @@ def test_rules_and_histories_that_a_step_would_ignore_are_refused():
         engine.decode_step(torch.zeros(1, dtype=torch.long), rules=LogitsRules())
     with pytest.raises(ValueError, match="history without rules"):
         engine.decode_step(torch.zeros(1, dtype=torch.long), sample=True, history=history)
+    with pytest.raises(ValueError, match="sample=True"):
+        engine.capture_decode(rules=LogitsRules())
