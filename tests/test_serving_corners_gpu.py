@@ -371,3 +371,52 @@ def test_a_prefill_joins_its_memory_unrounded(monkeypatch):
     assert len(parts) == cfg.num_hidden_layers
     for o in parts:
         assert o.dtype == torch.float32 and (o.bfloat16().float() != o).float().mean() > 0.9
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens,heads,kv,dim,rot,interleaved", [(1, 8, 2, 64, 64, False), (77, 5, 1, 128, 64, True), (700, 4, 4, 80, 20, False),
+                                                                 (9, 3, 3, 6, 2, True), (16, 0, 2, 64, 64, False)])
+def test_rotary_cache_of_other_types(dtype, tokens, heads, kv, dim, rot, interleaved):
+    from pdattention_b200.ops.rotary import rotary_cache, rotary_table
+
+    torch.manual_seed(tokens)
+    qkv = torch.randn(tokens, (heads + 2 * kv) * dim + 3, device=DEV).to(dtype)[:, : (heads + 2 * kv) * dim]
+    pos = torch.randint(0, 1000, (tokens,), device=DEV)
+    table = rotary_table(rot, 1000, interleaved=interleaved)
+    rows = tokens + 20
+    slots = torch.randperm(rows, device=DEV)[:tokens].int()
+    if tokens > 2:
+        slots[1], slots[2] = -1, rows  # not written
+    kc, vc = torch.full((2, rows, kv * dim), 7.0, device=DEV, dtype=dtype)
+    q = rotary_cache(qkv, heads, kv, dim, pos, table, kc, vc, slots)
+    x = qkv.reshape(tokens, heads + 2 * kv, dim)
+    want = rotate64(x, pos, table)
+    if heads:
+        rotary_close(q.view(tokens, heads, dim), want[:, :heads], x[:, :heads], rot)
+    kept = (slots >= 0) & (slots < rows)
+    at = slots[kept].long()
+    rotary_close(kc[at].view(-1, kv, dim), want[kept, heads: heads + kv], x[kept, heads: heads + kv], rot)
+    assert torch.equal(vc[at], x[kept, heads + kv:].flatten(1))
+    rest = torch.ones(rows, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert (kc[rest] == 7).all() and (vc[rest] == 7).all()
+
+
+@pytest.mark.parametrize("B,T,P,H,Hkv,D", [(64, 1, 8192, 32, 8, 128), (16, 4, 4096, 32, 8, 128), (8, 5, 700, 12, 12, 64),
+                                           (16, 16, 300, 4, 4, 128), (3, 60, 500, 8, 2, 64)])
+@pytest.mark.parametrize("cap", [4096, 16384])
+def test_capacities_far_above_the_lengths(B, T, P, H, Hkv, D, cap):
+    """The rows of an engine's cache: room for many tokens more, whatever is in it."""
+    from pdattention_b200.inference.shared_prefix import shared_prefix_attention
+
+    torch.manual_seed(cap + B)
+    w = Hkv * D
+    q = (1.5 * torch.randn(B, T, H * D, device=DEV)).bfloat16()
+    pk, pv = torch.randn(2, P, w, device=DEV).bfloat16()
+    lengths = torch.randint(T, 150, (B,), device=DEV, dtype=torch.int32)
+    k, v = torch.full((2, B, cap, w), float("nan"), device=DEV, dtype=torch.bfloat16)
+    for b in range(B):
+        n = int(lengths[b])
+        k[b, :n], v[b, :n] = torch.randn(2, n, w, device=DEV).bfloat16()
+    out, lse = shared_prefix_attention(q, pk, pv, k, v, lengths, H, Hkv, D, return_lse=True)
+    prefix_close(out, lse, prefix64(q, pk, pv, k[:, :150], v[:, :150], lengths, None, H, Hkv, D, 1 / math.sqrt(D)), D)
