@@ -618,7 +618,10 @@ class PRALlamaEngine:
                 row_batch: int | None = None, position_offset: torch.Tensor | None = None) -> torch.Tensor:
         """Left-aligned prompts ``ids`` ``[B, T]`` with ``lengths``: fills the local caches and
         returns the logits of each row's last prompt token ``[B, V]``.  ``row_batch`` bounds
-        how many rows run through the layers at once (activation memory)."""
+        how many rows run through the layers at once (activation memory).  Behind a shared prefix, too,
+        every row has a token of its own: the prefix's last one yields no logits."""
+        if self.prefix is not None and lengths.numel() and int(lengths.min()) < 1:
+            raise ValueError("behind a shared prefix every row needs at least one token of its own")
         cfg = self.cfg
         B, T = ids.shape
         ids = ids.to(self.device)

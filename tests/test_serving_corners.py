@@ -262,3 +262,14 @@ def test_rules_and_histories_that_a_step_would_ignore_are_refused():
         engine.decode_step(torch.zeros(1, dtype=torch.long), sample=True, history=history)
     with pytest.raises(ValueError, match="sample=True"):
         engine.capture_decode(rules=LogitsRules())
+
+
+def test_rows_of_nothing_but_the_prefix_are_refused():
+    from pdattention_b200.inference.llama_engine import PRALlamaEngine
+    from pdattention_b200.models.llama import tiny_llama
+
+    engine = PRALlamaEngine.__new__(PRALlamaEngine)
+    engine.cfg, engine.prefix = tiny_llama(), torch.zeros(2, 5, 8)
+    for ids, n in ((torch.zeros(3, 4), [4, 0, 1]), (torch.zeros(1, 0), [0]), (torch.zeros(2, 1), [1, -1])):
+        with pytest.raises(ValueError, match="token of its own"):
+            engine.prefill(ids.long(), torch.tensor(n), 4)
