@@ -11,9 +11,9 @@
 // depend on the compiler.  The greedy token is the lowest id of the largest z; NaN counts as the
 // largest; a row with nothing above -inf gives -1.
 //
-// Bound by bytes: each logit is read once (and written once), the history read once.  A cluster of
-// 1 to 8 CTAs owns a row, one slice of the vocabulary each.  The history cannot be looked up per logit,
-// so each CTA turns its slice of it around in shared memory: a bit per token that the history or a
+// Each logit is read once (and written once), the history by each CTA of its row, once or twice.  A
+// cluster of 1 to 8 CTAs owns a row, one slice of the vocabulary each.  The history cannot be looked up
+// per logit, so each CTA turns its slice of it around in shared memory: a bit per token that the history or a
 // bias names (their ranks by a prefix sum of the bits), and for each such token its id and a word with
 // its occurrences (bits 0-19 output count, bit 20 seen, bits 21-31 2,047 less its first bias entry, or
 // 0).  Integer atomics fill them, so any order gives the same table; a token's first bias entry sums all
@@ -24,11 +24,12 @@
 // thread (half of the warps at them while the others are at all logits: no shorter).  Where the history
 // may name half of a slice, a word per token takes no more room and the history is walked once instead
 // of twice (64 rows of 128,256 logits with 100,000 ids each: 368 -> 136 us).  256 rows of 152,064 bf16
-// logits with 8,192 ids each take 40 us (17 without a history, 12.6 is what their bytes need): the two
-// walks and the scattered logits of the named tokens wait for memory, one after the other.  (Looking the
-// penalties up within the pass over all logits took 107 us, a word per token of the slice instead of the
-// table 183 us.)  A thread only remembers which vector held its maximum: the element is looked up at the
-// end, by the warps' winners.  A thread's first logits and mask bytes are loaded before the table is built.
+// logits with 8,192 ids each take 41 us (16 without a history, 13.9 is what their bytes need; written back
+// 69, 29 and 25.8), one row of 128,256 with 512 ids 10.4, with 16,384 23.5: the two walks and the scattered
+// logits of the named tokens wait for memory, one after the other.  (Looking the penalties up within the
+// pass over all logits took 107 us, a word per token of the slice instead of the table 183 us.)  A thread
+// only remembers which vector held its maximum: the element is looked up at the end, by the warps' winners.
+// A thread's first logits and mask bytes are loaded before the table is built.
 #include <algorithm>
 #include <type_traits>
 

@@ -22,8 +22,8 @@
 //
 // What bounds it: a tile's chain of about 3,200 cycles per block (softmax 1,800, two products of 512,
 // the rest hand-overs of 200 to 300 between the roles), against 2,048 cycles of products and 2,048 of
-// exponentials for both tiles: 1.14 to 1.26 PFLOP/s on long suffixes (4 x 512 queries behind 16,384 keys
-// 490 us).  Measured beside it: an issuer per tile, or one that serves whichever tile is ready, half as long
+// exponentials for both tiles: 4 x 512 queries behind 16,384 keys 470 us and 1.18 PFLOP/s in a few calls after a
+// pause, 525 to 555 us and 1.0 PFLOP/s under the power cap in hundreds of them (8 x 512: 1.27 and 1.12).  Measured beside it: an issuer per tile, or one that serves whichever tile is ready, half as long
 // again (the tiles fall into step and compete for the tensor cores); two threads per row 2% longer; S in
 // two buffers of 64 columns 40% (an MMA of 64 columns takes 57 cycles, one of 128 takes 65); a quarter of
 // the exponentials as polynomials as long or longer; only one tile in its exponentials at a time 9% longer;
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
 
 // ---------------------------------------------------------------- own keys of few queries
 // Up to 16 query rows (t, g) of a (batch row, KV head) against its own keys: bound by reading K and V once.
-// A persistent grid of two CTAs per SM; each walks its run of 64-key blocks across items without
+// A persistent grid of two CTAs per SM (where two fit); each walks its run of 64-key blocks across items without
 // draining its pipeline: one thread streams K and V tiles (TMA, 128-byte swizzle) and the items' queries
 // (bulk copies) some stages ahead, four warps take 16 keys of every block each, with their own running
 // maximum and sum, and join at the end of an item.  The products are transposed, S^T = K Q^T and
@@ -547,7 +547,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
 // share of HBM.  P^T goes from accumulator to operand layout with movmatrix.  Equal runs of blocks, with
 // two more counted per item for its queries and its end (2,100 cycles beside a block's 1,000), keep every
 // SM busy to the end whatever the lengths: 36 SMs walk 768 items of 1 to 8 blocks in 60 us, without the two
-// in 80.  On all SMs it reads 5.4 TB/s.
+// in 80.  On all SMs it reads 128 rows of 2,048 keys (8 KV heads of 128) at 6.4 TB/s, 64 rows of 64 to 1,024 keys at
+// 4.2.  Of 10 to 16 query rows of head dim 128 only one CTA fits on an SM: 64 rows of 2,048 keys are read at 4.8 to
+// 4.9 TB/s then, at 5.9 with 8 query rows.
 constexpr int OB = 64;       // keys of a block
 constexpr int OWARPS = 4;
 constexpr int ITEM = 2;  // blocks' worth of time that beginning and ending an item takes

@@ -510,7 +510,7 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
       // for all: causal tiles of all lengths fill the last wave anyway, 4,096 queries without a prefix took 3%
       // longer).  In blocks of 128 keys: a CTA takes 5 more than its keys, the join 2 and what it writes and reads.
       // 3, 4 and 5 x 512 queries behind 16K (192, 256 and 320 tiles on 148 SMs) 544 -> 405, 485 -> 480 and
-      // 731 -> 656 us.
+      // 731 -> 571 us.
       const int behind = tiles % slots;
       double best = blocks + 5;
       for (int s = 2; s <= std::min(16, blocks); ++s) {
@@ -547,8 +547,10 @@ std::vector<OptTensor> prefix_attention(Tensor q, Tensor pk, Tensor pv, Tensor k
     a.splits = splits_for(a, prefix_blocks);
   }
   if (few) {
-    // Both parts at once where that is shorter.  The lengths are not known here: half of the capacity.
-    // Times in us as measured, for head dim 128 (64).
+    // Both parts at once where that is shorter.  The lengths are not known here: half of the capacity (64 rows of 64 to
+    // 150 own keys behind 8K take 30 us at a capacity of 160, 35 at 1,280 and 39 from 4,096 on).
+    // Times in us as measured, for head dim 128 (64), with two own CTAs on an SM; of 10 to 16 query rows of head dim 128
+    // one fits, and the own part then is the longer one (64 x 2 drafts behind 4K 33 us, 64 x 3 60).
     int own_ctas = INT32_MAX;
     if (a.P > 0) {
       int tiles, slots;

@@ -28,7 +28,8 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     sees no key gives 0 and ``-inf``.  bf16, head dim 64 or 128; every view with contiguous rows,
     16-byte aligned, and a batch stride of ``k`` and ``v`` that is a multiple of their row stride.  Keys and
     values that no query sees are never used, whatever they hold; a value that one query sees and
-    another does not must be finite (its weight is 0 there).  No gradients.
+    another does not must be finite (its weight is 0 there).  Scores, maxima and sums are fp32; each softmax weight
+    is rounded to bf16 where it meets its value.  No gradients.
     """
     out, lse = require().shared_prefix_attention(q, prefix_k, prefix_v, k, v, lengths, heads, kv_heads, head_dim,
                                                  prefix_lengths, 1.0 / math.sqrt(head_dim) if scale is None else scale,
