@@ -22,12 +22,13 @@
 //
 // What bounds it: a tile's chain of about 3,200 cycles per block (softmax 1,800, two products of 512,
 // the rest hand-overs of 200 to 300 between the roles), against 2,048 cycles of products and 2,048 of
-// exponentials for both tiles: 4 x 512 queries behind 16,384 keys 470 us and 1.18 PFLOP/s in a few calls after a
-// pause, 525 to 555 us and 1.0 PFLOP/s under the power cap in hundreds of them (8 x 512: 1.27 and 1.12).  Measured beside it: an issuer per tile, or one that serves whichever tile is ready, half as long
-// again (the tiles fall into step and compete for the tensor cores); two threads per row 2% longer; S in
-// two buffers of 64 columns 40% (an MMA of 64 columns takes 57 cycles, one of 128 takes 65); a quarter of
-// the exponentials as polynomials as long or longer; only one tile in its exponentials at a time 9% longer;
-// 224 registers for the softmax warps (setmaxnreg, with two idle warps) 2% longer.
+// exponentials for both tiles: 4 x 512 queries behind 16,384 keys 470 us and 1.18 PFLOP/s in a few calls
+// after a pause, 525 to 555 us and 1.0 PFLOP/s under the power cap in hundreds of them (8 x 512: 1.27
+// and 1.12).  Measured beside it: an issuer per tile, or one that serves whichever tile is ready, half
+// as long again (the tiles fall into step and compete for the tensor cores); two threads per row 2%
+// longer; S in two buffers of 64 columns 40% (an MMA of 64 columns takes 57 cycles, one of 128 takes
+// 65); a quarter of the exponentials as polynomials as long or longer; only one tile in its exponentials
+// at a time 9% longer; 224 registers for the softmax warps (setmaxnreg, with two idle warps) 2% longer.
 //
 // Keys past the ones any query of the CTA may see are never multiplied: their scores are replaced by
 // -inf, and their value rows are zeroed in shared memory (a stale row may hold NaN, and 0 * NaN is

@@ -112,8 +112,8 @@ def test_history_behind_a_shared_prefix():
     assert alone.ids.tolist() == [[5, 6, 0]] and alone.lengths.tolist() == [2]
 
 
-def test_a_prefix_that_was_not_finished_is_none(monkeypatch):
-    """An exception while the second chunk is encoded: the engine has no prefix, not half of one."""
+def prefix_engine(monkeypatch, rotary_cache):
+    """An engine without kernels: ``set_shared_prefix`` runs, every layer leaves its input alone."""
     from types import SimpleNamespace
 
     from pdattention_b200.inference import llama_engine
@@ -127,27 +127,52 @@ def test_a_prefix_that_was_not_finished_is_none(monkeypatch):
     engine.prefix = engine.prefix_ids = engine.cache = None
     engine._rope_cache = {}
     engine.w = SimpleNamespace(layers=[SimpleNamespace(ln_in=None, qkv=None, qkv_bias=None, o=None)] * cfg.num_hidden_layers)
+    monkeypatch.setattr(llama_engine, "rotary_cache", rotary_cache)
+    monkeypatch.setattr(llama_engine, "shared_prefix_attention", lambda q, *a: q)
+    engine._norm = engine._row_parallel = lambda x, *a, **kw: x
+    engine._gemm = lambda x, *a, **kw: torch.zeros(x.shape[0], cfg.q_dim + 2 * cfg.kv_dim)
+    engine._mlp = lambda lw, x: x
+    engine._ln = lambda w: None
+    engine._embed = lambda ids: torch.zeros(ids.numel(), cfg.hidden_size)
+    return engine
+
+
+def test_a_prefix_that_was_not_finished_is_none(monkeypatch):
+    """An exception while the second chunk is encoded: the engine has no prefix, not half of one."""
     calls = []
 
     def rotary_cache(qkv, heads, kv_heads, head_dim, pos, table, k, v, rows):
         calls.append(int(rows[0]))
         if rows[0] >= 10:
             raise torch.OutOfMemoryError("no room")
-        return qkv[:, : cfg.q_dim]
+        return qkv[:, : heads * head_dim]
 
-    monkeypatch.setattr(llama_engine, "rotary_cache", rotary_cache)
-    monkeypatch.setattr(llama_engine, "shared_prefix_attention", lambda q, *a: q)
-    rows = lambda x, *a, **kw: torch.zeros(x.shape[0], cfg.q_dim + 2 * cfg.kv_dim)  # noqa: E731
-    for name in ("_norm", "_gemm", "_row_parallel", "_mlp"):
-        setattr(engine, name, (lambda x, *a, **kw: x) if name != "_gemm" else rows)
-    engine._mlp = lambda lw, x: x
-    engine._ln = lambda w: None
-    engine._embed = lambda ids: torch.zeros(ids.numel(), cfg.hidden_size)
+    engine = prefix_engine(monkeypatch, rotary_cache)
     with pytest.raises(torch.OutOfMemoryError):
         engine.set_shared_prefix(torch.arange(25), chunk_tokens=10)
     assert max(calls) == 10 and engine.prefix is None and engine.prefix_ids is None and engine.prefix_tokens == 0
     engine.set_shared_prefix(torch.arange(9), chunk_tokens=10)
     assert engine.prefix_tokens == 9 and engine.prefix_ids.tolist() == list(range(9))
+
+
+@pytest.mark.parametrize("chunk,room,size", [(10, 7, 7), (5, 7, 5), (4096, 0, 1)])
+def test_prefix_chunks_fit_the_tensor_parallel_buffer(monkeypatch, chunk, room, size):
+    """A chunk's row-parallel partials fit the peer buffer (one row at least)."""
+    from types import SimpleNamespace
+
+    chunks = []
+
+    def rotary_cache(qkv, heads, kv_heads, head_dim, pos, table, k, v, rows):
+        assert torch.equal(pos, rows)  # unscaled: a token's position is its row
+        chunks.append(rows.tolist())
+        return qkv[:, : heads * head_dim]
+
+    engine = prefix_engine(monkeypatch, rotary_cache)
+    engine.tp = SimpleNamespace(max_partial=room * engine.cfg.hidden_size + engine.cfg.hidden_size - 1)
+    engine.set_shared_prefix(torch.arange(17), chunk_tokens=chunk)
+    layers = engine.cfg.num_hidden_layers
+    assert all(c == list(range(i // layers * size, min(17, (i // layers + 1) * size))) for i, c in enumerate(chunks))
+    assert len(chunks) == -(-17 // size) * layers and engine.prefix_tokens == 17
 
 
 @needs_ext
