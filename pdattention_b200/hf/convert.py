@@ -21,6 +21,8 @@ def config_from_hf(hf_config, **pra) -> PRALlamaConfig:
     scaling = None
     if rope.get("rope_type", rope.get("type", "default")) != "default":
         scaling = rope  # an unknown kind of scaling is refused by the configuration
+        if rope.get("rope_type", rope.get("type")) == "dynamic":  # there the window is the model's, whatever else is given
+            scaling["original_max_position_embeddings"] = hf_config.max_position_embeddings
         scaling.setdefault("original_max_position_embeddings", hf_config.max_position_embeddings)
     head_dim = getattr(hf_config, "head_dim", None) or hf_config.hidden_size // heads
     return PRALlamaConfig(

@@ -35,7 +35,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops.rotary import rotary_angles, rotary_frequencies
+from ..ops.rotary import dynamic_window, rotary_angles, rotary_frequencies
 
 _FAMILIES = ("llama", "mistral", "qwen2")
 
@@ -456,6 +456,10 @@ def hf_config(cfg: PRALlamaConfig):
                   tie_word_embeddings=cfg.tie_word_embeddings)
     if cfg.rope_scaling:
         common["rope_scaling"] = dict(cfg.rope_scaling)
+        window = dynamic_window(cfg.rope_scaling)
+        if window is not None:  # Hugging Face takes the model's positions for it
+            common["max_position_embeddings"] = window
+            del common["rope_scaling"]["original_max_position_embeddings"]
     if cfg.family == "qwen2":
         return transformers.Qwen2Config(**common)
     if cfg.family == "mistral":

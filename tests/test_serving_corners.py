@@ -298,3 +298,28 @@ def test_rows_of_nothing_but_the_prefix_are_refused():
     for ids, n in ((torch.zeros(3, 4), [4, 0, 1]), (torch.zeros(1, 0), [0]), (torch.zeros(2, 1), [1, -1])):
         with pytest.raises(ValueError, match="token of its own"):
             engine.prefill(ids.long(), torch.tensor(n), 4)
+
+
+def test_the_window_of_dynamic_scaling_to_and_from_hugging_face():
+    """Hugging Face has no original window for it: ``max_position_embeddings`` is the window."""
+    import transformers
+
+    from pdattention_b200.hf.convert import config_from_hf
+    from pdattention_b200.models.llama import PRALlamaReference, hf_config, tiny_llama
+
+    hcfg = transformers.LlamaConfig(hidden_size=64, num_attention_heads=4, head_dim=16, max_position_embeddings=128, rope_parameters={
+        "rope_type": "dynamic", "factor": 4.0, "rope_theta": 1e4, "original_max_position_embeddings": 32})
+    assert config_from_hf(hcfg).rope_scaling["original_max_position_embeddings"] == 128
+    cfg = tiny_llama(max_position_embeddings=128, rope_scaling={"rope_type": "dynamic", "factor": 4.0,
+                                                                "original_max_position_embeddings": 32})
+    ours = PRALlamaReference(cfg).eval()
+    ours.reset_parameters(seed=0, std=0.2)
+    hcfg = hf_config(cfg)
+    hcfg._attn_implementation = "eager"
+    hf = transformers.LlamaForCausalLM(hcfg).eval()
+    hf.load_state_dict(ours.state_dict(), strict=False)
+    ids = torch.randint(0, cfg.vocab_size, (1, 100), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():  # tolerance as above
+        assert torch.allclose(ours(ids), hf(ids).logits, atol=2e-3, rtol=1e-3)
+    assert cfg.rope_scaling["original_max_position_embeddings"] == 32
+    assert config_from_hf(hcfg).rope_scaling["original_max_position_embeddings"] == 32
